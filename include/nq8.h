@@ -48,6 +48,7 @@ extern "C" {
 #define NQ_ERR_NOT_INIT (-9)    /* nq_init was not called on this thread's device */
 #define NQ_ERR_UNSUPPORTED (-10)/* e.g. GLU epilogue on a weight not packed for it */
 #define NQ_ERR_DEVICE (-11)     /* device status word reported a kernel-side error */
+#define NQ_ERR_CACHE (-12)      /* nq_cache_status: a call on the cache could not be done */
 
 /* ---- element types of activations / outputs ---------------------------- */
 #define NQ_F32 0
@@ -306,6 +307,154 @@ int nq_conv_transpose1d_weight(const float *w, int64_t c_in, int64_t c_out, int 
 int nq_conv_transpose1d(const nq_weight *w, const void *x, int x_dtype, int64_t c_in, int64_t t_in, int64_t ldx,
                         int kernel, int stride, int padding, int output_padding, float x_leaky, const float *bias,
                         int epilogue, void *y, int y_dtype, int64_t ldy, void *stream);
+
+/* ---- decoding: attention, the paged cache, beam search ---------------------
+ * What a decoder step needs between its projections: attention over the past
+ * (the reference's flash_attention_fwd with its sliding window and
+ * attention_decode, kernels/moonshine_kernels.py:749-845,1457-1718, called by
+ * DecoderBackend::self_attention / cross_attention,
+ * src/moonshine/gpu_decoder.rs:21-88, and by the encoder,
+ * src/moonshine/encoder.rs:116-135), the cache it reads (kv_cache_append) and
+ * the choice of the next tokens (argmax_logits, src/moonshine/
+ * gpu_decoder_metal.rs:110-243; beam_decode, src/parakeet/transducer.rs:1116).
+ * Common rules:
+ *   - All arrays are the caller's device memory; nothing is allocated and
+ *     nothing is kept between calls, so every call may be captured into a
+ *     graph from its first time on.  A workspace belongs to its call until the
+ *     call has run: calls (and graphs) that may run at the same time need
+ *     different ones.
+ *   - dtype is NQ_F32 or NQ_BF16, the same for all rows of a call.  Scores,
+ *     softmax maxima and sums and output sums are f32; with bf16 rows the
+ *     softmax weights are rounded to bf16 for the tensor cores.
+ *   - Sequences are ragged: `offsets` (device int32 [n + 1], ascending) gives
+ *     the rows of each; NULL: the same number of rows each.  Rows that belong
+ *     to no sequence are neither read nor written.  Offsets and lengths are
+ *     clamped to the rows there are. */
+
+/* Rows [token][head][head_dim]; unit stride within a head, the others in
+ * elements.  Rows on 16 bytes (address, strides, head_dim) load fastest. */
+typedef struct nq_rows {
+  void *ptr;
+  int64_t token_stride;
+  int64_t head_stride;
+} nq_rows;
+
+/* out_i = sum over j of softmax_j(scale q_i . k_j) v_j over the keys that
+ * query i sees.  Of a sequence with n_q queries and n_k keys, query i stands
+ * at position p = n_k - n_q + i (its queries are its last tokens) and sees key
+ * j when  j <= p + right  and  (j >= p - left  or  j < sinks)  -- a sliding
+ * window and the first tokens, which stay visible.  left, right < 0: no limit
+ * (left = -1, right = 0 is causal attention, both -1 full attention).  A query
+ * that sees nothing gives zeros.  Query head h reads kv head
+ * h / (q_heads / kv_heads).  head_dim 1 to 128.  q_lens / k_lens (device int32
+ * [seqs] or NULL): only the first rows of each sequence's span count (padded
+ * batches); k_offsets / q_offsets NULL: k_rows / seqs (q_rows / seqs) rows
+ * each.  K and V rows that no query of the call sees may hold anything; those
+ * that one sees should be finite (a weight of 0 times an infinity is NaN).
+ * out must not overlap the inputs.  workspace (16-byte aligned, at least
+ * nq_window_attention_workspace bytes; NULL: none) lets few query rows over
+ * many keys be split over more of the GPU; results then differ by f32
+ * summation order.  Deterministic. */
+int64_t nq_window_attention_workspace(int dtype, int seqs, int64_t q_rows, int64_t k_rows, int q_heads, int kv_heads,
+                                      int head_dim, int left, int right, int sinks);
+int nq_window_attention(const nq_rows *q, const nq_rows *k, const nq_rows *v, const nq_rows *out, int dtype, int seqs,
+                        int64_t q_rows, int64_t k_rows, const int32_t *q_offsets, const int32_t *k_offsets,
+                        const int32_t *q_lens, const int32_t *k_lens, int q_heads, int kv_heads, int head_dim, int left,
+                        int right, int sinks, float scale, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* A key / value cache in pages, with all its bookkeeping on the device.  A
+ * slot holds one sequence: its length and the pages of its tokens in order;
+ * pages that several slots hold are counted.  Start with table = -1, lens =
+ * refs = state = 0.  Calls on one cache follow one another on the GPU (one
+ * stream, or events between); attention calls may run side by side.
+ * A call that cannot be done (no free pages, a slot at max_pages, an index out
+ * of range) changes nothing and sets a status bit; the cache's calls then do
+ * nothing until nq_cache_status has reported it.  nq_cache_write may have
+ * written some of its rows by then. */
+typedef struct nq_cache {
+  void *k, *v;      /* [layers][pages][kv_heads][page_tokens][head_dim], 16-byte aligned */
+  int32_t *table;   /* [slots][max_pages] page of each page_tokens tokens, -1: none */
+  int32_t *lens;    /* [slots] tokens */
+  int32_t *refs;    /* [pages] slots that hold the page, 0: free */
+  int32_t *state;   /* [nq_cache_state_ints(slots, pages)] status and scratch */
+  int dtype;        /* NQ_F32 | NQ_BF16 */
+  int layers, pages, page_tokens; /* page_tokens: a power of two, 8 to 1024; pages up to 2^20 */
+  int kv_heads, head_dim;         /* head_dim 1 to 128 */
+  int slots, max_pages;           /* max_pages * page_tokens up to 2^30 */
+} nq_cache;
+#define NQ_CACHE_OUT_OF_PAGES 0x1
+#define NQ_CACHE_SLOT_FULL 0x2
+#define NQ_CACHE_BAD_INDEX 0x4
+#define NQ_CACHE_SHARED_PAGE 0x8
+int64_t nq_cache_state_ints(int slots, int pages);
+
+/* Room for new tokens of slots [first, first + n) (at most 4096 a call):
+ * offsets[i + 1] - offsets[i] more for slot first + i, or `tokens` for each
+ * with offsets NULL.  Pages are taken lowest number first in the order of the
+ * slots.  A partly filled last page that other slots hold too is copied first
+ * (its tokens, in every layer), except by the last of its holders when all of
+ * them get tokens in this call.  Two launches. */
+int nq_cache_reserve(const nq_cache *c, int first, int n, const int32_t *offsets, int tokens, void *stream);
+
+/* The keys and values of the last reserved tokens: row offsets[i] + t is token
+ * lens[first + i] - (offsets[i + 1] - offsets[i]) + t of slot first + i.  k, v
+ * hold `rows` rows for each of `layers` layers from `layer` on, *_layer_stride
+ * elements apart. */
+int nq_cache_write(const nq_cache *c, const nq_rows *k, const nq_rows *v, int64_t k_layer_stride, int64_t v_layer_stride,
+                   int layer, int layers, int64_t rows, int first, int n, const int32_t *offsets, int tokens, void *stream);
+
+/* nq_window_attention over the cache's layer `layer`: sequence i is slot first + i
+ * with all its tokens as keys and the rows of q between offsets[i] and
+ * offsets[i + 1] as its last tokens' queries.  A key whose page is gone
+ * (nq_cache_trim) is not seen.  Single tokens (offsets NULL, q_rows = n) and
+ * whole chunks of a prompt alike. */
+int64_t nq_cache_attention_workspace(const nq_cache *c, int seqs, int64_t q_rows, int q_heads, int left, int right, int sinks);
+int nq_cache_attention(const nq_cache *c, int layer, const nq_rows *q, const nq_rows *out, int first, int n, int64_t q_rows,
+                       const int32_t *offsets, int q_heads, int left, int right, int sinks, float scale, void *workspace,
+                       int64_t workspace_bytes, void *stream);
+
+/* Slots [first, first + n) become what slots src[i] (device int32 [n]) were
+ * before the call; -1, or src NULL, frees.  The pages are shared, not copied;
+ * sources may repeat and may be among the slots written. */
+int nq_cache_fork(const nq_cache *c, int first, int n, const int32_t *src, void *stream);
+
+/* Gives back the pages of slots [first, first + n) that hold neither one of
+ * the first `sinks` tokens nor one of the last `window`: those that attention
+ * with left <= window and these sinks sees no more from the next token on. */
+int nq_cache_trim(const nq_cache *c, int first, int n, int sinks, int window, void *stream);
+
+/* Moves the live pages numbered at or above their count into the free ones
+ * below it, both in ascending order, and renumbers the tables: afterwards
+ * pages [0, live) are live and the rest is free.  state[1] = live. */
+int nq_cache_compact(const nq_cache *c, void *stream);
+
+/* Synchronizes `stream`, then reads and clears the cache's status: NQ_OK, or
+ * NQ_ERR_CACHE with the NQ_CACHE_* bits in *bits (may be NULL). */
+int nq_cache_status(const nq_cache *c, int *bits, void *stream);
+
+/* One step of beam search.  Row b * beams + k of logits ([items * beams] rows,
+ * ld elements apart) and scores[b * beams + k] belong to beam k of item b.
+ * Candidates: every token t of an unfinished beam with
+ *   scores + logits[t] - log sum_u exp(logits[u]),
+ * and of a finished beam the token `eos` alone with its score unchanged.  The
+ * `beams` best of each item, best first, equal ones by beam, then token (a
+ * beam's own by logit, then token): their scores, the rows they come from
+ * (out_parents, of all items' rows: what nq_cache_fork and nq_beam_reorder
+ * take), tokens, and whether they are finished (out_finished, may be NULL).
+ * NaN and +inf logits count as -inf, as does a NaN score; a candidate of score
+ * -inf is taken only after all others.  finished may be NULL; beams up to 32.
+ * Outputs may be the inputs of the same kind.  Two launches. */
+int64_t nq_beam_workspace(int items, int beams, int64_t vocab);
+int nq_beam_select(const void *logits, int dtype, int64_t ld, int items, int beams, int64_t vocab, const float *scores,
+                   const uint8_t *finished, int eos, float *out_scores, int32_t *out_parents, int32_t *out_tokens,
+                   uint8_t *out_finished, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* dst[i][r] = src[i][parents[r]] for up to 16 states of `rows` rows (up to
+ * 12288): row_bytes[i] bytes, src_stride[i] and dst_stride[i] bytes apart.  A
+ * parent out of range leaves its row.  dst[i] may be src[i] (with the same
+ * stride), and otherwise overlaps no state.  One launch. */
+int nq_beam_reorder(const void *const *src, void *const *dst, const int64_t *row_bytes, const int64_t *src_stride,
+                    const int64_t *dst_stride, int count, int rows, const int32_t *parents, void *stream);
 
 /* ---- FastConformer encoder (the caller of the Q8_0 path for configs 2/5) ---
  * Mirrors FastConformerConfig (src/parakeet/fast_conformer.rs:31-45) and

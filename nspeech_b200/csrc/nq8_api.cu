@@ -1130,6 +1130,15 @@ int linear_launches(const nq_weight *w, int64_t m, int x_dtype, bool aligned) {
   return plan_gemm(sm, w, m, x_dtype, x_dtype == NQ_BF16 && aligned).launches();
 }
 
+int device_info(int *sm_count, DevCtl *ctl) {
+  DeviceCtx *ctx = nullptr;
+  const int rc = current_ctx(&ctx, nullptr);
+  if (rc) return rc;
+  *sm_count = ctx->sm_count;
+  if (ctl) *ctl = DevCtl{ctx->status, g_wait_limit};
+  return NQ_OK;
+}
+
 bool attention_tc(int Tp) { return g_attention_kernel == NQ_ATTENTION_TCGEN05 && Tp <= attention_tc_max_tp(); }
 
 int layer_norm_rows(int mode, float *x, const void *u, float alpha, int rows, int D, const float *g1, const float *b1,

@@ -1,0 +1,496 @@
+// nq8_cache.cu -- the pages of a key / value cache: room for new tokens,
+// forking, copying on write, freeing, compacting, and the tokens' entry.
+//
+// A slot's sequence is a row of page numbers and a length; pages carry a count
+// of the slots that hold them.  All of it lives on the device and every call
+// is a fixed number of launches, so a decoding step can be captured into a
+// graph.  Results depend on the order of slots alone: pages are given out
+// lowest number first, and counts are integers, so atomics' order is not seen.
+// A call that cannot be done changes nothing and sets a status bit; later
+// calls then do nothing until the host has read the status.
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "nq8_cache.h"
+
+namespace nq {
+namespace {
+
+constexpr int kBlock = 1024;
+
+__device__ __forceinline__ int *copies_of(const CacheView &c) { return c.state + kStateLists; }
+__device__ __forceinline__ int *list_of(const CacheView &c, int i) {
+  return c.state + kStateLists + 3 * static_cast<int64_t>(c.slots) + i * static_cast<int64_t>(c.pages);
+}
+
+// Exclusive prefix sum over the block (kBlock threads); all: the total.
+__device__ __forceinline__ int block_scan(int x, int *warp_sums, int &all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int upto = x;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += y;
+  }
+  __syncthreads();  // the previous scan's sums are read
+  if (lane == 31) warp_sums[warp] = upto;
+  __syncthreads();
+  int w = warp_sums[lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += y;
+  }
+  all = __shfl_sync(0xffffffffu, w, 31);
+  const int before = __shfl_sync(0xffffffffu, w, warp > 0 ? warp - 1 : 0);
+  return upto - x + (warp > 0 ? before : 0);
+}
+
+// Tokens that slot i of a call gets: offsets[i + 1] - offsets[i], or `uniform`.
+__device__ __forceinline__ int count_of(const int *offsets, int uniform, int i) {
+  return offsets ? max(0, __ldg(offsets + i + 1) - __ldg(offsets + i)) : uniform;
+}
+
+// One bit per page, set where refs > 0, by whole warps.
+__device__ __forceinline__ void held_bits(const CacheView &c, uint32_t *bits) {
+  const int lane = threadIdx.x & 31;
+  const int words = (c.pages + 31) / 32;
+  constexpr int U = 8;  // loads in flight a thread
+  for (int w = (threadIdx.x >> 5) * U; w < words; w += kBlock / 32 * U) {
+    int r[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int page = (w + u) * 32 + lane;
+      r[u] = page < c.pages ? c.refs[page] : 1;  // past the end: not free
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t m = __ballot_sync(0xffffffffu, r[u] > 0);
+      if (lane == 0 && w + u < words) bits[w + u] = m;
+    }
+  }
+}
+
+// Room for the new tokens of slots [first, first + n): one CTA.
+// Shared: held bits of all pages, and per slot its shared last page (-1: none,
+// or it may keep it) and the rank of its first new page.
+__global__ void __launch_bounds__(kBlock) cache_reserve_kernel(const CacheView c, const int *__restrict__ offsets, int uniform,
+                                                               int first, int n) {
+  extern __shared__ uint32_t sh[];
+  __shared__ int sums[32];
+  __shared__ int bad, copies;
+  const int words = (c.pages + 31) / 32;
+  uint32_t *bits = sh;
+  int *tail = reinterpret_cast<int *>(sh + words), *start = tail + n;
+  pdl_wait();
+  pdl_trigger();
+  if (c.state[kStateStatus]) {
+    if (threadIdx.x == 0) c.state[kStateCopies] = 0;
+    return;
+  }
+  const int P = 1 << c.page_shift;
+  const int64_t room = static_cast<int64_t>(c.max_pages) << c.page_shift;
+  if (threadIdx.x == 0) bad = copies = 0;
+  held_bits(c, bits);
+  for (int i = threadIdx.x; i < n; i += kBlock) {
+    const int old = c.lens[first + i], add = count_of(offsets, uniform, i);
+    int t = -1;
+    if (add > 0 && (old & (P - 1)) && old > 0 && old <= room) {
+      t = c.table[static_cast<int64_t>(first + i) * c.max_pages + (old >> c.page_shift)];
+      if (t < 0 || t >= c.pages || c.refs[t] <= 1) t = -1;  // a page of its own
+    }
+    tail[i] = t;
+  }
+  __syncthreads();
+  // The pages that each slot takes, in the slots' order.
+  int total = 0;
+  for (int base = 0; base < n; base += kBlock) {
+    const int i = base + threadIdx.x;
+    int need = 0, copy = 0;
+    if (i < n) {
+      const int old = c.lens[first + i], add = count_of(offsets, uniform, i), t = tail[i];
+      if (t >= 0) {
+        // the last holder keeps the page where every holder of it appends
+        int same = 0, later = 0;
+        for (int j = 0; j < n; ++j) {
+          const int e = tail[j] == t;
+          same += e;
+          later |= e && j > i;
+        }
+        copy = c.refs[t] != same || later;
+      }
+      if (old < 0 || old + static_cast<int64_t>(add) > room) {
+        bad = kCacheSlotFull;
+      } else {
+        need = ((old + add + P - 1) >> c.page_shift) - ((old + P - 1) >> c.page_shift) + copy;
+        need = min(need, c.pages + 1);  // more than there are: the block's sum stays in range
+      }
+    }
+    int all;
+    const int at = block_scan(need, sums, all);
+    if (i < n) start[i] = ((total + at) << 1) | copy;
+    total += all;
+    if (total > c.pages) total = c.pages + 1;  // cannot be met; keeps the sum in range
+  }
+  int free_pages = 0;
+  {
+    int mine = 0, all;
+    for (int w = threadIdx.x; w < words; w += kBlock) mine += __popc(~bits[w]);
+    block_scan(mine, sums, all);
+    free_pages = all;
+  }
+  __syncthreads();
+  if (bad || total > free_pages) {
+    if (threadIdx.x == 0) {
+      c.state[kStateStatus] = bad ? bad : kCacheOutOfPages;
+      c.state[kStateCopies] = 0;
+    }
+    return;
+  }
+  // The `total` lowest free pages in order.
+  int *list = list_of(c, 0);
+  for (int base = 0, done = 0; base < words && done < total; base += kBlock) {
+    const int w = base + threadIdx.x;
+    uint32_t m = w < words ? ~bits[w] : 0u;
+    int all;
+    int at = done + block_scan(__popc(m), sums, all);
+    for (; m && at < total; m &= m - 1) list[at++] = w * 32 + __ffs(m) - 1;
+    done += all;
+  }
+  __syncthreads();
+  int *cp = copies_of(c);
+  const int lane = threadIdx.x & 31;
+  for (int i = threadIdx.x >> 5; i < n; i += kBlock / 32) {
+    const int old = c.lens[first + i], add = count_of(offsets, uniform, i), copy = start[i] & 1, at = start[i] >> 1;
+    const int have = (old + P - 1) >> c.page_shift, want = (old + add + P - 1) >> c.page_shift;
+    int *row = c.table + static_cast<int64_t>(first + i) * c.max_pages;
+    for (int x = lane; x < want - have + copy; x += 32) {
+      const int page = list[at + x];
+      c.refs[page] = 1;
+      if (copy && x == 0) {
+        const int e = atomicAdd(&copies, 1);
+        cp[3 * e] = tail[i];
+        cp[3 * e + 1] = page;
+        cp[3 * e + 2] = old & (P - 1);
+        atomicSub(c.refs + tail[i], 1);
+        row[old >> c.page_shift] = page;
+      } else {
+        row[have + x - copy] = page;
+      }
+    }
+    __syncwarp();
+    if (lane == 0) c.lens[first + i] = old + add;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) c.state[kStateCopies] = copies;
+}
+
+// The copied last pages: entry blockIdx.x of the list, layer and side of
+// blockIdx.y, the first rows of each head's part of the page.
+template <typename T>
+__global__ void __launch_bounds__(128) cache_copy_kernel(const CacheView c) {
+  pdl_wait();
+  pdl_trigger();
+  if (c.state[kStateStatus]) return;
+  const int n = c.state[kStateCopies];
+  const int layer = blockIdx.y >> 1;
+  char *pool = static_cast<char *>(blockIdx.y & 1 ? c.v : c.k);
+  const int64_t head_bytes = (static_cast<int64_t>(c.dim) << c.page_shift) * c.size;
+  const int64_t page_bytes = head_bytes * c.kv_heads;
+  for (int e = blockIdx.x; e < n; e += gridDim.x) {
+    const int *cp = copies_of(c) + 3 * e;
+    const int units = cp[2] * c.dim * c.size / static_cast<int>(sizeof(T));  // of one head
+    const char *src = pool + (static_cast<int64_t>(layer) * c.pages + cp[0]) * page_bytes;
+    char *dst = pool + (static_cast<int64_t>(layer) * c.pages + cp[1]) * page_bytes;
+    for (int x = threadIdx.x; x < units * c.kv_heads; x += blockDim.x) {
+      const int h = x / units;
+      const int64_t o = h * head_bytes + static_cast<int64_t>(x - h * units) * sizeof(T);
+      *reinterpret_cast<T *>(dst + o) = *reinterpret_cast<const T *>(src + o);
+    }
+  }
+}
+
+// New tokens into their places: 16 rows of one layer a CTA.  Within a head a
+// page's rows are adjacent, so the threads go along rows first.
+constexpr int kWriteRows = 16;
+template <typename T>
+__global__ void __launch_bounds__(256) cache_write_kernel(const CacheView c, const char *__restrict__ k, const char *__restrict__ v,
+                                                          int64_t k_ts, int64_t k_hs, int64_t k_ls, int64_t v_ts, int64_t v_hs,
+                                                          int64_t v_ls, int layer0, int rows, const int *__restrict__ offsets,
+                                                          int uniform, int first, int n) {
+  __shared__ int64_t place[kWriteRows];  // page row of head 0 (in rows of `dim`), -1: none
+  pdl_wait();
+  pdl_trigger();
+  if (c.state[kStateStatus]) return;
+  const int row0 = blockIdx.x * kWriteRows, layer = blockIdx.y;
+  if (threadIdx.x < kWriteRows) {
+    const int r = row0 + threadIdx.x;
+    int64_t at = -1;
+    int fault = 0;
+    if (r < rows) {
+      int i, begin, end;
+      if (offsets) {
+        int lo = 0, hi = n;  // the last i with offsets[i] <= r
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) / 2;
+          if (__ldg(offsets + mid) <= r) lo = mid;
+          else hi = mid;
+        }
+        i = lo;
+        begin = __ldg(offsets + i);
+        end = __ldg(offsets + i + 1);
+      } else {
+        i = uniform > 0 ? r / uniform : n;
+        begin = i * uniform;
+        end = begin + uniform;
+      }
+      if (i < n && r >= begin && r < end) {
+        const int64_t pos = c.lens[first + i] - static_cast<int64_t>(end - r);
+        fault = kCacheBadIndex;
+        if (pos >= 0 && pos < static_cast<int64_t>(c.max_pages) << c.page_shift) {
+          const int page = c.table[static_cast<int64_t>(first + i) * c.max_pages + (pos >> c.page_shift)];
+          if (page >= 0 && page < c.pages) {
+            fault = c.refs[page] == 1 ? 0 : kCacheSharedPage;
+            if (!fault) at = (static_cast<int64_t>(page) * c.kv_heads << c.page_shift) + (pos & ((1 << c.page_shift) - 1));
+          }
+        }
+      }
+    }
+    place[threadIdx.x] = at;
+    if (fault) atomicOr(c.state + kStateStatus, fault);
+  }
+  __syncthreads();
+  const int units = c.dim * c.size / static_cast<int>(sizeof(T));  // of a row of one head
+  const int64_t base = static_cast<int64_t>(layer0 + layer) * c.pages * c.kv_heads << c.page_shift;
+  const int row_bytes = c.dim * c.size;
+  for (int x = threadIdx.x; x < units * kWriteRows * c.kv_heads; x += blockDim.x) {
+    const int u = x % units, r = x / units % kWriteRows, h = x / (units * kWriteRows);
+    if (place[r] < 0) continue;
+    const int64_t to = (base + place[r] + (static_cast<int64_t>(h) << c.page_shift)) * row_bytes + u * sizeof(T);
+    const int64_t tok = row0 + r;
+    *reinterpret_cast<T *>(static_cast<char *>(c.k) + to) =
+        *reinterpret_cast<const T *>(k + (layer * k_ls + tok * k_ts + h * k_hs) * c.size + u * sizeof(T));
+    *reinterpret_cast<T *>(static_cast<char *>(c.v) + to) =
+        *reinterpret_cast<const T *>(v + (layer * v_ls + tok * v_ts + h * v_hs) * c.size + u * sizeof(T));
+  }
+}
+
+// Slots [first, first + n) become what the slots src[i] were.  A CTA owns a
+// few columns of the table for all n rows and reads them before it writes
+// any, so sources may be among the rows written and repeat.
+__global__ void __launch_bounds__(256) cache_fork_kernel(const CacheView c, const int *__restrict__ src, int first, int n, int cols) {
+  extern __shared__ int fork_sh[];  // [n][cols]
+  pdl_wait();
+  pdl_trigger();
+  if (c.state[kStateStatus]) return;
+  const int col0 = blockIdx.x * cols;
+  const int width = min(cols, c.max_pages - col0);
+  const bool lens_too = blockIdx.x == gridDim.x - 1;  // one more CTA moves the lengths
+  auto source = [&](int i) { return src ? __ldg(src + i) : -1; };
+  // Every CTA looks at all sources, so that a bad one leaves all columns alone.
+  int wrong = 0;
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    const int f = source(i);
+    wrong |= f < -1 || f >= c.slots;
+  }
+  if (__syncthreads_or(wrong)) {
+    if (lens_too && threadIdx.x == 0) atomicOr(c.state + kStateStatus, kCacheBadIndex);
+    return;
+  }
+  if (lens_too) {
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+      const int f = source(i);
+      fork_sh[i] = f < 0 ? 0 : c.lens[f];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += blockDim.x) c.lens[first + i] = fork_sh[i];
+    return;
+  }
+  for (int x = threadIdx.x; x < n * cols; x += blockDim.x) {
+    const int i = x / cols, col = x % cols, f = source(i);
+    fork_sh[x] = f < 0 || col >= width ? -1 : c.table[static_cast<int64_t>(f) * c.max_pages + col0 + col];
+  }
+  __syncthreads();
+  for (int x = threadIdx.x; x < n * cols; x += blockDim.x) {
+    const int i = x / cols, col = x % cols;
+    if (col >= width) continue;
+    int *e = c.table + static_cast<int64_t>(first + i) * c.max_pages + col0 + col;
+    const int was = *e, is = fork_sh[x];
+    if (was == is) continue;
+    if (is >= 0 && is < c.pages) atomicAdd(c.refs + is, 1);
+    if (was >= 0 && was < c.pages) atomicSub(c.refs + was, 1);
+    *e = is;
+  }
+}
+
+// Pages that hold neither one of the first `sinks` tokens nor one of the last
+// `window` of their slot are given back.
+__global__ void __launch_bounds__(128) cache_trim_kernel(const CacheView c, int first, int sinks, int window) {
+  pdl_wait();
+  pdl_trigger();
+  if (c.state[kStateStatus]) return;
+  const int slot = first + blockIdx.x, P = 1 << c.page_shift;
+  const int len = c.lens[slot];
+  const int lo = (sinks + static_cast<int64_t>(P) - 1) >> c.page_shift;
+  const int hi = len > window ? min((len - window) >> c.page_shift, c.max_pages) : 0;  // pages [lo, hi) lie between
+  for (int col = lo + threadIdx.x; col < hi; col += blockDim.x) {
+    int *e = c.table + static_cast<int64_t>(slot) * c.max_pages + col;
+    const int was = *e;
+    if (was >= 0 && was < c.pages) atomicSub(c.refs + was, 1);
+    *e = -1;
+  }
+}
+
+// Which pages move: the live ones at or above their count, in order, into the
+// free ones below it.  list 0: moved pages, list 1: their places, list 2: the
+// place of each moved page.
+__global__ void __launch_bounds__(kBlock) cache_plan_kernel(const CacheView c) {
+  extern __shared__ uint32_t bits[];
+  __shared__ int sums[32];
+  pdl_wait();
+  pdl_trigger();
+  if (c.state[kStateStatus]) {
+    if (threadIdx.x == 0) c.state[kStateCopies] = 0;
+    return;
+  }
+  const int words = (c.pages + 31) / 32;
+  held_bits(c, bits);
+  __syncthreads();
+  auto held = [&](int w) {  // without the bits past the last page
+    const uint32_t m = bits[w];
+    return w == words - 1 && (c.pages & 31) ? m & ((1u << (c.pages & 31)) - 1u) : m;
+  };
+  int mine = 0, live;
+  for (int w = threadIdx.x; w < words; w += kBlock) mine += __popc(held(w));
+  block_scan(mine, sums, live);
+  int *from = list_of(c, 0), *to = list_of(c, 1), *place = list_of(c, 2);
+  int moves = 0, holes = 0;
+  for (int base = 0; base < words; base += kBlock) {
+    const int w = base + threadIdx.x;
+    uint32_t up = 0, down = 0;
+    if (w < words) {
+      const int page = w * 32;
+      const uint32_t low = page + 32 <= live ? 0xffffffffu : page >= live ? 0u : (1u << (live - page)) - 1u;  // pages below the count
+      up = held(w) & ~low;
+      down = ~bits[w] & low;
+    }
+    int all;
+    int at = moves + block_scan(__popc(up), sums, all);
+    moves += all;
+    for (; up; up &= up - 1) from[at++] = w * 32 + __ffs(up) - 1;
+    at = holes + block_scan(__popc(down), sums, all);
+    holes += all;
+    for (; down; down &= down - 1) to[at++] = w * 32 + __ffs(down) - 1;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < moves; i += kBlock) {
+    place[from[i]] = to[i];
+    c.refs[to[i]] = c.refs[from[i]];
+    c.refs[from[i]] = 0;
+  }
+  if (threadIdx.x == 0) {
+    c.state[kStateCopies] = moves;
+    c.state[kStateLive] = live;
+  }
+}
+
+// The moves' data and the table's new page numbers.
+constexpr int kMoveBytes = 16384;
+__global__ void __launch_bounds__(256) cache_move_kernel(const CacheView c) {
+  pdl_wait();
+  pdl_trigger();
+  if (c.state[kStateStatus]) return;
+  const int moves = c.state[kStateCopies], live = c.state[kStateLive];
+  const int *from = list_of(c, 0), *to = list_of(c, 1), *place = list_of(c, 2);
+  if (moves == 0) return;
+  const int64_t entries = static_cast<int64_t>(c.slots) * c.max_pages;
+  for (int64_t x = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; x < entries; x += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int page = c.table[x];
+    if (page >= live && page < c.pages) c.table[x] = place[page];
+  }
+  const int64_t page_bytes = (static_cast<int64_t>(c.dim) * c.kv_heads << c.page_shift) * c.size;  // a multiple of 16
+  const int pieces = static_cast<int>((page_bytes + kMoveBytes - 1) / kMoveBytes);
+  const int64_t units = static_cast<int64_t>(moves) * c.layers * 2 * pieces;
+  for (int64_t x = blockIdx.x; x < units; x += gridDim.x) {
+    const int piece = static_cast<int>(x % pieces);
+    const int64_t y = x / pieces;
+    const int side = static_cast<int>(y & 1), layer = static_cast<int>((y >> 1) % c.layers), i = static_cast<int>((y >> 1) / c.layers);
+    char *pool = static_cast<char *>(side ? c.v : c.k);
+    const int64_t lo = static_cast<int64_t>(piece) * kMoveBytes;
+    const uint4 *src = reinterpret_cast<const uint4 *>(pool + (static_cast<int64_t>(layer) * c.pages + from[i]) * page_bytes + lo);
+    uint4 *dst = reinterpret_cast<uint4 *>(pool + (static_cast<int64_t>(layer) * c.pages + to[i]) * page_bytes + lo);
+    const int n = static_cast<int>((page_bytes - lo < kMoveBytes ? page_bytes - lo : kMoveBytes) / 16);
+    constexpr int U = kMoveBytes / 16 / 256;
+    uint4 r[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (static_cast<int>(threadIdx.x) + 256 * u < n) r[u] = src[threadIdx.x + 256 * u];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (static_cast<int>(threadIdx.x) + 256 * u < n) dst[threadIdx.x + 256 * u] = r[u];
+  }
+}
+
+template <auto KERN>
+cudaError_t set_smem(size_t bytes) {
+  static bool done[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (bytes <= 48 * 1024 || (dev < 64 && done[dev])) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+  if (e == cudaSuccess && dev < 64) done[dev] = true;
+  return e;
+}
+
+}  // namespace
+
+cudaError_t launch_cache_reserve(const CacheView &c, const int *offsets, int uniform, int first, int n, cudaStream_t s) {
+  const size_t smem = (static_cast<size_t>(c.pages) + 31) / 32 * 4 + static_cast<size_t>(n) * 8;
+  cudaError_t e = set_smem<cache_reserve_kernel>(smem);
+  if (e != cudaSuccess) return e;
+  e = launch_pdl(cache_reserve_kernel, dim3(1), dim3(kBlock), smem, s, 1, c, offsets, uniform, first, n);
+  if (e != cudaSuccess) return e;
+  const dim3 grid(n < 512 ? n : 512, c.layers * 2);
+  return c.dim * c.size % 16 == 0 ? launch_pdl(cache_copy_kernel<uint4>, grid, dim3(128), 0, s, 1, c)
+         : c.dim * c.size % 4 == 0 ? launch_pdl(cache_copy_kernel<uint32_t>, grid, dim3(128), 0, s, 1, c)
+                                   : launch_pdl(cache_copy_kernel<uint16_t>, grid, dim3(128), 0, s, 1, c);
+}
+
+cudaError_t launch_cache_write(const CacheView &c, const void *k, const void *v, int64_t ts, int64_t hs, int64_t ls, int64_t v_ts,
+                               int64_t v_hs, int64_t v_ls, int layer, int layers, int rows, const int *offsets, int uniform,
+                               int first, int n, cudaStream_t s) {
+  const dim3 grid((rows + kWriteRows - 1) / kWriteRows, layers);
+  auto fits = [&](int unit) {
+    const int64_t x = reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | (ts * c.size) | (hs * c.size) | (ls * c.size) |
+                      (v_ts * c.size) | (v_hs * c.size) | (v_ls * c.size) | (static_cast<int64_t>(c.dim) * c.size);
+    return x % unit == 0;
+  };
+  auto go = [&](auto kern) {
+    return launch_pdl(kern, grid, dim3(256), 0, s, 1, c, static_cast<const char *>(k), static_cast<const char *>(v), ts, hs, ls, v_ts,
+                      v_hs, v_ls, layer, rows, offsets, uniform, first, n);
+  };
+  return fits(16) ? go(cache_write_kernel<uint4>) : fits(4) ? go(cache_write_kernel<uint32_t>) : go(cache_write_kernel<uint16_t>);
+}
+
+cudaError_t launch_cache_fork(const CacheView &c, const int *src, int first, int n, cudaStream_t s) {
+  const int cols = n <= 1024 ? 32 : 8;  // at most 128 KB of shared memory
+  const size_t smem = static_cast<size_t>(n) * cols * 4;
+  const cudaError_t e = set_smem<cache_fork_kernel>(smem);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(cache_fork_kernel, dim3((c.max_pages + cols - 1) / cols + 1), dim3(256), smem, s, 1, c, src, first, n, cols);
+}
+
+cudaError_t launch_cache_trim(const CacheView &c, int first, int n, int sinks, int window, cudaStream_t s) {
+  return launch_pdl(cache_trim_kernel, dim3(n), dim3(128), 0, s, 1, c, first, sinks, window);
+}
+
+cudaError_t launch_cache_compact(const CacheView &c, int sm_count, cudaStream_t s) {
+  const size_t smem = (static_cast<size_t>(c.pages) + 31) / 32 * 4;
+  cudaError_t e = set_smem<cache_plan_kernel>(smem);
+  if (e != cudaSuccess) return e;
+  e = launch_pdl(cache_plan_kernel, dim3(1), dim3(kBlock), smem, s, 1, c);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(cache_move_kernel, dim3(sm_count * 8), dim3(256), 0, s, 1, c);
+}
+
+}  // namespace nq

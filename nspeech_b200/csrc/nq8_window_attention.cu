@@ -1,0 +1,954 @@
+// nq8_window_attention.cu -- softmax attention through a sliding window whose
+// first tokens ("sinks") stay visible, over plain rows or a paged cache.
+//
+// Work item: a tile of R query rows of one kv head.  The rows of a tile are
+// (token, head of the group) pairs, token-major, so the heads that share keys
+// read them once, and a tile spans few positions, hence few keys outside the
+// window.  The tile's keys are the sinks [0, s) and the window [lo, hi] of all
+// its rows; they are walked in 64-key (bf16) or 32-key (f32) tiles with the
+// running maximum and sum of the softmax (f32, log2 units), one pass.
+//
+// bf16: scores and P V by warp-level MMA (m16n8k16, f32 accumulators), P
+// rounded to bf16 as the MMA's operand.  Few rows (a decoder's token): the
+// four warps take different keys of each tile and join at the end, so a step
+// streams K and V at the rate of memory instead of idling three warps.
+// f32: products in f32 FMA (no tensor-core form holds 24 bits).
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "nq8_window_attention.h"
+
+namespace nq {
+namespace {
+
+constexpr int kThreads = 128;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 16-byte copy global -> shared; zeros where !there (src is not read).
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a)
+               : "memory");
+}
+
+// One sequence: its first query row, its queries, first key row (plain rows)
+// and keys.
+struct Seq {
+  int q0, nq, k0, nk;
+};
+__device__ __forceinline__ void span(const int *off, const int *len, int rows, int seqs, int b, int &begin, int &n) {
+  int e;
+  if (off) {
+    begin = min(max(__ldg(off + b), 0), rows);
+    e = min(max(__ldg(off + b + 1), begin), rows);
+  } else {
+    const int each = rows / seqs;
+    begin = b * each;
+    e = begin + each;
+  }
+  n = e - begin;
+  if (len) n = min(n, max(__ldg(len + b), 0));
+}
+__device__ __forceinline__ Seq seq_of(const WinAttnParams &p, int b) {
+  Seq s;
+  span(p.q_off, p.q_len, p.q_rows, p.seqs, b, s.q0, s.nq);
+  if (p.table) {
+    s.k0 = 0;
+    s.nk = static_cast<int>(min(static_cast<long long>(max(__ldg(p.k_len + b), 0)),
+                                static_cast<long long>(p.max_pages) << p.page_shift));
+  } else {
+    span(p.k_off, p.k_len, p.k_rows, p.seqs, b, s.k0, s.nk);
+  }
+  return s;
+}
+// The row tile `tile` of all sequences' tiles of `rows` rows: sequence and
+// first row in it.  Every warp finds it by itself, 32 sequences at a time.
+__device__ __forceinline__ bool find_tile(const WinAttnParams &p, int tile, int rows, int &b, int &row0) {
+  if (!p.q_off && !p.q_len) {
+    const int per = ((p.q_rows / p.seqs) * p.group + rows - 1) / rows;
+    b = per ? tile / per : p.seqs;
+    row0 = per ? (tile - b * per) * rows : 0;
+    return b < p.seqs;
+  }
+  const int lane = threadIdx.x & 31;
+  int done = 0;
+  for (int base = 0; base < p.seqs; base += 32) {
+    int n = 0;
+    if (base + lane < p.seqs) {
+      int q0, nq;
+      span(p.q_off, p.q_len, p.q_rows, p.seqs, base + lane, q0, nq);
+      n = (nq * p.group + rows - 1) / rows;
+    }
+    int upto = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    const int all = __shfl_sync(0xffffffffu, upto, 31);
+    if (tile < done + all) {
+      const unsigned m = __ballot_sync(0xffffffffu, tile < done + upto);
+      const int w = __ffs(m) - 1;
+      b = base + w;
+      row0 = (tile - done - __shfl_sync(0xffffffffu, upto - n, w)) * rows;
+      return true;
+    }
+    done += all;
+  }
+  return false;
+}
+
+// The keys of a row tile: the sinks [0, s_end) and the window [lo, hi].
+struct Keys {
+  int lo, hi, s_end;  // s_end = 0 where the window's tiles hold the sinks too
+  int sink_tiles, tiles;
+};
+template <int KT>
+__device__ __forceinline__ Keys keys_of(const WinAttnParams &p, const Seq &s, int i_first, int i_last) {
+  Keys k;
+  const int p_lo = s.nk - s.nq + i_first, p_hi = s.nk - s.nq + i_last;
+  k.hi = p.right >= kWinUnlimited ? s.nk - 1 : min(s.nk - 1, p_hi + p.right);
+  k.lo = p.left >= kWinUnlimited ? 0 : max(0, p_lo - p.left);
+  k.s_end = max(0, min(min(p.sinks, k.lo), k.hi + 1));
+  k.sink_tiles = (k.s_end + KT - 1) / KT;
+  if (k.lo <= k.sink_tiles * KT) {  // the two parts touch: one run of tiles
+    if (k.s_end > 0) k.lo = 0;
+    k.s_end = 0;
+    k.sink_tiles = 0;
+  }
+  k.tiles = k.sink_tiles + (k.hi >= k.lo ? (k.hi - k.lo + KT) / KT : 0);
+  return k;
+}
+template <int KT>
+__device__ __forceinline__ int tile_base(const Keys &k, int t) {
+  return t < k.sink_tiles ? t * KT : k.lo + (t - k.sink_tiles) * KT;
+}
+__device__ __forceinline__ bool key_there(const Keys &k, int j) {
+  return j <= k.hi && (j >= k.lo || j < k.s_end);
+}
+
+// Element offset of key j's row for kv head h; -1 where the key's page is
+// missing or the key is outside the tile's keys (its row reads as zeros).
+template <bool PAGED>
+__device__ __forceinline__ int64_t key_row(const WinAttnParams &p, const Keys &k, const Seq &s, const int *table, int h,
+                                           int j, bool v) {
+  if (!key_there(k, j)) return -1;
+  if constexpr (PAGED) {
+    const int pg = __ldg(table + (j >> p.page_shift));
+    if (pg < 0 || pg >= p.pages) return -1;
+    const int r = j & ((1 << p.page_shift) - 1);
+    return (((static_cast<int64_t>(pg) * p.kv_heads + h) << p.page_shift) + r) * p.dim;
+  } else {
+    return v ? (s.k0 + static_cast<int64_t>(j)) * p.v_ts + h * p.v_hs : (s.k0 + static_cast<int64_t>(j)) * p.k_ts + h * p.k_hs;
+  }
+}
+
+// Joins the splits' partial results of one row tile, in split order.
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads) win_attn_join(const __grid_constant__ WinAttnParams p, int rows) {
+  pdl_wait();
+  pdl_trigger();
+  int b, row0;
+  if (!find_tile(p, blockIdx.x, rows, b, row0)) return;
+  const Seq s = seq_of(p, b);
+  const int h = blockIdx.y, heads = p.kv_heads * p.group;
+  const int64_t all = static_cast<int64_t>(p.q_rows) * heads;
+  constexpr int kLanes = DP / 4, kRowsAtOnce = kThreads / kLanes;
+  const int c = (threadIdx.x % kLanes) * 4;
+  for (int r = row0 + threadIdx.x / kLanes; r < min(row0 + rows, s.nq * p.group); r += kRowsAtOnce) {
+    const int i = r / p.group, hq = h * p.group + r % p.group;
+    const int64_t row = static_cast<int64_t>(s.q0 + i) * heads + hq;
+    float m = -INFINITY;
+    for (int z = 0; z < p.splits; ++z) m = fmaxf(m, p.part_ml[z * all + row].x);
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (m > -INFINITY) {
+      for (int z = 0; z < p.splits; ++z) {
+        const float2 ml = p.part_ml[z * all + row];
+        if (ml.x == -INFINITY) continue;
+        const float f = ex2(ml.x - m);
+        const float4 x = *reinterpret_cast<const float4 *>(p.part_o + (z * all + row) * DP + c);
+        l += ml.y * f;
+        o.x += x.x * f;
+        o.y += x.y * f;
+        o.z += x.z * f;
+        o.w += x.w * f;
+      }
+    }
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    T *out = static_cast<T *>(p.out) + (s.q0 + static_cast<int64_t>(i)) * p.o_ts + hq * p.o_hs;
+    const float e[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      if (c + x < p.dim) out[c + x] = T(e[x]);
+  }
+}
+
+// ---------------------------------------------------------------------- bf16
+// WR warps along the rows (16 each), WK = 4 / WR along the keys of a tile.
+template <int DP, int STAGES>
+struct MmaSmem {
+  static constexpr int kKT = 64;
+  static constexpr int kTileBytes = kKT * DP * 2;
+  static constexpr int kRing = STAGES + 1;  // row offsets and holes are made one tile ahead of the copies
+  static constexpr int kOffK = 0;
+  static constexpr int kOffV = STAGES * kTileBytes;
+  static constexpr int kOffQ = 2 * STAGES * kTileBytes;
+  static constexpr int kOffRow = kOffQ + 64 * DP * 2;
+  static constexpr int kOffHole = kOffRow + kRing * kKT * 8;
+  static constexpr int kBytes = kOffHole + kRing * 8;
+};
+
+template <int DP, int WR, int STAGES, bool PAGED, bool VEC>
+__global__ void __launch_bounds__(kThreads) win_attn_mma(const __grid_constant__ WinAttnParams p) {
+  using L = MmaSmem<DP, STAGES>;
+  constexpr int KT = L::kKT, WK = 4 / WR, KW = KT / WK, R = 16 * WR, CH = DP / 8;
+  static_assert(4 * 16 * (DP + 4) * 4 <= 2 * STAGES * L::kTileBytes, "the warps' join fits the key tiles");
+  extern __shared__ __align__(128) uint8_t smem[];
+  const uint32_t sb = smem_u32(smem);
+  int64_t *row_off = reinterpret_cast<int64_t *>(smem + L::kOffRow);
+  uint32_t *holes = reinterpret_cast<uint32_t *>(smem + L::kOffHole);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  pdl_wait();
+  pdl_trigger();
+  int b, row0;
+  // later tiles of a causal sequence see more keys: they go first
+  if (!find_tile(p, gridDim.x - 1 - blockIdx.x, R, b, row0)) return;
+  const Seq s = seq_of(p, b);
+  const int h = blockIdx.y, G = p.group;
+  const int n_rows = s.nq * G;
+  const int r_last = min(row0 + R, n_rows) - 1;
+  const Keys k = keys_of<KT>(p, s, row0 / G, r_last / G);
+  const int t0 = static_cast<int>(static_cast<int64_t>(k.tiles) * blockIdx.z / p.splits);
+  const int t1 = static_cast<int>(static_cast<int64_t>(k.tiles) * (blockIdx.z + 1) / p.splits);
+  const int nt = t1 - t0;
+  const int *table = PAGED ? p.table + static_cast<int64_t>(b) * p.table_ld : nullptr;
+  const __nv_bfloat16 *kp = static_cast<const __nv_bfloat16 *>(p.k), *vp = static_cast<const __nv_bfloat16 *>(p.v);
+
+  // Row offsets of tile t (and its holes: keys whose page is missing).
+  auto rows_of_tile = [&](int t) {
+    if constexpr (PAGED) {
+      if (warp < 2 && t < nt) {
+        const int slot = t % L::kRing;
+        const int j = tile_base<KT>(k, t0 + t) + tid;
+        const int64_t o = key_row<true>(p, k, s, table, h, j, false);
+        row_off[slot * KT + tid] = o;
+        const unsigned m = __ballot_sync(0xffffffffu, o < 0);
+        if (lane == 0) holes[slot * 2 + warp] = m;
+      }
+    }
+  };
+  auto copy_row = [&](uint32_t dst, const __nv_bfloat16 *src, bool there, int c) {
+    if constexpr (VEC) {
+      cp16(dst, src + 8 * c, there && 8 * c < p.dim);
+    } else {
+      uint32_t w[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int e = 8 * c + 2 * x;
+        const __nv_bfloat16 z = __float2bfloat16_rn(0.f);
+        const __nv_bfloat16 a = there && e < p.dim ? src[e] : z, d = there && e + 1 < p.dim ? src[e + 1] : z;
+        __nv_bfloat162 y(a, d);
+        w[x] = *reinterpret_cast<uint32_t *>(&y);
+      }
+      asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+    }
+  };
+  auto sw = [](int row, int c) { return static_cast<uint32_t>(row * (DP * 2) + ((c ^ (row & 7)) << 4)); };
+  auto load_tile = [&](int t) {
+    if (t < nt) {
+      const int st = t % STAGES, slot = t % L::kRing, base = tile_base<KT>(k, t0 + t);
+      const uint32_t ks = sb + L::kOffK + st * L::kTileBytes, vs = sb + L::kOffV + st * L::kTileBytes;
+      const int c = tid % CH;
+#pragma unroll
+      for (int r = tid / CH; r < KT; r += kThreads / CH) {
+        int64_t ok, ov;
+        if constexpr (PAGED) {
+          ok = ov = row_off[slot * KT + r];
+        } else {
+          ok = key_row<false>(p, k, s, nullptr, h, base + r, false);
+          ov = ok < 0 ? -1 : key_row<false>(p, k, s, nullptr, h, base + r, true);
+        }
+        copy_row(ks + sw(r, c), kp + (ok < 0 ? 0 : ok), ok >= 0, c);
+        copy_row(vs + sw(r, c), vp + (ov < 0 ? 0 : ov), ov >= 0, c);
+      }
+    }
+    cp_commit();
+  };
+
+  // Q tile.
+  const __nv_bfloat16 *qp = static_cast<const __nv_bfloat16 *>(p.q);
+  for (int x = tid; x < R * CH; x += kThreads) {
+    const int r = x / CH, c = x % CH, rr = row0 + r;
+    const bool there = rr < n_rows;
+    const int i = there ? rr / G : 0, g = there ? rr - i * G : 0;
+    copy_row(sb + L::kOffQ + sw(r, c), qp + (there ? (s.q0 + static_cast<int64_t>(i)) * p.q_ts + (h * G + g) * p.q_hs : 0), there, c);
+  }
+#pragma unroll
+  for (int t = 0; t < STAGES; ++t) rows_of_tile(t);
+  __syncthreads();
+#pragma unroll
+  for (int t = 0; t < STAGES - 1; ++t) load_tile(t);  // the first group holds Q too
+
+  const int wr = warp % WR, wk = warp / WR;
+  const int qr = lane >> 2;  // this thread's rows of the warp's 16: qr and qr + 8
+  int pos[2];                // their positions
+#pragma unroll
+  for (int x = 0; x < 2; ++x) pos[x] = s.nk - s.nq + min(row0 + 16 * wr + qr + 8 * x, n_rows - 1) / G;
+  const int pos_lo = s.nk - s.nq + row0 / G, pos_hi = s.nk - s.nq + r_last / G;
+  uint32_t qf[DP / 16][4];
+  float o[DP / 8][4];
+#pragma unroll
+  for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[d][e] = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+  for (int t = 0; t < nt; ++t) {
+    cp_wait<STAGES - 2>();
+    if constexpr (!VEC) asm volatile("" ::: "memory");
+    __syncthreads();
+    if (t == 0) {
+      const int r = 16 * wr + (lane & 7) + ((lane >> 3) & 1) * 8;
+#pragma unroll
+      for (int kk = 0; kk < DP / 16; ++kk) ldsm4(qf[kk], sb + L::kOffQ + sw(r, 2 * kk + (lane >> 4)));
+    }
+    load_tile(t + STAGES - 1);
+    rows_of_tile(t + STAGES);
+    const int st = t % STAGES, slot = t % L::kRing, base = tile_base<KT>(k, t0 + t);
+    const uint32_t ks = sb + L::kOffK + st * L::kTileBytes, vs = sb + L::kOffV + st * L::kTileBytes;
+    float sc[KW / 8][4];
+#pragma unroll
+    for (int n = 0; n < KW / 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sc[n][e] = 0.f;
+    {
+      const int r = wk * KW + (lane & 7) + ((lane >> 4) << 3), c = (lane >> 3) & 1;
+#pragma unroll
+      for (int kk = 0; kk < DP / 16; ++kk)
+#pragma unroll
+        for (int n = 0; n < KW / 16; ++n) {
+          uint32_t f[4];
+          ldsm4(f, ks + sw(r + 16 * n, 2 * kk + c));
+          mma_16816_bf16(sc[2 * n], qf[kk], f[0], f[1]);
+          mma_16816_bf16(sc[2 * n + 1], qf[kk], f[2], f[3]);
+        }
+    }
+    uint32_t hole[2] = {0u, 0u};
+    if constexpr (PAGED) {
+      hole[0] = holes[slot * 2];
+      hole[1] = holes[slot * 2 + 1];
+    }
+    // every row of the tile sees every key of it
+    const bool inside = base + KT - 1 <= k.hi && base + KT - 1 <= min(s.nk - 1, p.right >= kWinUnlimited ? s.nk - 1 : pos_lo + p.right) &&
+                        (p.left >= kWinUnlimited || base >= pos_hi - p.left || base + KT <= p.sinks) && !(hole[0] | hole[1]);
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int n = 0; n < KW / 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float x = sc[n][e] * p.sl2;
+        if (!inside) {
+          const int jl = wk * KW + 8 * n + 2 * (lane & 3) + (e & 1), j = base + jl;
+          const int at = pos[e >> 1];
+          const bool see = key_there(k, j) && (p.right >= kWinUnlimited || j <= at + p.right) &&
+                           (p.left >= kWinUnlimited || j >= at - p.left || j < p.sinks) && !((hole[jl >> 5] >> (jl & 31)) & 1u);
+          x = see ? x : -INFINITY;
+        }
+        sc[n][e] = x;
+        top[e >> 1] = fmaxf(top[e >> 1], x);
+      }
+    float ref[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 1));
+      top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 2));
+      top[x] = fmaxf(top[x], m[x]);
+      ref[x] = top[x] == -INFINITY ? 0.f : top[x];
+      const float f = ex2(m[x] - ref[x]);
+      l[x] *= f;
+      m[x] = top[x];
+#pragma unroll
+      for (int d = 0; d < DP / 8; ++d) {
+        o[d][2 * x] *= f;
+        o[d][2 * x + 1] *= f;
+      }
+    }
+    uint32_t pf[KW / 8][2];
+#pragma unroll
+    for (int n = 0; n < KW / 8; ++n)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const float a = ex2(sc[n][2 * x] - ref[x]), c = ex2(sc[n][2 * x + 1] - ref[x]);
+        l[x] += a + c;
+        pf[n][x] = pack_bf16x2(a, c);
+      }
+    {
+      const int r = wk * KW + (lane & 7) + ((lane >> 3) & 1) * 8, c = lane >> 4;
+#pragma unroll
+      for (int n = 0; n < KW / 16; ++n) {
+        const uint32_t a[4] = {pf[2 * n][0], pf[2 * n][1], pf[2 * n + 1][0], pf[2 * n + 1][1]};
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d) {
+          uint32_t f[4];
+          ldsm4t(f, vs + sw(r + 16 * n, 2 * d + c));
+          mma_16816_bf16(o[2 * d], a, f[0], f[1]);
+          mma_16816_bf16(o[2 * d + 1], a, f[2], f[3]);
+        }
+      }
+    }
+  }
+  cp_wait<0>();
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
+    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
+  }
+  const int heads = p.kv_heads * G;
+  const int64_t all = static_cast<int64_t>(p.q_rows) * heads;
+  __nv_bfloat16 *outp = static_cast<__nv_bfloat16 *>(p.out);
+  if constexpr (WK == 1) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int r = row0 + 16 * wr + qr + 8 * x;
+      if (r >= n_rows) continue;
+      const int i = r / G, hq = h * G + r % G;
+      if (p.splits > 1) {
+        const int64_t row = blockIdx.z * all + static_cast<int64_t>(s.q0 + i) * heads + hq;
+        if ((lane & 3) == 0) p.part_ml[row] = make_float2(m[x], l[x]);
+#pragma unroll
+        for (int d = 0; d < DP / 8; ++d)
+          *reinterpret_cast<float2 *>(p.part_o + row * DP + 8 * d + 2 * (lane & 3)) = make_float2(o[d][2 * x], o[d][2 * x + 1]);
+      } else {
+        const float inv = l[x] > 0.f ? 1.f / l[x] : (l[x] == 0.f ? 0.f : l[x]);
+        __nv_bfloat16 *out = outp + (s.q0 + static_cast<int64_t>(i)) * p.o_ts + hq * p.o_hs;
+#pragma unroll
+        for (int d = 0; d < DP / 8; ++d) {
+          const int c = 8 * d + 2 * (lane & 3);
+          if constexpr (VEC) {
+            if (c < p.dim) *reinterpret_cast<uint32_t *>(out + c) = pack_bf16x2(o[d][2 * x] * inv, o[d][2 * x + 1] * inv);
+          } else {
+            if (c < p.dim) out[c] = __float2bfloat16_rn(o[d][2 * x] * inv);
+            if (c + 1 < p.dim) out[c + 1] = __float2bfloat16_rn(o[d][2 * x + 1] * inv);
+          }
+        }
+      }
+    }
+  } else {
+    // Join the WK warps of each 16 rows through shared memory.
+    constexpr int P = DP + 4;
+    __syncthreads();
+    float *jo = reinterpret_cast<float *>(smem);                        // [4 warps][16][P]
+    float2 *jml = reinterpret_cast<float2 *>(smem + L::kOffQ);          // [4 warps][16]
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int r = 16 * warp + qr + 8 * x;
+      if ((lane & 3) == 0) jml[r] = make_float2(m[x], l[x]);
+#pragma unroll
+      for (int d = 0; d < DP / 8; ++d)
+        *reinterpret_cast<float2 *>(jo + r * P + 8 * d + 2 * (lane & 3)) = make_float2(o[d][2 * x], o[d][2 * x + 1]);
+    }
+    __syncthreads();
+    constexpr int kPer = kThreads / R;        // threads of a row
+    const int r = tid / kPer, rr = row0 + r;  // r < R
+    if (rr < n_rows) {
+      const int w0 = r / 16;                  // warp w0 + WR x holds the row's part x
+      float mm = -INFINITY, ll = 0.f, f[WK];
+#pragma unroll
+      for (int x = 0; x < WK; ++x) mm = fmaxf(mm, jml[16 * (w0 + WR * x) + r % 16].x);
+#pragma unroll
+      for (int x = 0; x < WK; ++x) {
+        const float2 ml = jml[16 * (w0 + WR * x) + r % 16];
+        f[x] = ml.x == -INFINITY ? 0.f : ex2(ml.x - mm);
+        ll += ml.y * f[x];
+      }
+      const int i = rr / G, hq = h * G + rr % G;
+      const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
+      const int64_t row = blockIdx.z * all + static_cast<int64_t>(s.q0 + i) * heads + hq;
+      __nv_bfloat16 *out = outp + (s.q0 + static_cast<int64_t>(i)) * p.o_ts + hq * p.o_hs;
+      if (p.splits > 1 && tid % kPer == 0) p.part_ml[row] = make_float2(mm, ll);
+#pragma unroll
+      for (int c = (tid % kPer) * 4; c < DP; c += kPer * 4) {
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < WK; ++x) {
+          if (f[x] == 0.f) continue;  // a part without a visible key
+          const float4 y = *reinterpret_cast<const float4 *>(jo + (16 * (w0 + WR * x) + r % 16) * P + c);
+          v[0] += y.x * f[x];
+          v[1] += y.y * f[x];
+          v[2] += y.z * f[x];
+          v[3] += y.w * f[x];
+        }
+        if (p.splits > 1) {
+          *reinterpret_cast<float4 *>(p.part_o + row * DP + c) = make_float4(v[0], v[1], v[2], v[3]);
+        } else if constexpr (VEC) {
+          if (c < p.dim)
+            *reinterpret_cast<uint2 *>(out + c) = make_uint2(pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (c + e < p.dim) out[c + e] = __float2bfloat16_rn(v[e] * inv);
+        }
+      }
+    }
+  }
+}
+
+// ----------------------------------------------------------------------- f32
+// Tile form: 64 rows x 32 keys, 4 x 4 scores and 4 x DP / 8 outputs a thread.
+template <int DP>
+struct F32Smem {
+  static constexpr int kR = 64, kKT = 32, kP = DP + 4, kPP = kKT + 4;
+  static constexpr int kOffQ = 0;
+  static constexpr int kOffK = kOffQ + kR * kP * 4;
+  static constexpr int kOffV = kOffK + 2 * kKT * kP * 4;
+  static constexpr int kOffP = kOffV + 2 * kKT * kP * 4;
+  static constexpr int kOffRow = kOffP + kR * kPP * 4;
+  static constexpr int kBytes = kOffRow + 3 * kKT * 8;
+};
+
+template <bool VEC>
+__device__ __forceinline__ void copy4(float *dst, const float *src, bool there, int c, int dim) {
+  if constexpr (VEC) {
+    cp16(smem_u32(dst), src + c, there && c < dim);
+  } else {
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (there) {
+      if (c < dim) x.x = src[c];
+      if (c + 1 < dim) x.y = src[c + 1];
+      if (c + 2 < dim) x.z = src[c + 2];
+      if (c + 3 < dim) x.w = src[c + 3];
+    }
+    *reinterpret_cast<float4 *>(dst) = x;
+  }
+}
+
+template <int DP, bool PAGED, bool VEC>
+__global__ void __launch_bounds__(kThreads) win_attn_f32(const __grid_constant__ WinAttnParams p) {
+  using L = F32Smem<DP>;
+  constexpr int R = L::kR, KT = L::kKT, P = L::kP, PP = L::kPP, CH = DP / 4, NC = DP / 32;
+  extern __shared__ __align__(128) uint8_t smem[];
+  float *qs = reinterpret_cast<float *>(smem + L::kOffQ), *ps = reinterpret_cast<float *>(smem + L::kOffP);
+  int64_t *row_off = reinterpret_cast<int64_t *>(smem + L::kOffRow);
+  const int tid = threadIdx.x;
+  pdl_wait();
+  pdl_trigger();
+  int b, row0;
+  if (!find_tile(p, gridDim.x - 1 - blockIdx.x, R, b, row0)) return;
+  const Seq s = seq_of(p, b);
+  const int h = blockIdx.y, G = p.group, n_rows = s.nq * G, r_last = min(row0 + R, n_rows) - 1;
+  const Keys k = keys_of<KT>(p, s, row0 / G, r_last / G);
+  const int t0 = static_cast<int>(static_cast<int64_t>(k.tiles) * blockIdx.z / p.splits);
+  const int nt = static_cast<int>(static_cast<int64_t>(k.tiles) * (blockIdx.z + 1) / p.splits) - t0;
+  const int *table = PAGED ? p.table + static_cast<int64_t>(b) * p.table_ld : nullptr;
+  const float *kp = static_cast<const float *>(p.k), *vp = static_cast<const float *>(p.v), *qp = static_cast<const float *>(p.q);
+  auto rows_of_tile = [&](int t) {
+    if (PAGED && tid < KT && t < nt) row_off[(t % 3) * KT + tid] = key_row<true>(p, k, s, table, h, tile_base<KT>(k, t0 + t) + tid, false);
+  };
+  auto load_tile = [&](int t) {
+    if (t < nt) {
+      float *ks = reinterpret_cast<float *>(smem + L::kOffK) + (t & 1) * KT * P;
+      float *vs = reinterpret_cast<float *>(smem + L::kOffV) + (t & 1) * KT * P;
+      const int c = (tid % CH) * 4, base = tile_base<KT>(k, t0 + t);
+#pragma unroll
+      for (int r = tid / CH; r < KT; r += kThreads / CH) {
+        int64_t ok, ov;
+        if constexpr (PAGED) {
+          ok = ov = row_off[(t % 3) * KT + r];
+        } else {
+          ok = key_row<false>(p, k, s, nullptr, h, base + r, false);
+          ov = ok < 0 ? -1 : key_row<false>(p, k, s, nullptr, h, base + r, true);
+        }
+        copy4<VEC>(ks + r * P + c, kp + (ok < 0 ? 0 : ok), ok >= 0, c, p.dim);
+        copy4<VEC>(vs + r * P + c, vp + (ov < 0 ? 0 : ov), ov >= 0, c, p.dim);
+      }
+    }
+    cp_commit();
+  };
+  for (int x = tid; x < R * CH; x += kThreads) {
+    const int r = x / CH, c = (x % CH) * 4, rr = row0 + r;
+    const bool there = rr < n_rows;
+    const int i = there ? rr / G : 0, g = there ? rr - i * G : 0;
+    copy4<VEC>(qs + r * P + c, qp + (there ? (s.q0 + static_cast<int64_t>(i)) * p.q_ts + (h * G + g) * p.q_hs : 0), there, c, p.dim);
+  }
+  rows_of_tile(0);
+  rows_of_tile(1);
+  __syncthreads();
+  load_tile(0);
+  const int ty = tid >> 3, tx = tid & 7;  // rows ty + 16 i, keys tx + 8 j, columns 4 tx + 32 j
+  int pos[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) pos[i] = s.nk - s.nq + min(row0 + ty + 16 * i, n_rows - 1) / G;
+  float m[4], l[4], o[4][4 * NC];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+#pragma unroll
+    for (int c = 0; c < 4 * NC; ++c) o[i][c] = 0.f;
+  }
+  for (int t = 0; t < nt; ++t) {
+    load_tile(t + 1);
+    cp_wait<1>();
+    __syncthreads();
+    rows_of_tile(t + 2);
+    const float *ks = reinterpret_cast<const float *>(smem + L::kOffK) + (t & 1) * KT * P;
+    const float *vs = reinterpret_cast<const float *>(smem + L::kOffV) + (t & 1) * KT * P;
+    const int base = tile_base<KT>(k, t0 + t);
+    float sc[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sc[i][j] = 0.f;
+#pragma unroll 4
+    for (int d = 0; d < DP; d += 4) {
+      float4 a[4], c[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4 *>(qs + (ty + 16 * i) * P + d);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) c[j] = *reinterpret_cast<const float4 *>(ks + (tx + 8 * j) * P + d);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          sc[i][j] = fmaf(a[i].x, c[j].x, sc[i][j]);
+          sc[i][j] = fmaf(a[i].y, c[j].y, sc[i][j]);
+          sc[i][j] = fmaf(a[i].z, c[j].z, sc[i][j]);
+          sc[i][j] = fmaf(a[i].w, c[j].w, sc[i][j]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float top = m[i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = base + tx + 8 * j;
+        bool see = key_there(k, key) && (p.right >= kWinUnlimited || key <= pos[i] + p.right) &&
+                   (p.left >= kWinUnlimited || key >= pos[i] - p.left || key < p.sinks);
+        if (PAGED) see = see && row_off[(t % 3) * KT + tx + 8 * j] >= 0;
+        sc[i][j] = see ? sc[i][j] * p.sl2 : -INFINITY;
+        top = fmaxf(top, sc[i][j]);
+      }
+#pragma unroll
+      for (int x = 1; x < 8; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+      const float ref = top == -INFINITY ? 0.f : top;
+      const float f = exp2f(m[i] - ref);
+      m[i] = top;
+      l[i] *= f;
+#pragma unroll
+      for (int c = 0; c < 4 * NC; ++c) o[i][c] *= f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float e = exp2f(sc[i][j] - ref);
+        l[i] += e;
+        ps[(ty + 16 * i) * PP + tx + 8 * j] = e;
+      }
+    }
+    __syncwarp();  // a row's eight threads are of one warp
+#pragma unroll 2
+    for (int j = 0; j < KT; j += 4) {
+      float4 e[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) e[i] = *reinterpret_cast<const float4 *>(ps + (ty + 16 * i) * PP + j);
+#pragma unroll
+      for (int jj = 0; jj < 4; ++jj)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const float4 x = *reinterpret_cast<const float4 *>(vs + (j + jj) * P + 32 * c + 4 * tx);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float w = jj == 0 ? e[i].x : jj == 1 ? e[i].y : jj == 2 ? e[i].z : e[i].w;
+            o[i][4 * c] = fmaf(w, x.x, o[i][4 * c]);
+            o[i][4 * c + 1] = fmaf(w, x.y, o[i][4 * c + 1]);
+            o[i][4 * c + 2] = fmaf(w, x.z, o[i][4 * c + 2]);
+            o[i][4 * c + 3] = fmaf(w, x.w, o[i][4 * c + 3]);
+          }
+        }
+    }
+    __syncthreads();
+  }
+  cp_wait<0>();
+  const int heads = p.kv_heads * G;
+  const int64_t all = static_cast<int64_t>(p.q_rows) * heads;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int x = 1; x < 8; x <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], x);
+    const int rr = row0 + ty + 16 * i;
+    if (rr >= n_rows) continue;
+    const int tok = rr / G, hq = h * G + rr % G;
+    if (p.splits > 1) {
+      const int64_t row = blockIdx.z * all + static_cast<int64_t>(s.q0 + tok) * heads + hq;
+      if (tx == 0) p.part_ml[row] = make_float2(m[i], l[i]);
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        *reinterpret_cast<float4 *>(p.part_o + row * DP + 32 * c + 4 * tx) = make_float4(o[i][4 * c], o[i][4 * c + 1], o[i][4 * c + 2], o[i][4 * c + 3]);
+    } else {
+      const float inv = l[i] > 0.f ? 1.f / l[i] : (l[i] == 0.f ? 0.f : l[i]);
+      float *out = static_cast<float *>(p.out) + (s.q0 + static_cast<int64_t>(tok)) * p.o_ts + hq * p.o_hs;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int col = 32 * c + 4 * tx;
+        if constexpr (VEC) {
+          if (col < p.dim)
+            *reinterpret_cast<float4 *>(out + col) = make_float4(o[i][4 * c] * inv, o[i][4 * c + 1] * inv, o[i][4 * c + 2] * inv, o[i][4 * c + 3] * inv);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (col + e < p.dim) out[col + e] = o[i][4 * c + e] * inv;
+        }
+      }
+    }
+  }
+}
+
+// Row form, for a decoder's single tokens: at most R (1, 2, 4) rows share a
+// key, and a warp takes 8 loads of 32 / (DP / 4) keys at a time straight from
+// memory (lane: four columns), K and V together, so that 16 KB of a CTA are in
+// flight; the four warps and the keys' lane groups join at the end.
+template <int DP, int R, bool PAGED, bool VEC>
+__global__ void __launch_bounds__(kThreads) win_attn_f32_rows(const __grid_constant__ WinAttnParams p) {
+  constexpr int LPK = DP / 4, KPL = 32 / LPK, U = 8, KT = U * KPL;
+  __shared__ float4 jo[4][R][32];
+  __shared__ float2 jml[4][R][KPL];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, sub = lane / LPK, c = (lane % LPK) * 4;
+  pdl_wait();
+  pdl_trigger();
+  int b, row0;
+  if (!find_tile(p, gridDim.x - 1 - blockIdx.x, R, b, row0)) return;
+  const Seq s = seq_of(p, b);
+  const int h = blockIdx.y, G = p.group, n_rows = s.nq * G, r_last = min(row0 + R, n_rows) - 1;
+  const Keys k = keys_of<KT>(p, s, row0 / G, r_last / G);
+  const int t0 = static_cast<int>(static_cast<int64_t>(k.tiles) * blockIdx.z / p.splits);
+  const int t1 = static_cast<int>(static_cast<int64_t>(k.tiles) * (blockIdx.z + 1) / p.splits);
+  const int *table = PAGED ? p.table + static_cast<int64_t>(b) * p.table_ld : nullptr;
+  const float *kp = static_cast<const float *>(p.k), *vp = static_cast<const float *>(p.v), *qp = static_cast<const float *>(p.q);
+  auto fetch = [&](const float *src, bool there) {
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if constexpr (VEC) {
+      if (there && c < p.dim) x = __ldg(reinterpret_cast<const float4 *>(src + c));
+    } else if (there) {
+      if (c < p.dim) x.x = src[c];
+      if (c + 1 < p.dim) x.y = src[c + 1];
+      if (c + 2 < p.dim) x.z = src[c + 2];
+      if (c + 3 < p.dim) x.w = src[c + 3];
+    }
+    return x;
+  };
+  float4 q[R], o[R];
+  int pos[R];
+  float m[R], l[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int rr = min(row0 + r, n_rows - 1), i = rr / G;
+    q[r] = fetch(qp + (s.q0 + static_cast<int64_t>(i)) * p.q_ts + (h * G + rr - i * G) * p.q_hs, true);
+    pos[r] = s.nk - s.nq + i;
+    o[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+  }
+  // this lane's key rows of tile t
+  auto rows_of = [&](int t, int64_t (&off)[U]) {
+    const int base = t < t1 ? tile_base<KT>(k, t) : 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) off[u] = t < t1 ? key_row<PAGED>(p, k, s, table, h, base + u * KPL + sub, false) : -1;
+  };
+  int64_t off[U];
+  rows_of(t0 + warp, off);
+  for (int t = t0 + warp; t < t1; t += 4) {
+    const int base = tile_base<KT>(k, t);
+    float4 kk[U], vv[U];
+    bool there[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      there[u] = off[u] >= 0;
+      const int64_t ov = PAGED ? off[u] : key_row<PAGED>(p, k, s, table, h, base + u * KPL + sub, true);
+      kk[u] = fetch(kp + (there[u] ? off[u] : 0), there[u]);
+      vv[u] = fetch(vp + (there[u] ? ov : 0), there[u]);
+    }
+    rows_of(t + 4, off);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float sc[U], top = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float x = q[r].x * kk[u].x;
+        x = fmaf(q[r].y, kk[u].y, x);
+        x = fmaf(q[r].z, kk[u].z, x);
+        x = fmaf(q[r].w, kk[u].w, x);
+#pragma unroll
+        for (int y = LPK / 2; y > 0; y >>= 1) x += __shfl_xor_sync(0xffffffffu, x, y);
+        const int key = base + u * KPL + sub;
+        const bool see = there[u] && (p.right >= kWinUnlimited || key <= pos[r] + p.right) &&
+                         (p.left >= kWinUnlimited || key >= pos[r] - p.left || key < p.sinks);
+        sc[u] = see ? x * p.sl2 : -INFINITY;
+        top = fmaxf(top, sc[u]);
+      }
+      top = fmaxf(top, m[r]);  // each lane group keeps its own keys' maximum
+      const float ref = top == -INFINITY ? 0.f : top, f = exp2f(m[r] - ref);
+      m[r] = top;
+      l[r] *= f;
+      o[r].x *= f;
+      o[r].y *= f;
+      o[r].z *= f;
+      o[r].w *= f;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float e = exp2f(sc[u] - ref);
+        l[r] += e;
+        o[r].x = fmaf(e, vv[u].x, o[r].x);
+        o[r].y = fmaf(e, vv[u].y, o[r].y);
+        o[r].z = fmaf(e, vv[u].z, o[r].z);
+        o[r].w = fmaf(e, vv[u].w, o[r].w);
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    jo[warp][r][lane] = o[r];
+    if (lane % LPK == 0) jml[warp][r][sub] = make_float2(m[r], l[r]);
+  }
+  __syncthreads();
+  const int heads = p.kv_heads * G;
+  const int64_t all = static_cast<int64_t>(p.q_rows) * heads;
+  for (int x = tid; x < R * LPK; x += kThreads) {
+    const int r = x / LPK, cc = x % LPK, rr = row0 + r;
+    if (rr >= n_rows) continue;
+    float mm = -INFINITY, ll = 0.f;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < 4 * KPL; ++w) mm = fmaxf(mm, jml[w / KPL][r][w % KPL].x);
+#pragma unroll
+    for (int w = 0; w < 4 * KPL; ++w) {
+      const float2 ml = jml[w / KPL][r][w % KPL];
+      if (ml.x == -INFINITY) continue;
+      const float f = exp2f(ml.x - mm);
+      const float4 z = jo[w / KPL][r][(w % KPL) * LPK + cc];
+      ll += ml.y * f;
+      y.x += z.x * f;
+      y.y += z.y * f;
+      y.z += z.z * f;
+      y.w += z.w * f;
+    }
+    const int i = rr / G, hq = h * G + rr % G;
+    if (p.splits > 1) {
+      const int64_t row = blockIdx.z * all + static_cast<int64_t>(s.q0 + i) * heads + hq;
+      if (cc == 0) p.part_ml[row] = make_float2(mm, ll);
+      *reinterpret_cast<float4 *>(p.part_o + row * DP + 4 * cc) = y;
+    } else {
+      const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
+      float *out = static_cast<float *>(p.out) + (s.q0 + static_cast<int64_t>(i)) * p.o_ts + hq * p.o_hs;
+      const float e[4] = {y.x * inv, y.y * inv, y.z * inv, y.w * inv};
+#pragma unroll
+      for (int z = 0; z < 4; ++z)
+        if (4 * cc + z < p.dim) out[4 * cc + z] = e[z];
+    }
+  }
+}
+
+template <auto KERN>
+cudaError_t launch_smem(dim3 grid, size_t smem, cudaStream_t stream, const WinAttnParams &p) {
+  static bool done[64] = {false};  // per device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (smem > 48 * 1024 && !(dev < 64 && done[dev])) {
+    const cudaError_t e = cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return e;
+    if (dev < 64) done[dev] = true;
+  }
+  return launch_pdl(KERN, grid, dim3(kThreads), smem, stream, 1, p);
+}
+
+template <int DP, bool PAGED, bool VEC>
+cudaError_t launch_form(const WinAttnParams &p, int f32, const WinAttnPlan &pl, cudaStream_t stream) {
+  const dim3 grid(pl.tiles, p.kv_heads, pl.splits);
+  constexpr int kDeep = DP == 64 ? 4 : 3;
+  if (f32) {
+    if (pl.rows == 1) return launch_smem<win_attn_f32_rows<DP, 1, PAGED, VEC>>(grid, 0, stream, p);
+    if (pl.rows == 2) return launch_smem<win_attn_f32_rows<DP, 2, PAGED, VEC>>(grid, 0, stream, p);
+    if (pl.rows == 4) return launch_smem<win_attn_f32_rows<DP, 4, PAGED, VEC>>(grid, 0, stream, p);
+    return launch_smem<win_attn_f32<DP, PAGED, VEC>>(grid, F32Smem<DP>::kBytes, stream, p);
+  }
+  if (pl.rows == 16) return launch_smem<win_attn_mma<DP, 1, kDeep, PAGED, VEC>>(grid, MmaSmem<DP, kDeep>::kBytes, stream, p);
+  if (pl.rows == 32) return launch_smem<win_attn_mma<DP, 2, kDeep, PAGED, VEC>>(grid, MmaSmem<DP, kDeep>::kBytes, stream, p);
+  return launch_smem<win_attn_mma<DP, 4, 2, PAGED, VEC>>(grid, MmaSmem<DP, 2>::kBytes, stream, p);
+}
+
+bool aligned16(const void *x, int64_t a, int64_t b, int size) {
+  return reinterpret_cast<uintptr_t>(x) % 16 == 0 && (a * size) % 16 == 0 && (b * size) % 16 == 0;
+}
+
+}  // namespace
+
+WinAttnPlan win_attn_plan(int sm_count, int f32, bool uniform, int seqs, int q_rows, int64_t key_bound, int kv_heads, int group, int dim,
+                          int left, int right, int sinks) {
+  WinAttnPlan pl;
+  const int64_t rows = static_cast<int64_t>(q_rows) * group;
+  const int64_t mean = (rows + seqs - 1) / seqs;  // rows of a sequence and kv head
+  if (f32) {
+    pl.rows = mean <= 1 ? 1 : mean <= 2 ? 2 : mean <= 4 ? 4 : 64;
+  } else {
+    pl.rows = mean <= 16 ? 16 : mean <= 32 ? 32 : 64;
+  }
+  // every sequence's last tile may be a part of one
+  pl.tiles = static_cast<int>(uniform ? seqs * ((mean + pl.rows - 1) / pl.rows) : rows / pl.rows + seqs);
+  // Keys of a tile at most, and the CTAs that the call has without a split.
+  int64_t keys = key_bound;
+  if (left < kWinUnlimited && right < kWinUnlimited)
+    keys = keys < static_cast<int64_t>(left) + right + sinks + pl.rows ? keys : static_cast<int64_t>(left) + right + sinks + pl.rows;
+  const int64_t have = ((rows + pl.rows - 1) / pl.rows > seqs ? (rows + pl.rows - 1) / pl.rows : seqs) * kv_heads;
+  const int64_t want = 2LL * sm_count;
+  int64_t z = have > 0 ? want / have : 1;
+  const int64_t most = keys / 256;  // at least four 64-key tiles a CTA
+  z = z < most ? z : most;
+  pl.splits = static_cast<int>(z < 1 ? 1 : z > 64 ? 64 : z);
+  const int dp = dim <= 64 ? 64 : 128;
+  pl.workspace = pl.splits > 1 ? static_cast<size_t>(pl.splits) * q_rows * kv_heads * group * (dp * 4 + 8) : 0;
+  return pl;
+}
+
+cudaError_t launch_win_attn(const WinAttnParams &p, int f32, const WinAttnPlan &pl, cudaStream_t stream) {
+  const int size = f32 ? 4 : 2;
+  const bool vec = (p.dim * size) % 16 == 0 && aligned16(p.q, p.q_ts, p.q_hs, size) && aligned16(p.out, p.o_ts, p.o_hs, size) &&
+                   (p.table ? aligned16(p.k, 0, 0, size) && aligned16(p.v, 0, 0, size)
+                            : aligned16(p.k, p.k_ts, p.k_hs, size) && aligned16(p.v, p.v_ts, p.v_hs, size));
+  const bool paged = p.table != nullptr;
+  cudaError_t e;
+  if (p.dim <= 64) {
+    e = paged ? vec ? launch_form<64, true, true>(p, f32, pl, stream) : launch_form<64, true, false>(p, f32, pl, stream)
+              : vec ? launch_form<64, false, true>(p, f32, pl, stream) : launch_form<64, false, false>(p, f32, pl, stream);
+  } else {
+    e = paged ? vec ? launch_form<128, true, true>(p, f32, pl, stream) : launch_form<128, true, false>(p, f32, pl, stream)
+              : vec ? launch_form<128, false, true>(p, f32, pl, stream) : launch_form<128, false, false>(p, f32, pl, stream);
+  }
+  if (e != cudaSuccess || pl.splits == 1) return e;
+  const dim3 grid(pl.tiles, p.kv_heads);
+  if (f32)
+    return p.dim <= 64 ? launch_pdl(win_attn_join<float, 64>, grid, dim3(kThreads), 0, stream, 1, p, pl.rows)
+                       : launch_pdl(win_attn_join<float, 128>, grid, dim3(kThreads), 0, stream, 1, p, pl.rows);
+  return p.dim <= 64 ? launch_pdl(win_attn_join<__nv_bfloat16, 64>, grid, dim3(kThreads), 0, stream, 1, p, pl.rows)
+                     : launch_pdl(win_attn_join<__nv_bfloat16, 128>, grid, dim3(kThreads), 0, stream, 1, p, pl.rows);
+}
+
+}  // namespace nq

@@ -27,6 +27,7 @@ NQ_ERR_IO = -8
 NQ_ERR_NOT_INIT = -9
 NQ_ERR_UNSUPPORTED = -10
 NQ_ERR_DEVICE = -11
+NQ_ERR_CACHE = -12
 
 NQ_F32 = 0
 NQ_BF16 = 1
@@ -48,6 +49,11 @@ NQ_ATTENTION_MMA_SYNC = 1
 NQ_CONV_AUTO = 0
 NQ_CONV_IM2COL = 1
 
+NQ_CACHE_OUT_OF_PAGES = 0x1
+NQ_CACHE_SLOT_FULL = 0x2
+NQ_CACHE_BAD_INDEX = 0x4
+NQ_CACHE_SHARED_PAGE = 0x8
+
 NQ_GEMV_AUTO = 0
 NQ_GEMV_SPLIT = 1
 NQ_GEMV_CLUSTER = 2
@@ -67,6 +73,20 @@ class EncoderConfig(ctypes.Structure):
     _fields_ = [("feat_in", ctypes.c_int), ("d_model", ctypes.c_int), ("n_heads", ctypes.c_int),
                 ("ff_mult", ctypes.c_int), ("n_layers", ctypes.c_int), ("conv_kernel", ctypes.c_int),
                 ("sub_channels", ctypes.c_int), ("scale_input", ctypes.c_int)]
+
+
+class Rows(ctypes.Structure):
+    """nq_rows: rows [token][head][head_dim], strides in elements."""
+
+    _fields_ = [("ptr", ctypes.c_void_p), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
+class Cache(ctypes.Structure):
+    """nq_cache: the device arrays and sizes of a paged cache."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("k", "v", "table", "lens", "refs", "state")] +
+                [(n, ctypes.c_int) for n in ("dtype", "layers", "pages", "page_tokens", "kv_heads", "head_dim", "slots",
+                                             "max_pages")])
 
 
 _lib = None
@@ -137,6 +157,21 @@ SIGNATURES = {
     "nq_chain_steps": (_I, [_P]),
     "nq_chain_run": (_I, [_P, _P]),
     "nq_chain_free": (None, [_P]),
+    "nq_window_attention_workspace": (_I64, [_I, _I, _I64, _I64, _I, _I, _I, _I, _I, _I]),
+    "nq_window_attention": (_I, [_P, _P, _P, _P, _I, _I, _I64, _I64, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, ctypes.c_float,
+                                 _P, _I64, _P]),
+    "nq_cache_state_ints": (_I64, [_I, _I]),
+    "nq_cache_reserve": (_I, [_P, _I, _I, _P, _I, _P]),
+    "nq_cache_write": (_I, [_P, _P, _P, _I64, _I64, _I, _I, _I64, _I, _I, _P, _I, _P]),
+    "nq_cache_attention_workspace": (_I64, [_P, _I, _I64, _I, _I, _I, _I]),
+    "nq_cache_attention": (_I, [_P, _I, _P, _P, _I, _I, _I64, _P, _I, _I, _I, _I, ctypes.c_float, _P, _I64, _P]),
+    "nq_cache_fork": (_I, [_P, _I, _I, _P, _P]),
+    "nq_cache_trim": (_I, [_P, _I, _I, _I, _I, _P]),
+    "nq_cache_compact": (_I, [_P, _P]),
+    "nq_cache_status": (_I, [_P, ctypes.POINTER(_I), _P]),
+    "nq_beam_workspace": (_I64, [_I, _I, _I64]),
+    "nq_beam_select": (_I, [_P, _I, _I64, _I, _I, _I64, _P, _P, _I, _P, _P, _P, _P, _P, _I64, _P]),
+    "nq_beam_reorder": (_I, [_P, _P, _P, _P, _P, _I, _I, _P, _P]),
     "nq_set_wait_limit": (_I, [_I64]),
     "nq_debug_wait_timeout": (_I, [_P]),
 }
