@@ -9,7 +9,6 @@ right is no limit.  ``nspeech_b200.cache`` runs the same over a paged cache.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 from typing import Optional
@@ -20,6 +19,9 @@ from . import lib as _l
 from .fast_matmul import MatMulError
 
 _CODES = {torch.float32: _l.NQ_F32, torch.bfloat16: _l.NQ_BF16}
+_ref = ctypes.byref
+_Quad = _l.Rows * 4
+_Pair = _l.Rows * 2
 
 
 def _code(t: torch.Tensor, name: str) -> int:
@@ -29,47 +31,50 @@ def _code(t: torch.Tensor, name: str) -> int:
     return code
 
 
-def _here(t: torch.Tensor, name: str):
-    """The tensor's device made ready, as a context in which it is the current one."""
-    if not t.is_cuda:
-        raise MatMulError(f"{name} must live on a CUDA device")
-    index, now = t.device.index, torch.cuda.current_device()
+def _device(t: torch.Tensor, name: str) -> int:
+    """The tensor's device, made ready."""
+    index = t.get_device()
     if index not in _l._inited:
+        if not t.is_cuda:
+            raise MatMulError(f"{name} must live on a CUDA device")
+        now = torch.cuda.current_device()
         _l.init(index)
         torch.cuda.set_device(now)
-    return contextlib.nullcontext() if index == now else torch.cuda.device(index)
+    return index
 
 
-def _stream(t: torch.Tensor, stream: Optional[torch.cuda.Stream], *made: Optional[torch.Tensor]) -> int:
-    """The stream to launch on: `stream`, or the current one of t's device.  Tensors made for the call on the current
+def _stream(index: int, stream: Optional[torch.cuda.Stream], *made: Optional[torch.Tensor]) -> int:
+    """The stream to launch on: `stream`, or the current one of the device.  Tensors made for the call on the current
     stream are kept from reuse until `stream` is through with them."""
     if stream is None:
-        return torch.cuda.current_stream(t.device).cuda_stream
-    if stream.device != t.device:
-        raise MatMulError(f"the stream is on {stream.device}, the tensors on {t.device}")
+        return torch.cuda.current_stream(index).cuda_stream
+    if stream.device.index != index:
+        raise MatMulError(f"the stream is on {stream.device}, the tensors on cuda:{index}")
     for m in made:
         if m is not None:
             m.record_stream(stream)
     return stream.cuda_stream
 
 
-def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device) -> _l.Rows:
-    if t.dim() != 3 or t.dtype != dtype or t.device != device or (t.stride(2) != 1 and t.shape[2] > 1 and t.numel()):
-        raise MatMulError(f"{name} must be [rows, heads, head_dim] of {dtype} on {device} with unit last stride")
-    return _l.Rows(t.data_ptr(), t.stride(0), t.stride(1))
+def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, index: int):
+    """(address, token stride, head stride) of rows [token][head][head_dim]."""
+    st = t.stride()
+    if t.dtype != dtype or t.get_device() != index or len(st) != 3 or (st[2] != 1 and t.shape[2] > 1 and t.numel()):
+        raise MatMulError(f"{name} must be [rows, heads, head_dim] of {dtype} on cuda:{index} with unit last stride")
+    return t.data_ptr(), st[0], st[1]
 
 
-def _ints(t: Optional[torch.Tensor], name: str, n: Optional[int], device: torch.device) -> Optional[int]:
+def _ints(t: Optional[torch.Tensor], name: str, n: Optional[int], index: int) -> Optional[int]:
     if t is None:
         return None
-    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.device != device or (n is not None and t.numel() != n):
-        raise MatMulError(f"{name} must be contiguous int32{'' if n is None else f' [{n}]'} on {device}")
+    if t.dtype != torch.int32 or t.dim() != 1 or t.get_device() != index or not t.is_contiguous() or (n is not None and t.numel() != n):
+        raise MatMulError(f"{name} must be contiguous int32{'' if n is None else f' [{n}]'} on cuda:{index}")
     return t.data_ptr()
 
 
 def _output(out: Optional[torch.Tensor], q: torch.Tensor) -> torch.Tensor:
     if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
     if out.shape != q.shape:
         raise MatMulError(f"out has shape {tuple(out.shape)}, q {tuple(q.shape)}")
     return out
@@ -95,24 +100,30 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: in
     keys by ``k_offsets`` alike.  Without offsets each of `seqs` sequences (1 unless given) has as many rows.
     ``q_lens`` / ``k_lens`` (int32 [seqs]): only so many of a span's rows count, the others are padding.  Rows of no
     sequence are left as they are in `out`; a query that sees no key gives zeros."""
-    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+    sq, sk = q.shape, k.shape
+    if len(sq) != 3 or len(sk) != 3:
         raise MatMulError("q, k and v must be [rows, heads, head_dim]")
-    if k.shape != v.shape or q.shape[2] != k.shape[2] or q.shape[1] % max(1, k.shape[1]):
-        raise MatMulError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit together")
-    code, dev = _code(q, "q"), q.device
-    with _here(q, "q"):
-        if seqs is None:
-            seqs = next((t.numel() - d for t, d in ((q_offsets, 1), (k_offsets, 1), (q_lens, 0), (k_lens, 0)) if t is not None), 1)
-        out = _output(out, q)
-        rows = [_rows(t, n, q.dtype, dev) for t, n in ((q, "q"), (k, "k"), (v, "v"), (out, "out"))]
-        ptrs = [_ints(t, n, seqs + d, dev) for t, n, d in ((q_offsets, "q_offsets", 1), (k_offsets, "k_offsets", 1),
-                                                           (q_lens, "q_lens", 0), (k_lens, "k_lens", 0))]
-        nq, hq, d = q.shape
-        nk, hk = k.shape[:2]
-        need = _workspace_bytes(code, seqs, nq, nk, hq, hk, d, left, right, sinks)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        s = _stream(q, stream, out, ws)
-        _l.check(_l.load().nq_window_attention(
-            *(ctypes.byref(r) for r in rows), code, seqs, nq, nk, *ptrs, hq, hk, d, left, right, sinks,
-            d ** -0.5 if scale is None else scale, ws.data_ptr() if need else None, need, s))
+    nq, hq, d = sq
+    nk, hk, dk = sk
+    if v.shape != sk or dk != d or hk == 0 or hq % hk:
+        raise MatMulError(f"q {tuple(sq)}, k {tuple(sk)} and v {tuple(v.shape)} do not fit together")
+    dtype = q.dtype
+    code, dev = _code(q, "q"), _device(q, "q")
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return window_attention(q, k, v, left, right, sinks, scale, q_offsets, k_offsets, q_lens, k_lens, seqs, out, stream)
+    if seqs is None:
+        seqs = (q_offsets.numel() - 1 if q_offsets is not None else k_offsets.numel() - 1 if k_offsets is not None else
+                q_lens.numel() if q_lens is not None else k_lens.numel() if k_lens is not None else 1)
+    out = _output(out, q)
+    rows = _Quad(_rows(q, "q", dtype, dev), _rows(k, "k", dtype, dev), _rows(v, "v", dtype, dev), _rows(out, "out", dtype, dev))
+    need = _workspace_bytes(code, seqs, nq, nk, hq, hk, d, left, right, sinks)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    rc = _l.load().nq_window_attention(
+        rows, _ref(rows, 24), _ref(rows, 48), _ref(rows, 72), code, seqs, nq, nk, _ints(q_offsets, "q_offsets", seqs + 1, dev),
+        _ints(k_offsets, "k_offsets", seqs + 1, dev), _ints(q_lens, "q_lens", seqs, dev), _ints(k_lens, "k_lens", seqs, dev),
+        hq, hk, d, left, right, sinks, d ** -0.5 if scale is None else scale, ws.data_ptr() if need else None, need,
+        _stream(dev, stream, out, ws))
+    if rc:
+        _l.check(rc)
     return out

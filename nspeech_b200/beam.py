@@ -14,7 +14,7 @@ from typing import List, Optional, Sequence, Tuple
 import torch
 
 from . import lib as _l
-from .attention import _code, _here, _ints, _stream
+from .attention import _code, _device, _ints, _stream
 from .fast_matmul import MatMulError
 
 
@@ -26,11 +26,12 @@ def _workspace_bytes(items: int, beams: int, vocab: int) -> int:
     return n
 
 
-def _pair(t: Optional[torch.Tensor], name: str, shape, dtypes, device) -> Optional[int]:
-    if t is None:
-        return None
-    if tuple(t.shape) != shape or t.dtype not in dtypes or t.device != device or not t.is_contiguous():
-        raise MatMulError(f"{name} must be contiguous {list(shape)} of {' or '.join(str(d) for d in dtypes)} on {device}")
+_FLAGS = (torch.bool, torch.uint8)
+
+
+def _pair(t: torch.Tensor, name: str, shape, dtypes, index: int) -> int:
+    if t.shape != shape or t.dtype not in dtypes or t.get_device() != index or not t.is_contiguous():
+        raise MatMulError(f"{name} must be contiguous {list(shape)} of {' or '.join(str(d) for d in dtypes)} on cuda:{index}")
     return t.data_ptr()
 
 
@@ -46,23 +47,35 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: Optional[t
     if logits.dim() != 3:
         raise MatMulError("logits must be [items, beams, vocab]")
     items, beams, vocab = logits.shape
-    code, dev = _code(logits, "logits"), logits.device
-    if vocab > 1 and logits.stride(2) != 1 or items > 1 and logits.stride(0) != beams * logits.stride(1):
+    by = logits.stride()
+    if vocab > 1 and by[2] != 1 or items > 1 and by[0] != beams * by[1]:
         raise MatMulError("logits must have unit stride along the vocabulary and evenly spaced rows")
-    ld = logits.stride(1) if beams > 1 else logits.stride(0) if items > 1 else vocab
-    pair, flags = (items, beams), (torch.bool, torch.uint8)
-    with _here(logits, "logits"):
-        need = _workspace_bytes(items, beams, vocab)
-        if out is None:
-            out = (torch.empty(pair, dtype=torch.float32, device=dev), torch.empty(pair, dtype=torch.int32, device=dev),
-                   torch.empty(pair, dtype=torch.int32, device=dev), torch.empty(pair, dtype=torch.bool, device=dev))
-        ptrs = (_pair(scores, "scores", pair, (torch.float32,), dev), _pair(finished, "finished", pair, flags, dev))
-        outs = [_pair(t, n, pair, d, dev) for t, n, d in zip(out, ("out scores", "out parents", "out tokens", "out finished"),
-                                                             ((torch.float32,), (torch.int32,), (torch.int32,), flags))]
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        s = _stream(logits, stream, ws, *out)
-        _l.check(_l.load().nq_beam_select(logits.data_ptr(), code, ld, items, beams, vocab, ptrs[0], ptrs[1], eos, *outs,
-                                          ws.data_ptr(), need, s))
+    code, dev = _code(logits, "logits"), _device(logits, "logits")
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return beam_select(logits, scores, finished, eos, out, stream)
+    pair = (items, beams)
+    need = _workspace_bytes(items, beams, vocab)
+    p_scores = _pair(scores, "scores", pair, (torch.float32,), dev)
+    p_finished = _pair(finished, "finished", pair, _FLAGS, dev) if finished is not None else None
+    if out is None:
+        n = items * beams
+        # one allocation for the outputs and the workspace: three rows of 32-bit words, the flags, then 8-byte entries
+        at = (13 * n + 7) // 8 * 8
+        buf = torch.empty(at + need, dtype=torch.uint8, device=logits.device)
+        words = buf[:12 * n].view(torch.int32).view(3, items, beams)
+        out = words[0].view(torch.float32), words[1], words[2], buf[12 * n:13 * n].view(torch.bool).view(items, beams)
+        base = buf.data_ptr()
+        p_out, p_ws, made = (base, base + 4 * n, base + 8 * n, base + 12 * n), base + at, buf
+    else:
+        p_out = [_pair(t, f"out[{i}]", pair, d, dev) for i, (t, d) in enumerate(zip(out, ((torch.float32,), (torch.int32,),
+                                                                                         (torch.int32,), _FLAGS)))]
+        made = torch.empty(need, dtype=torch.uint8, device=logits.device)
+        p_ws = made.data_ptr()
+    rc = _l.load().nq_beam_select(logits.data_ptr(), code, by[1] if beams > 1 else by[0] if items > 1 else vocab, items, beams, vocab,
+                                  p_scores, p_finished, eos, *p_out, p_ws, need, _stream(dev, stream, made))
+    if rc:
+        _l.check(rc)
     return out
 
 
@@ -70,29 +83,46 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, out: Opt
                  stream: Optional[torch.cuda.Stream] = None) -> List[torch.Tensor]:
     """out[i][r] = states[i][parents[r]] for every state (any dtype, [rows, ...] with contiguous rows), in one launch for
     up to 16 states.  parents: int32, `rows` of them in any shape (``beam_select``'s).  out[i] may be states[i]."""
-    states = list(states)
     if not states:
         return []
-    rows, dev = parents.numel(), parents.device
-    ptr = _ints(parents.reshape(-1) if parents.is_contiguous() else parents, "parents", rows, dev)
-    with _here(parents, "parents"):
-        made = out is None
-        out = [torch.empty_like(t, memory_format=torch.contiguous_format) for t in states] if made else list(out)
-        if len(out) != len(states):
-            raise MatMulError(f"{len(out)} outputs for {len(states)} states")
-        for t, o in zip(states, out):
-            for x in (t, o):
-                if x.dim() < 1 or x.shape[0] != rows or x.device != dev or x.dtype != t.dtype or x.shape != t.shape:
-                    raise MatMulError(f"a state must be [{rows}, ...] on {dev}, like its output")
-                if rows and not x[0].is_contiguous():
-                    raise MatMulError("a state's rows must be contiguous")
-        size = [t.numel() // rows * t.element_size() if rows else 0 for t in states]
-        s = _stream(parents, stream, *(out if made else ()))
-        for i in range(0, len(states), 16):
-            part = [j for j in range(i, min(i + 16, len(states))) if size[j]]
-            m = len(part)
-            P, I = ctypes.c_void_p * m, ctypes.c_int64 * m
-            stride = [[x[j].stride(0) * x[j].element_size() if rows > 1 else size[j] for j in part] for x in (states, out)]
-            _l.check(_l.load().nq_beam_reorder(P(*(states[j].data_ptr() for j in part)), P(*(out[j].data_ptr() for j in part)),
-                                               I(*(size[j] for j in part)), I(*stride[0]), I(*stride[1]), m, rows, ptr, s))
+    rows, dev = parents.numel(), _device(parents, "parents")
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return beam_reorder(states, parents, out, stream)
+    ptr = _ints(parents.view(-1) if parents.is_contiguous() else parents, "parents", rows, dev)
+    made = out is None
+    out = [torch.empty_like(t, memory_format=torch.contiguous_format) for t in states] if made else list(out)
+    if len(out) != len(states):
+        raise MatMulError(f"{len(out)} outputs for {len(states)} states")
+    src, dst, size, src_by, dst_by = [], [], [], [], []
+    for t, o in zip(states, out):
+        shape = t.shape
+        if not shape or shape[0] != rows or t.get_device() != dev or o.get_device() != dev or o.dtype != t.dtype or o.shape != shape:
+            raise MatMulError(f"a state must be [{rows}, ...] on cuda:{dev}, like its output")
+        n = t.numel()
+        if n == 0:
+            continue
+        each = t.element_size()
+        row = n // rows * each
+        by = []
+        for x in (t, o):
+            if x.is_contiguous():
+                by.append(row)
+            elif x[0].is_contiguous():
+                by.append(x.stride(0) * each if rows > 1 else row)
+            else:
+                raise MatMulError("a state's rows must be contiguous")
+        src.append(t.data_ptr())
+        dst.append(o.data_ptr())
+        size.append(row)
+        src_by.append(by[0])
+        dst_by.append(by[1])
+    s = _stream(dev, stream, *(out if made else ()))
+    for i in range(0, len(src), 16):
+        m = min(16, len(src) - i)
+        a = (ctypes.c_int64 * (5 * m))(*src[i:i + m], *dst[i:i + m], *size[i:i + m], *src_by[i:i + m], *dst_by[i:i + m])
+        rc = _l.load().nq_beam_reorder(a, ctypes.byref(a, 8 * m), ctypes.byref(a, 16 * m), ctypes.byref(a, 24 * m),
+                                       ctypes.byref(a, 32 * m), m, rows, ptr, s)
+        if rc:
+            _l.check(rc)
     return out

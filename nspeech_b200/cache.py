@@ -17,7 +17,7 @@ from typing import Optional
 import torch
 
 from . import lib as _l
-from .attention import _code, _here, _ints, _output, _rows, _stream
+from .attention import _Pair, _code, _device, _ints, _output, _ref, _rows, _stream
 from .fast_matmul import MatMulError
 
 
@@ -40,11 +40,11 @@ class PagedCache:
         for t, name in ((table, "table"), (lens, "lens"), (refs, "refs")):
             if t.dtype != torch.int32:
                 raise MatMulError(f"{name} must be int32")
-        with _here(k, "k"):
-            ints = _l.load().nq_cache_state_ints(slots, pages)
-            if ints < 0:
-                _l.check(int(ints))
-            self.state = torch.zeros(ints, dtype=torch.int32, device=k.device)
+        self._dev = _device(k, "k")
+        ints = _l.load().nq_cache_state_ints(slots, pages)
+        if ints < 0:
+            _l.check(int(ints))
+        self.state = torch.zeros(ints, dtype=torch.int32, device=k.device)
         self.k, self.v, self.table, self.lens, self.refs = k, v, table, lens, refs
         self.device = k.device
         self._c = _l.Cache(k.data_ptr(), v.data_ptr(), table.data_ptr(), lens.data_ptr(), refs.data_ptr(), self.state.data_ptr(),
@@ -70,11 +70,21 @@ class PagedCache:
         """Live pages as of the last ``compact``: a CUDA int32 [1]."""
         return self.state[1:2]
 
+    def _call(self, fn, *args) -> None:
+        """A call with this cache's device as the current one."""
+        if torch.cuda.current_device() == self._dev:
+            rc = fn(self._p, *args)
+        else:
+            with torch.cuda.device(self._dev):
+                rc = fn(self._p, *args)
+        if rc:
+            _l.check(rc)
+
     def _range(self, new, first: int, n: Optional[int]):
         """New tokens per slot: (offsets pointer, tokens each, slots)."""
         if isinstance(new, torch.Tensor):
             n = new.numel() - 1 if n is None else n
-            return _ints(new, "offsets", n + 1, self.device), 0, n
+            return _ints(new, "offsets", n + 1, self._dev), 0, n
         return None, int(new), self.slots - first if n is None else n
 
     # ------------------------------------------------------------------ pages
@@ -82,52 +92,47 @@ class PagedCache:
         """Room for new tokens of slots [first, first + n): `tokens` each, or offsets [n + 1] (CUDA int32) whose
         differences are their numbers.  Takes the lowest free pages in slot order; a shared partial last page is copied."""
         off, each, n = self._range(tokens, first, n)
-        with _here(self.k, "k"):
-            _l.check(_l.load().nq_cache_reserve(self._p, first, n, off, each, _stream(self.k, stream)))
+        self._call(_l.load().nq_cache_reserve, first, n, off, each, _stream(self._dev, stream))
 
     def write(self, k: torch.Tensor, v: torch.Tensor, tokens, first: int = 0, n: Optional[int] = None, layer: int = 0,
               stream: Optional[torch.cuda.Stream] = None) -> None:
         """The reserved tokens' keys and values, [rows, kv_heads, head_dim] for `layer` or [layers, rows, kv_heads,
         head_dim] for the layers from `layer` on; `tokens` as in ``reserve``."""
         off, each, n = self._range(tokens, first, n)
-        if k.shape != v.shape or k.dim() not in (3, 4) or tuple(k.shape[-2:]) != (self._c.kv_heads, self._c.head_dim):
+        shape, dtype = k.shape, self.k.dtype
+        if shape != v.shape or len(shape) not in (3, 4) or shape[-2] != self._c.kv_heads or shape[-1] != self._c.head_dim:
             raise MatMulError(f"k and v must be [(layers,) rows, {self._c.kv_heads}, {self._c.head_dim}]")
-        many = k.dim() == 4
-        layers, rows = (k.shape[0] if many else 1), k.shape[-3]
-        sides = [_rows(t[0] if many and layers else t.reshape(0, *k.shape[-2:]) if many else t, name, self.k.dtype, self.device)
-                 for t, name in ((k, "k"), (v, "v"))]
-        strides = (k.stride(0), v.stride(0)) if many else (0, 0)
-        with _here(self.k, "k"):
-            _l.check(_l.load().nq_cache_write(self._p, ctypes.byref(sides[0]), ctypes.byref(sides[1]), *strides, layer, layers,
-                                              rows, first, n, off, each, _stream(self.k, stream)))
+        if len(shape) == 4:
+            layers, by = shape[0], (k.stride(0), v.stride(0))
+            if layers == 0:
+                return
+            k, v = k[0], v[0]
+        else:
+            layers, by = 1, (0, 0)
+        rows = _Pair(_rows(k, "k", dtype, self._dev), _rows(v, "v", dtype, self._dev))
+        self._call(_l.load().nq_cache_write, rows, _ref(rows, 24), *by, layer, layers, shape[-3], first, n, off, each,
+                   _stream(self._dev, stream))
 
     def fork(self, src: torch.Tensor, first: int = 0, stream: Optional[torch.cuda.Stream] = None) -> None:
         """Slots [first, first + len(src)) become what slots `src` (CUDA int32) were before; -1 frees."""
-        ptr = _ints(src, "src", None, self.device)
-        with _here(self.k, "k"):
-            _l.check(_l.load().nq_cache_fork(self._p, first, src.numel(), ptr, _stream(self.k, stream)))
+        self._call(_l.load().nq_cache_fork, first, src.numel(), _ints(src, "src", None, self._dev), _stream(self._dev, stream))
 
     def free(self, first: int = 0, n: Optional[int] = None, stream: Optional[torch.cuda.Stream] = None) -> None:
         """Empties slots [first, first + n)."""
-        with _here(self.k, "k"):
-            _l.check(_l.load().nq_cache_fork(self._p, first, self.slots - first if n is None else n, None, _stream(self.k, stream)))
+        self._call(_l.load().nq_cache_fork, first, self.slots - first if n is None else n, None, _stream(self._dev, stream))
 
     def trim(self, window: int, sinks: int = 0, first: int = 0, n: Optional[int] = None,
              stream: Optional[torch.cuda.Stream] = None) -> None:
         """Gives back pages that hold neither one of a slot's first `sinks` tokens nor one of its last `window`."""
-        with _here(self.k, "k"):
-            _l.check(_l.load().nq_cache_trim(self._p, first, self.slots - first if n is None else n, sinks, window,
-                                             _stream(self.k, stream)))
+        self._call(_l.load().nq_cache_trim, first, self.slots - first if n is None else n, sinks, window, _stream(self._dev, stream))
 
     def compact(self, stream: Optional[torch.cuda.Stream] = None) -> None:
         """Moves the live pages to the lowest numbers (``live`` of them); tables follow."""
-        with _here(self.k, "k"):
-            _l.check(_l.load().nq_cache_compact(self._p, _stream(self.k, stream)))
+        self._call(_l.load().nq_cache_compact, _stream(self._dev, stream))
 
     def check(self, stream: Optional[torch.cuda.Stream] = None) -> None:
         """Synchronises and raises NqError if a call since the last check could not be done."""
-        with _here(self.k, "k"):
-            _l.check(_l.load().nq_cache_status(self._p, None, _stream(self.k, stream)))
+        self._call(_l.load().nq_cache_status, None, _stream(self._dev, stream))
 
     # -------------------------------------------------------------- attention
     def attention(self, q: torch.Tensor, layer: int, offsets: Optional[torch.Tensor] = None, first: int = 0,
@@ -135,26 +140,25 @@ class PagedCache:
                   out: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
         """Attention of q [rows, q_heads, head_dim], the last tokens of slots [first, first + n) (offsets [n + 1], or the
         same number each), over their cached tokens; window and sinks as in ``window_attention``."""
-        if q.dim() != 3 or q.shape[2] != self._c.head_dim or q.shape[1] % self._c.kv_heads:
+        sq, dtype = q.shape, self.k.dtype
+        if len(sq) != 3 or sq[2] != self._c.head_dim or sq[1] % self._c.kv_heads:
             raise MatMulError(f"q must be [rows, a multiple of {self._c.kv_heads} heads, {self._c.head_dim}]")
         if n is None:
             n = offsets.numel() - 1 if offsets is not None else self.slots - first
-        off = _ints(offsets, "offsets", n + 1, self.device)
-        with _here(self.k, "k"):
-            out = _output(out, q)
-            rows = [_rows(t, name, self.k.dtype, self.device) for t, name in ((q, "q"), (out, "out"))]
-            key = (n, q.shape[0], q.shape[1], left, right, sinks)
-            need = self._ws.get(key)
-            if need is None:
-                need = _l.load().nq_cache_attention_workspace(self._p, *key)
-                if need < 0:
-                    _l.check(int(need))
-                if len(self._ws) > 4096:
-                    self._ws.clear()
-                self._ws[key] = need
-            ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-            s = _stream(self.k, stream, out, ws)
-            _l.check(_l.load().nq_cache_attention(
-                self._p, layer, ctypes.byref(rows[0]), ctypes.byref(rows[1]), first, n, q.shape[0], off, q.shape[1], left, right,
-                sinks, q.shape[2] ** -0.5 if scale is None else scale, ws.data_ptr() if need else None, need, s))
+        out = _output(out, q)
+        rows = _Pair(_rows(q, "q", dtype, self._dev), _rows(out, "out", dtype, self._dev))
+        key = (n, sq[0], sq[1], left, right, sinks)
+        need = self._ws.get(key)
+        if need is None:
+            need = _l.load().nq_cache_attention_workspace(self._p, *key)
+            if need < 0:
+                _l.check(int(need))
+            if len(self._ws) > 4096:
+                self._ws.clear()
+            self._ws[key] = need
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        self._call(_l.load().nq_cache_attention, layer, rows, _ref(rows, 24), first, n, sq[0],
+                   _ints(offsets, "offsets", n + 1, self._dev), sq[1], left, right, sinks,
+                   sq[2] ** -0.5 if scale is None else scale, ws.data_ptr() if need else None, need,
+                   _stream(self._dev, stream, out, ws))
         return out

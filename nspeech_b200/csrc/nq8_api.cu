@@ -1139,6 +1139,24 @@ int device_info(int *sm_count, DevCtl *ctl) {
   return NQ_OK;
 }
 
+int tensor_map(CUtensorMap *map, const void *ptr, int rank, const uint64_t *dims, const uint64_t *strides, const uint32_t *box) {
+  DeviceCtx *ctx = nullptr;
+  const int rc = current_ctx(&ctx, nullptr);
+  if (rc) return rc;
+  cuuint64_t d[3], st[2];
+  cuuint32_t b[3], one[3] = {1, 1, 1};
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    b[i] = box[i];
+    if (i + 1 < rank) st[i] = strides[i];
+  }
+  const CUresult r = ctx->encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void *>(ptr), d, st, b, one,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(NQ_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+  return NQ_OK;
+}
+
 bool attention_tc(int Tp) { return g_attention_kernel == NQ_ATTENTION_TCGEN05 && Tp <= attention_tc_max_tp(); }
 
 int layer_norm_rows(int mode, float *x, const void *u, float alpha, int rows, int D, const float *g1, const float *b1,

@@ -13,7 +13,10 @@
 #include "nq8_window_attention.h"
 
 namespace nq {
-int device_info(int *sm_count, DevCtl *ctl);  // of the current device (nq8_api.cu)
+// nq8_api.cu, for the current device: its SMs and control block; a tensor map
+// of bf16 elements with the 128-byte swizzle (strides in bytes, innermost 1).
+int device_info(int *sm_count, DevCtl *ctl);
+int tensor_map(CUtensorMap *map, const void *ptr, int rank, const uint64_t *dims, const uint64_t *strides, const uint32_t *box);
 }
 
 namespace {
@@ -97,16 +100,61 @@ nq::CacheView view(const nq_cache *c) {
   return v;
 }
 
+// Rows that a tensor map takes: 16-byte aligned address and strides (a single
+// head or row needs no stride).
+struct MapRows {
+  const void *ptr;
+  int64_t ts, hs;
+  int rows, heads;
+  bool fits() const {
+    return aligned(ptr, 16) && rows > 0 && (heads == 1 || (hs > 0 && hs % 8 == 0)) && (rows == 1 || (ts > 0 && ts % 8 == 0));
+  }
+  int make(CUtensorMap *m, int dim, int box_heads, int box_rows) const {
+    const uint64_t dims[3] = {static_cast<uint64_t>(dim), static_cast<uint64_t>(heads), static_cast<uint64_t>(rows)};
+    const uint64_t any = static_cast<uint64_t>(dim) * 2;
+    const uint64_t strides[2] = {heads == 1 ? any : static_cast<uint64_t>(hs) * 2, rows == 1 ? any : static_cast<uint64_t>(ts) * 2};
+    const uint32_t box[3] = {64, static_cast<uint32_t>(box_heads), static_cast<uint32_t>(box_rows)};
+    return nq::tensor_map(m, ptr, 3, dims, strides, box);
+  }
+};
+
+// The tensor maps of the tensor-core form; *fits: whether the call is one that
+// it takes (its sizes, 16-byte alignment, a positive scale).
+int tensor_maps(const nq::WinAttnParams &p, int dtype, CUtensorMap *tq, CUtensorMap *tk, CUtensorMap *tv, bool *fits) {
+  *fits = false;
+  const int heads = p.kv_heads * p.group;
+  const MapRows q{p.q, p.q_ts, p.q_hs, p.q_rows, heads}, out{p.out, p.o_ts, p.o_hs, p.q_rows, heads};
+  if (p.dim % 8 || !(p.sl2 > 0.f) || !nq::win_attn_tc_fits(dtype == NQ_F32, p.seqs, p.q_rows, p.group) || !q.fits() || !out.fits())
+    return NQ_OK;
+  int rc;
+  if (p.table) {
+    const int64_t rows = (static_cast<int64_t>(p.pages) * p.kv_heads) << p.page_shift;
+    if (rows > INT32_MAX) return NQ_OK;
+    const uint64_t dims[2] = {static_cast<uint64_t>(p.dim), static_cast<uint64_t>(rows)}, stride[1] = {static_cast<uint64_t>(p.dim) * 2};
+    const uint32_t box[2] = {64, static_cast<uint32_t>(1 << p.page_shift < nq::kWinTcKeys ? 1 << p.page_shift : nq::kWinTcKeys)};
+    if ((rc = nq::tensor_map(tk, p.k, 2, dims, stride, box)) || (rc = nq::tensor_map(tv, p.v, 2, dims, stride, box))) return rc;
+  } else {
+    const MapRows k{p.k, p.k_ts, p.k_hs, p.k_rows, p.kv_heads}, v{p.v, p.v_ts, p.v_hs, p.k_rows, p.kv_heads};
+    if (!k.fits() || !v.fits()) return NQ_OK;
+    if ((rc = k.make(tk, p.dim, 1, nq::kWinTcKeys)) || (rc = v.make(tv, p.dim, 1, nq::kWinTcKeys))) return rc;
+  }
+  if ((rc = q.make(tq, p.dim, p.group, 128 / p.group))) return rc;
+  *fits = true;
+  return NQ_OK;
+}
+
 int run_attention(const char *who, nq::WinAttnParams &p, int dtype, int64_t key_bound, void *workspace, int64_t workspace_bytes,
                   void *stream) {
   int sm = 0;
-  const int rc = nq::device_info(&sm, &p.ctl);
+  int rc = nq::device_info(&sm, &p.ctl);
   if (rc) return rc;
-  const bool uniform = !p.q_off && !p.q_len;
-  nq::WinAttnPlan pl = nq::win_attn_plan(sm, dtype == NQ_F32, uniform, p.seqs, p.q_rows, key_bound, p.kv_heads, p.group, p.dim,
-                                         p.left, p.right, p.sinks);
-  if (!workspace) pl.splits = 1;
-  if (pl.splits > 1) {
+  CUtensorMap tq, tk, tv;
+  bool tensor = false;
+  if ((rc = tensor_maps(p, dtype, &tq, &tk, &tv, &tensor))) return rc;
+  const nq::WinAttnPlan pl = nq::win_attn_plan(sm, dtype == NQ_F32, tensor, !p.q_off && !p.q_len, p.seqs, p.q_rows, key_bound,
+                                               p.kv_heads, p.group, p.dim, p.left, p.right, p.sinks);
+  p.splits = workspace ? pl.splits : 1;
+  if (p.splits > 1) {
     if (static_cast<size_t>(workspace_bytes < 0 ? 0 : workspace_bytes) < pl.workspace)
       return bad(NQ_ERR_SHAPE, "%s: a workspace of %lld bytes, %zu are needed", who, (long long)workspace_bytes, pl.workspace);
     if (!aligned(workspace, 16)) return bad(NQ_ERR_ALIGN, "%s: the workspace must be 16-byte aligned", who);
@@ -114,8 +162,22 @@ int run_attention(const char *who, nq::WinAttnParams &p, int dtype, int64_t key_
     p.part_o = static_cast<float *>(workspace);
     p.part_ml = reinterpret_cast<float2 *>(p.part_o + rows * (p.dim <= 64 ? 64 : 128));
   }
-  p.splits = pl.splits;
-  return done(nq::launch_win_attn(p, dtype == NQ_F32, pl, static_cast<cudaStream_t>(stream)), who);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return done(tensor ? nq::launch_win_attn_tc(tq, tk, tv, p, pl, s) : nq::launch_win_attn(p, dtype == NQ_F32, pl, s), who);
+}
+
+// The larger of the two forms' workspaces: which one runs depends on addresses.
+int64_t attention_workspace(int dtype, int seqs, int64_t q_rows, int64_t key_bound, const Heads &h, int left, int right, int sinks) {
+  if (seqs == 0 || q_rows == 0) return 0;
+  const int sm = sms(), group = h.q / h.kv, n = static_cast<int>(q_rows);
+  size_t most = 0;
+  for (const bool tensor : {false, true})
+    if (!tensor || nq::win_attn_tc_fits(dtype == NQ_F32, seqs, n, group)) {
+      const size_t w = nq::win_attn_plan(sm, dtype == NQ_F32, tensor, false, seqs, n, key_bound, h.kv, group, h.dim, limit(left),
+                                         limit(right), sinks).workspace;
+      most = w > most ? w : most;
+    }
+  return static_cast<int64_t>(most);
 }
 
 }  // namespace
@@ -127,9 +189,7 @@ int64_t nq_window_attention_workspace(int dtype, int seqs, int64_t q_rows, int64
   const Heads h{q_heads, kv_heads, head_dim};
   const int rc = check_attention("nq_window_attention_workspace", dtype, seqs, q_rows, h, sinks, false);
   if (rc) return rc;
-  if (seqs == 0 || q_rows == 0) return 0;
-  return static_cast<int64_t>(nq::win_attn_plan(sms(), dtype == NQ_F32, false, seqs, static_cast<int>(q_rows), k_rows / seqs, kv_heads,
-                                                q_heads / kv_heads, head_dim, limit(left), limit(right), sinks).workspace);
+  return attention_workspace(dtype, seqs, q_rows, seqs ? k_rows / seqs : 0, h, left, right, sinks);
 }
 
 int nq_window_attention(const nq_rows *q, const nq_rows *k, const nq_rows *v, const nq_rows *out, int dtype, int seqs, int64_t q_rows,
@@ -192,10 +252,7 @@ int64_t nq_cache_attention_workspace(const nq_cache *c, int seqs, int64_t q_rows
   const Heads h{q_heads, c->kv_heads, c->head_dim};
   rc = check_attention(who, c->dtype, seqs, q_rows, h, sinks, false);
   if (rc) return rc;
-  if (seqs == 0 || q_rows == 0) return 0;
-  return static_cast<int64_t>(nq::win_attn_plan(sms(), c->dtype == NQ_F32, false, seqs, static_cast<int>(q_rows),
-                                                static_cast<int64_t>(c->max_pages) * c->page_tokens, c->kv_heads,
-                                                q_heads / c->kv_heads, c->head_dim, limit(left), limit(right), sinks).workspace);
+  return attention_workspace(c->dtype, seqs, q_rows, static_cast<int64_t>(c->max_pages) * c->page_tokens, h, left, right, sinks);
 }
 
 int nq_cache_attention(const nq_cache *c, int layer, const nq_rows *q, const nq_rows *out, int first, int n, int64_t q_rows,

@@ -18,18 +18,15 @@
 #include <math.h>
 #include <stdint.h>
 
-#include "nq8_window_attention.h"
+#include "nq8_window_attention.cuh"
 
 namespace nq {
 namespace {
 
+using namespace win;
+
 constexpr int kThreads = 128;
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // 16-byte copy global -> shared; zeros where !there (src is not read).
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
@@ -50,102 +47,6 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(a)
                : "memory");
-}
-
-// One sequence: its first query row, its queries, first key row (plain rows)
-// and keys.
-struct Seq {
-  int q0, nq, k0, nk;
-};
-__device__ __forceinline__ void span(const int *off, const int *len, int rows, int seqs, int b, int &begin, int &n) {
-  int e;
-  if (off) {
-    begin = min(max(__ldg(off + b), 0), rows);
-    e = min(max(__ldg(off + b + 1), begin), rows);
-  } else {
-    const int each = rows / seqs;
-    begin = b * each;
-    e = begin + each;
-  }
-  n = e - begin;
-  if (len) n = min(n, max(__ldg(len + b), 0));
-}
-__device__ __forceinline__ Seq seq_of(const WinAttnParams &p, int b) {
-  Seq s;
-  span(p.q_off, p.q_len, p.q_rows, p.seqs, b, s.q0, s.nq);
-  if (p.table) {
-    s.k0 = 0;
-    s.nk = static_cast<int>(min(static_cast<long long>(max(__ldg(p.k_len + b), 0)),
-                                static_cast<long long>(p.max_pages) << p.page_shift));
-  } else {
-    span(p.k_off, p.k_len, p.k_rows, p.seqs, b, s.k0, s.nk);
-  }
-  return s;
-}
-// The row tile `tile` of all sequences' tiles of `rows` rows: sequence and
-// first row in it.  Every warp finds it by itself, 32 sequences at a time.
-__device__ __forceinline__ bool find_tile(const WinAttnParams &p, int tile, int rows, int &b, int &row0) {
-  if (!p.q_off && !p.q_len) {
-    const int per = ((p.q_rows / p.seqs) * p.group + rows - 1) / rows;
-    b = per ? tile / per : p.seqs;
-    row0 = per ? (tile - b * per) * rows : 0;
-    return b < p.seqs;
-  }
-  const int lane = threadIdx.x & 31;
-  int done = 0;
-  for (int base = 0; base < p.seqs; base += 32) {
-    int n = 0;
-    if (base + lane < p.seqs) {
-      int q0, nq;
-      span(p.q_off, p.q_len, p.q_rows, p.seqs, base + lane, q0, nq);
-      n = (nq * p.group + rows - 1) / rows;
-    }
-    int upto = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += x;
-    }
-    const int all = __shfl_sync(0xffffffffu, upto, 31);
-    if (tile < done + all) {
-      const unsigned m = __ballot_sync(0xffffffffu, tile < done + upto);
-      const int w = __ffs(m) - 1;
-      b = base + w;
-      row0 = (tile - done - __shfl_sync(0xffffffffu, upto - n, w)) * rows;
-      return true;
-    }
-    done += all;
-  }
-  return false;
-}
-
-// The keys of a row tile: the sinks [0, s_end) and the window [lo, hi].
-struct Keys {
-  int lo, hi, s_end;  // s_end = 0 where the window's tiles hold the sinks too
-  int sink_tiles, tiles;
-};
-template <int KT>
-__device__ __forceinline__ Keys keys_of(const WinAttnParams &p, const Seq &s, int i_first, int i_last) {
-  Keys k;
-  const int p_lo = s.nk - s.nq + i_first, p_hi = s.nk - s.nq + i_last;
-  k.hi = p.right >= kWinUnlimited ? s.nk - 1 : min(s.nk - 1, p_hi + p.right);
-  k.lo = p.left >= kWinUnlimited ? 0 : max(0, p_lo - p.left);
-  k.s_end = max(0, min(min(p.sinks, k.lo), k.hi + 1));
-  k.sink_tiles = (k.s_end + KT - 1) / KT;
-  if (k.lo <= k.sink_tiles * KT) {  // the two parts touch: one run of tiles
-    if (k.s_end > 0) k.lo = 0;
-    k.s_end = 0;
-    k.sink_tiles = 0;
-  }
-  k.tiles = k.sink_tiles + (k.hi >= k.lo ? (k.hi - k.lo + KT) / KT : 0);
-  return k;
-}
-template <int KT>
-__device__ __forceinline__ int tile_base(const Keys &k, int t) {
-  return t < k.sink_tiles ? t * KT : k.lo + (t - k.sink_tiles) * KT;
-}
-__device__ __forceinline__ bool key_there(const Keys &k, int j) {
-  return j <= k.hi && (j >= k.lo || j < k.s_end);
 }
 
 // Element offset of key j's row for kv head h; -1 where the key's page is
@@ -882,7 +783,7 @@ cudaError_t launch_smem(dim3 grid, size_t smem, cudaStream_t stream, const WinAt
 
 template <int DP, bool PAGED, bool VEC>
 cudaError_t launch_form(const WinAttnParams &p, int f32, const WinAttnPlan &pl, cudaStream_t stream) {
-  const dim3 grid(pl.tiles, p.kv_heads, pl.splits);
+  const dim3 grid(pl.tiles, p.kv_heads, p.splits);
   constexpr int kDeep = DP == 64 ? 4 : 3;
   if (f32) {
     if (pl.rows == 1) return launch_smem<win_attn_f32_rows<DP, 1, PAGED, VEC>>(grid, 0, stream, p);
@@ -901,12 +802,22 @@ bool aligned16(const void *x, int64_t a, int64_t b, int size) {
 
 }  // namespace
 
-WinAttnPlan win_attn_plan(int sm_count, int f32, bool uniform, int seqs, int q_rows, int64_t key_bound, int kv_heads, int group, int dim,
-                          int left, int right, int sinks) {
+// The tensor-core form takes 256 rows a CTA and wins from about 32 rows of a
+// sequence and kv head on (B200, 10 heads of 64: 40 rows 6.1 against 7.1 us,
+// 16 rows 5.9 against 4.9; 24 sequences of 20 rows 13.1 against 7.1, of 70
+// rows 13.9 against 17.4; long prompts 2.5 to 4.7 times faster).
+bool win_attn_tc_fits(int f32, int seqs, int q_rows, int group) {
+  return !f32 && group <= 128 && static_cast<int64_t>(q_rows) * group > 32 * static_cast<int64_t>(seqs);
+}
+
+WinAttnPlan win_attn_plan(int sm_count, int f32, bool tensor, bool uniform, int seqs, int q_rows, int64_t key_bound, int kv_heads,
+                          int group, int dim, int left, int right, int sinks) {
   WinAttnPlan pl;
   const int64_t rows = static_cast<int64_t>(q_rows) * group;
   const int64_t mean = (rows + seqs - 1) / seqs;  // rows of a sequence and kv head
-  if (f32) {
+  if (tensor) {
+    pl.rows = 2 * (128 / group * group);
+  } else if (f32) {
     pl.rows = mean <= 1 ? 1 : mean <= 2 ? 2 : mean <= 4 ? 4 : 64;
   } else {
     pl.rows = mean <= 16 ? 16 : mean <= 32 ? 32 : 64;
@@ -917,15 +828,27 @@ WinAttnPlan win_attn_plan(int sm_count, int f32, bool uniform, int seqs, int q_r
   int64_t keys = key_bound;
   if (left < kWinUnlimited && right < kWinUnlimited)
     keys = keys < static_cast<int64_t>(left) + right + sinks + pl.rows ? keys : static_cast<int64_t>(left) + right + sinks + pl.rows;
-  const int64_t have = ((rows + pl.rows - 1) / pl.rows > seqs ? (rows + pl.rows - 1) / pl.rows : seqs) * kv_heads;
-  const int64_t want = 2LL * sm_count;
+  const int64_t each = (rows + pl.rows - 1) / pl.rows;
+  const int64_t have = (each > seqs ? each : seqs) * kv_heads;
+  // Two CTAs an SM of the warp-level forms, of at least 256 keys; one of the
+  // tensor-core form, of at least 1024 (it fills and drains in the time of 256).
+  const int64_t want = tensor ? sm_count : 2LL * sm_count;
   int64_t z = have > 0 ? want / have : 1;
-  const int64_t most = keys / 256;  // at least four 64-key tiles a CTA
+  const int64_t most = keys / (tensor ? 1024 : 256);
   z = z < most ? z : most;
   pl.splits = static_cast<int>(z < 1 ? 1 : z > 64 ? 64 : z);
   const int dp = dim <= 64 ? 64 : 128;
   pl.workspace = pl.splits > 1 ? static_cast<size_t>(pl.splits) * q_rows * kv_heads * group * (dp * 4 + 8) : 0;
   return pl;
+}
+
+cudaError_t launch_win_attn_join(const WinAttnParams &p, int f32, const WinAttnPlan &pl, cudaStream_t stream) {
+  const dim3 grid(pl.tiles, p.kv_heads);
+  if (f32)
+    return p.dim <= 64 ? launch_pdl(win_attn_join<float, 64>, grid, dim3(kThreads), 0, stream, 1, p, pl.rows)
+                       : launch_pdl(win_attn_join<float, 128>, grid, dim3(kThreads), 0, stream, 1, p, pl.rows);
+  return p.dim <= 64 ? launch_pdl(win_attn_join<__nv_bfloat16, 64>, grid, dim3(kThreads), 0, stream, 1, p, pl.rows)
+                     : launch_pdl(win_attn_join<__nv_bfloat16, 128>, grid, dim3(kThreads), 0, stream, 1, p, pl.rows);
 }
 
 cudaError_t launch_win_attn(const WinAttnParams &p, int f32, const WinAttnPlan &pl, cudaStream_t stream) {
@@ -942,13 +865,7 @@ cudaError_t launch_win_attn(const WinAttnParams &p, int f32, const WinAttnPlan &
     e = paged ? vec ? launch_form<128, true, true>(p, f32, pl, stream) : launch_form<128, true, false>(p, f32, pl, stream)
               : vec ? launch_form<128, false, true>(p, f32, pl, stream) : launch_form<128, false, false>(p, f32, pl, stream);
   }
-  if (e != cudaSuccess || pl.splits == 1) return e;
-  const dim3 grid(pl.tiles, p.kv_heads);
-  if (f32)
-    return p.dim <= 64 ? launch_pdl(win_attn_join<float, 64>, grid, dim3(kThreads), 0, stream, 1, p, pl.rows)
-                       : launch_pdl(win_attn_join<float, 128>, grid, dim3(kThreads), 0, stream, 1, p, pl.rows);
-  return p.dim <= 64 ? launch_pdl(win_attn_join<__nv_bfloat16, 64>, grid, dim3(kThreads), 0, stream, 1, p, pl.rows)
-                     : launch_pdl(win_attn_join<__nv_bfloat16, 128>, grid, dim3(kThreads), 0, stream, 1, p, pl.rows);
+  return e != cudaSuccess || p.splits == 1 ? e : launch_win_attn_join(p, f32, pl, stream);
 }
 
 }  // namespace nq

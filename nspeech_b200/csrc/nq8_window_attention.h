@@ -53,9 +53,20 @@ struct WinAttnPlan {
   int tiles;   // CTAs along x: an upper bound of the row tiles of all sequences
   size_t workspace;
 };
+// tensor: the tensor-core form (nq8_window_attention_tc.cu) instead of the
+// warp-level ones; win_attn_tc_fits says whether a call's sizes are for it.
 // key_bound: keys of a sequence, about.  uniform: every sequence has q_rows / seqs rows.
-WinAttnPlan win_attn_plan(int sm_count, int f32, bool uniform, int seqs, int q_rows, int64_t key_bound, int kv_heads, int group, int dim,
-                          int left, int right, int sinks);
+bool win_attn_tc_fits(int f32, int seqs, int q_rows, int group);
+WinAttnPlan win_attn_plan(int sm_count, int f32, bool tensor, bool uniform, int seqs, int q_rows, int64_t key_bound, int kv_heads,
+                          int group, int dim, int left, int right, int sinks);
+constexpr int kWinTcKeys = 128;  // keys (rows of a box of tm_k, tm_v over plain rows)
+// tm_q: box {64, group, 128 / group} over {dim, heads, rows}; tm_k, tm_v: box
+// {64, 1, 128} over {dim, kv heads, rows}, or over a layer's pages box
+// {64, min(128, page tokens)} over {dim, rows of all pages}; 128-byte swizzle.
+cudaError_t launch_win_attn_tc(const CUtensorMap &tm_q, const CUtensorMap &tm_k, const CUtensorMap &tm_v, const WinAttnParams &p,
+                               const WinAttnPlan &plan, cudaStream_t stream);
+// The splits' join (p.splits > 1), run by both launchers.
+cudaError_t launch_win_attn_join(const WinAttnParams &p, int f32, const WinAttnPlan &plan, cudaStream_t stream);
 cudaError_t launch_win_attn(const WinAttnParams &p, int f32, const WinAttnPlan &plan, cudaStream_t stream);
 
 }  // namespace nq

@@ -180,6 +180,8 @@ SIGNATURES = {
 def load() -> ctypes.CDLL:
     """Load libnq8.so and bind every exported symbol (no CUDA work)."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is None:
             if not os.path.exists(LIB_PATH):

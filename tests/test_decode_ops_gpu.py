@@ -147,6 +147,47 @@ def test_strides_padding_and_rows_left_alone(dt):
     assert bool((out[43:] == -7).all())
 
 
+@pytest.mark.parametrize("n,hq,hk,d,left,right,sinks", [(1500, 4, 1, 128, -1, 0, 0), (1100, 3, 3, 64, 200, 0, 4), (700, 7, 1, 96, 500, 40, 130),
+                                                       (2100, 2, 1, 40, 1000, 0, 300), (900, 2, 2, 128, 3, 700, 1)])
+def test_long_prompts_in_bf16(n, hq, hk, d, left, right, sinks):
+    """Many row tiles and key tiles; sinks that reach into the window's tiles; peaked softmax."""
+    from nspeech_b200.attention import window_attention
+    g = torch.Generator().manual_seed(n)
+    q, k, v = (torch.randn((n, h, d), generator=g).bfloat16() for h in (hq, hk, hk))
+    for factor in (1.0, 30.0):
+        got = window_attention((q * factor).cuda(), k.cuda(), v.cuda(), left, right, sinks)
+        check_rows(got, *attention64(q * factor, k, v, left, right, sinks))
+
+
+def test_negative_and_zero_scale():
+    from nspeech_b200.attention import window_attention
+    g = torch.Generator().manual_seed(6)
+    for dt in ("f32", "bf16"):
+        q, k, v = (torch.randn((150, 2, 64), generator=g).to(DT[dt]) for _ in range(3))
+        for scale in (-0.2, 0.0):
+            got = window_attention(q.cuda(), k.cuda(), v.cuda(), 40, 0, 2, scale=scale)
+            check_rows(got, *attention64(q, k, v, 40, 0, 2, scale))
+
+
+@pytest.mark.parametrize("page", [8, 256, 1024])
+@pytest.mark.parametrize("left,sinks", [(-1, 0), (700, 4), (100, 200)])
+def test_prompt_chunks_over_the_cache(page, left, sinks):
+    """Many queries over many pages, some of them given back; pages larger than a key tile."""
+    lens, news = [2500, 300, 1300], [300, 300, 77]
+    cache, rows = make_cache("bf16", lens, page, 2, 64, seed=page)
+    q = torch.randn((sum(news), 4, 64), generator=torch.Generator().manual_seed(left + 2)).bfloat16()
+    got = cache.attention(q.cuda(), 1, offsets(news), left=left, sinks=sinks)
+    at = np.concatenate([[0], np.cumsum(news)])
+    for i, (a, b) in enumerate(zip(at, at[1:])):
+        check_rows(got[a:b], *attention64(q[a:b], rows[i][0][1], rows[i][1][1], left, 0, sinks))
+    cache.trim(600, 9)
+    cache.check()
+    got = cache.attention(q.cuda(), 1, offsets(news), left=left, sinks=sinks)
+    for i, (a, b) in enumerate(zip(at, at[1:])):
+        there = (cache.table[i] >= 0).repeat_interleave(page)[:lens[i]].cpu()
+        check_rows(got[a:b], *attention64(q[a:b], rows[i][0][1], rows[i][1][1], left, 0, sinks, there=there))
+
+
 def test_scale_and_no_rows():
     from nspeech_b200.attention import window_attention
     g = torch.Generator().manual_seed(4)
