@@ -197,6 +197,31 @@ def load() -> ctypes.CDLL:
     return _lib
 
 
+_native = None
+
+
+def native():
+    """The module of the decoding operators (``_lib/nq8_py.so``): the C ABI called on torch tensors."""
+    global _native
+    if _native is None:
+        load()
+        path = os.path.join(_HERE, "_lib", "nq8_py.so")
+        if not os.path.exists(path):
+            raise ImportError(f"{path} is missing: build it with `make -C nspeech_b200/csrc` (there is no CPU fallback)")
+        import importlib.machinery
+        import importlib.util
+
+        import torch  # noqa: F401  (its libraries come first)
+
+        from .fast_matmul import MatMulError
+        spec = importlib.util.spec_from_loader("nq8_py", importlib.machinery.ExtensionFileLoader("nq8_py", path))
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.errors(MatMulError, NqError)
+        _native = module
+    return _native
+
+
 def last_error() -> str:
     buf = ctypes.create_string_buffer(1024)
     load().nq_last_error(buf, len(buf))
