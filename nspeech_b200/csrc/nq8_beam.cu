@@ -10,12 +10,13 @@
 // the terms of a sum are f32, everything added up is f64, so that candidates
 // of two beams compare as their exact scores do up to about 1e-8.
 //
-// Selection of the W best of a part without sorting it: the values are kept as
-// keys (ordered value, inverted index), all different.  The W-th largest of
-// the maxima of 32 thread groups bounds the W-th largest key from below, the
-// W-th largest of the thread maxima above that bound does so more closely, and
-// only W threads hold keys above the second bound: at most 16 W keys, ranked
-// by counting.  Nothing depends on the values' distribution but the count.
+// Selection of the W best of a round of logits without sorting it: the W-th
+// largest of the maxima of 32 thread groups is no larger than the W-th largest
+// value, so only values from it on are looked at (about W ln of them for
+// unordered logits), and they are ranked by counting.  Where more than a list
+// holds lie above it (many equal values), the same is done with keys (value
+// and inverted index, all different) and a second bound from the thread maxima
+// leaves W threads' values at most.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -28,9 +29,10 @@ namespace {
 
 using Key = unsigned long long;
 constexpr int kPartThreads = 256;
-constexpr int kPerThread = 16;
+constexpr int kPerThread = 32;
 constexpr int kPartElems = kPartThreads * kPerThread;  // logits of one round of a CTA
 constexpr int kBeamSplitsMax = 16;
+constexpr int kList = kBeamMax * kPerThread;           // the most that the exact bound leaves
 
 // An f32 as an unsigned integer of the same order.
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -40,22 +42,69 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 __device__ __forceinline__ float unordered(uint32_t u) {
   return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
-__device__ __forceinline__ Key make_key(float x, uint32_t index) {
-  return static_cast<Key>(ordered(x)) << 32 | static_cast<uint32_t>(~index);
+__device__ __forceinline__ Key make_key(float x, uint32_t index) {  // -0 as +0
+  return static_cast<Key>(ordered(x + 0.f)) << 32 | static_cast<uint32_t>(~index);
 }
 __device__ __forceinline__ Key shfl_xor_key(Key v, int o) { return __shfl_xor_sync(0xffffffffu, v, o); }
 
-// NaN and +inf count as -inf; -0 as +0.
-__device__ __forceinline__ float clean(float x) { return x < INFINITY ? x + 0.f : -INFINITY; }
+// NaN and +inf count as -inf.
+__device__ __forceinline__ float clean(float x) { return x < INFINITY ? x : -INFINITY; }
 
-// One part of one row: CTA (blockIdx.x of `splits`, row blockIdx.y).
+// Two at a time: 2^(x log2e - m'), with m' the rounded multiple of the
+// round's maximum; the one factor that its rounding makes is put right in f64.
+constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float halves(uint64_t v) {  // their sum
+  float a, b;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+  return a + b;
+}
+__device__ __forceinline__ uint64_t ex2_2(uint64_t v) {
+  float a, b;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+  return f2(ex2(a), ex2(b));
+}
+
+// Keys of this round and the earlier best, ranked by counting; the W best to
+// best[cur ^ 1].
+__device__ __forceinline__ void merge_best(const Key *list, int n, const Key *old, Key *best, int W, int tid) {
+  for (int a = tid; a < n + W; a += kPartThreads) {
+    const Key k = a < n ? list[a] : old[a - n];
+    if (k == 0) continue;
+    int above = 0;
+    for (int z = 0; z < n; ++z) above += list[z] > k;
+    for (int z = 0; z < W; ++z) above += old[z] > k;
+    if (above < W) best[above] = k;
+  }
+}
+
+// One part of one row: CTA (blockIdx.x of `splits`, row blockIdx.y).  Values
+// that may be among the W best are listed as the rounds go by; the list is
+// ranked at the end, or when it is half full.
 template <bool BF16, bool VEC>
-__global__ void __launch_bounds__(kPartThreads) beam_part_kernel(const __grid_constant__ BeamParams p) {
-  __shared__ Key group_max[32];
-  __shared__ Key list[kBeamMax * kPerThread > kPartThreads ? kBeamMax * kPerThread : kPartThreads];
+__global__ void __launch_bounds__(kPartThreads, 4) beam_part_kernel(const __grid_constant__ BeamParams p) {
+  __shared__ float group_max[2][32];
+  __shared__ Key key_max[32];
+  __shared__ Key list[kList];
   __shared__ Key best[2][kBeamMax];
-  __shared__ int counts[4];
+  __shared__ int added[2];  // entries listed in rounds of either parity, ever
+  __shared__ int listed, ties;
   __shared__ double sums[kPartThreads / 32];
+  extern __shared__ __align__(16) float4 xs[];  // [kPerThread / 4][kPartThreads]
   pdl_wait();
   pdl_trigger();
   const int row = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
@@ -65,228 +114,464 @@ __global__ void __launch_bounds__(kPartThreads) beam_part_kernel(const __grid_co
   const int c0 = static_cast<int>(static_cast<int64_t>(rounds) * blockIdx.x / p.splits);
   const int c1 = static_cast<int>(static_cast<int64_t>(rounds) * (blockIdx.x + 1) / p.splits);
   const char *src = static_cast<const char *>(p.logits) + row * p.ld * (BF16 ? 2 : 4);
-  constexpr int kVec = BF16 ? 8 : 4;
-
-  float run_max = -INFINITY;
-  double run_sum = 0.0;  // of exp(x - run_max), over the CTA's rounds (thread 0)
-  if (tid < kBeamMax) best[0][tid] = 0;
-  int cur = 0;
-  for (int c = c0; c < c1; ++c) {
-    const int base = c * kPartElems;
-    float x[kPerThread];
-    auto index = [&](int e) { return base + (e / kVec * kPartThreads + tid) * kVec + e % kVec; };
+  constexpr int kVec = VEC ? BF16 ? 8 : 4 : 1;  // logits of a load
+  auto index = [&](int base, int e) { return base + (e / kVec * kPartThreads + tid) * kVec + e % kVec; };
+  // The thread's logits of a round lie in shared memory (its own place: no
+  // synchronisation), those of the next round are on their way in registers.
+  constexpr int kRaw = VEC ? kPerThread / kVec * 4 : kPerThread;
+  uint32_t raw[kRaw];
+  auto fetch = [&](int c) {  // -inf past the end
+    if constexpr (VEC) {
 #pragma unroll
-    for (int u = 0; u < kPerThread / kVec; ++u) {
-      const int i = index(u * kVec);
-      if (VEC && i + kVec <= p.vocab) {
-        const uint4 w = __ldg(reinterpret_cast<const uint4 *>(src + static_cast<int64_t>(i) * (BF16 ? 2 : 4)));
-        const uint32_t r[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if constexpr (BF16) {
-            x[u * kVec + 2 * e] = bf16_bits_to_f32(r[e] & 0xffffu);
-            x[u * kVec + 2 * e + 1] = __uint_as_float(r[e] & 0xffff0000u);
-          } else {
-            x[u * kVec + e] = __uint_as_float(r[e]);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) {
-          float y = -INFINITY;
-          if (i + e < p.vocab) {
-            if constexpr (BF16)
-              y = __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(src)[i + e]);
-            else
-              y = reinterpret_cast<const float *>(src)[i + e];
-          }
-          x[u * kVec + e] = y;
-        }
+      for (int u = 0; u < kPerThread / kVec; ++u) {
+        const int i = index(c * kPartElems, u * kVec);
+        constexpr uint32_t none = BF16 ? 0xff80ff80u : 0xff800000u;
+        uint4 v = make_uint4(none, none, none, none);
+        if (i < p.vocab) v = __ldg(reinterpret_cast<const uint4 *>(src + static_cast<int64_t>(i) * (BF16 ? 2 : 4)));
+        raw[4 * u] = v.x, raw[4 * u + 1] = v.y, raw[4 * u + 2] = v.z, raw[4 * u + 3] = v.w;
       }
-    }
-    // The thread's largest key: larger value first, then lower index.
-    Key mine = 0;
-#pragma unroll
-    for (int e = 0; e < kPerThread; ++e) {
-      x[e] = clean(x[e]);
-      const int i = index(e);
-      if (i < p.vocab) {
-        const Key k = make_key(x[e], static_cast<uint32_t>(i));
-        mine = k > mine ? k : mine;
-      }
-    }
-    Key g = mine;
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
-      const Key y = shfl_xor_key(g, o);
-      g = y > g ? y : g;
-    }
-    if ((tid & 7) == 0) group_max[tid >> 3] = g;
-    if (tid < 2) counts[tid] = 0;
-    __syncthreads();
-    // Every warp for itself: the round's maximum, and the W-th largest group maximum.
-    const Key gm = group_max[lane];
-    int rank = 0;
-    Key top = gm;
-#pragma unroll
-    for (int o = 0; o < 32; ++o) rank += group_max[o] > gm || (group_max[o] == gm && o < lane);
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const Key y = shfl_xor_key(top, o);
-      top = y > top ? y : top;
-    }
-    const Key bound1 = __shfl_sync(0xffffffffu, gm, __ffs(__ballot_sync(0xffffffffu, rank == W - 1)) - 1);
-    const float new_max = fmaxf(run_max, unordered(static_cast<uint32_t>(top >> 32)));
-    // Sum of exponentials.
-    float part = 0.f;
-    if (new_max > -INFINITY) {
-#pragma unroll
-      for (int e = 0; e < kPerThread; ++e) part += expf(x[e] - new_max);  // 0 where x is -inf
-    }
-    double d = part;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-    if (lane == 0) sums[tid >> 5] = d;
-    const Key floor_key = best[cur][W - 1];  // the W-th best of earlier rounds
-    const bool select = top > floor_key;
-    if (select && mine >= bound1 && mine) list[atomicAdd(&counts[0], 1)] = mine;
-    __syncthreads();
-    if (tid == 0 && new_max > -INFINITY) {
-      double s = 0.0;
-#pragma unroll
-      for (int w = 0; w < kPartThreads / 32; ++w) s += sums[w];
-      run_sum = (run_max > -INFINITY ? run_sum * exp(static_cast<double>(run_max) - new_max) : 0.0) + s;
-    }
-    run_max = new_max;
-    if (select) {
-      // W-th largest of the listed thread maxima (all different), 0 if fewer
-      const int n1 = counts[0];
-      if (tid == 0 && n1 < W) group_max[0] = 0;  // group_max is free now: it carries the second bound
-      for (int a = tid; a < n1; a += kPartThreads) {
-        const Key k = list[a];
-        int above = 0;
-        for (int z = 0; z < n1; ++z) above += list[z] > k;
-        if (above == W - 1) group_max[0] = k;
-      }
-      __syncthreads();
-      const Key bound2 = group_max[0] > floor_key ? group_max[0] : floor_key;
+    } else {
 #pragma unroll
       for (int e = 0; e < kPerThread; ++e) {
-        const int i = index(e);
-        if (i >= p.vocab) continue;
-        const Key k = make_key(x[e], static_cast<uint32_t>(i));
-        if (k >= bound2 && k > floor_key) list[atomicAdd(&counts[1], 1)] = k;
+        const int i = index(c * kPartElems, e);
+        raw[e] = BF16 ? 0xff80u : 0xff800000u;
+        if (i < p.vocab) {
+          if constexpr (BF16)
+            raw[e] = __ldg(reinterpret_cast<const uint16_t *>(src) + i);
+          else
+            raw[e] = __ldg(reinterpret_cast<const uint32_t *>(src) + i);
+        }
       }
-      if (tid < kBeamMax) best[cur ^ 1][tid] = 0;
-      __syncthreads();
-      const int n2 = counts[1];
-      // Rank among this round's keys and the earlier best.
-      for (int a = tid; a < n2 + W; a += kPartThreads) {
-        const Key k = a < n2 ? list[a] : best[cur][a - n2];
-        if (k == 0) continue;
-        int above = 0;
-        for (int z = 0; z < n2; ++z) above += list[z] > k;
-        for (int z = 0; z < W; ++z) above += best[cur][z] > k;
-        if (above < W) best[cur ^ 1][above] = k;
-      }
-      cur ^= 1;
+    }
+  };
+  auto place = [&](int q) { return xs + (q * kPartThreads + tid); };  // elements 4 q .. 4 q + 3
+  // Puts the fetched logits in place, f(values) on the way.
+  auto keep = [&](auto f) {
+#pragma unroll
+    for (int q = 0; q < kPerThread / 4; ++q) {
+      float4 v;
+      if constexpr (VEC && BF16)
+        v = make_float4(bf16_bits_to_f32(raw[2 * q] & 0xffffu), __uint_as_float(raw[2 * q] & 0xffff0000u),
+                        bf16_bits_to_f32(raw[2 * q + 1] & 0xffffu), __uint_as_float(raw[2 * q + 1] & 0xffff0000u));
+      else if constexpr (BF16)
+        v = make_float4(bf16_bits_to_f32(raw[4 * q]), bf16_bits_to_f32(raw[4 * q + 1]), bf16_bits_to_f32(raw[4 * q + 2]),
+                        bf16_bits_to_f32(raw[4 * q + 3]));
+      else
+        v = make_float4(__uint_as_float(raw[4 * q]), __uint_as_float(raw[4 * q + 1]), __uint_as_float(raw[4 * q + 2]),
+                        __uint_as_float(raw[4 * q + 3]));
+      *place(q) = v;
+      f(v);
+    }
+  };
+  auto each = [&](auto f) {  // f(e, value) for the thread's elements
+#pragma unroll
+    for (int q = 0; q < kPerThread / 4; ++q) {
+      const float4 v = *place(q);
+      f(4 * q, v.x);
+      f(4 * q + 1, v.y);
+      f(4 * q + 2, v.z);
+      f(4 * q + 3, v.w);
+    }
+  };
+  auto clean_all = [&]() {
+#pragma unroll 1
+    for (int q = 0; q < kPerThread / 4; ++q) {
+      const float4 v = *place(q);
+      *place(q) = make_float4(clean(v.x), clean(v.y), clean(v.z), clean(v.w));
+    }
+  };
+  if (tid < kBeamMax) best[0][tid] = best[1][tid] = 0;
+  if (tid == 0) added[0] = added[1] = 0;
+  int cur = 0;
+  float ref = -INFINITY;  // the sum's reference: the first rounds' maximum
+  double sum = 0.0;       // this thread's part of the sum of exp(x - ref)
+  // At least W values of earlier rounds are `floor` or more; -inf counts with floored.
+  float floor = -INFINITY;
+  bool floored = false;
+
+  // The list's n entries and the earlier best are ranked together (all threads).
+  auto rank_list = [&](int n) {
+    merge_best(list, n, best[cur], best[cur ^ 1], W, tid);
+    __syncthreads();
+    if (tid < kBeamMax) best[cur][tid] = 0;  // the next merge's place
+    cur ^= 1;
+    __syncthreads();
+  };
+  // Round c had more values at its bound than the list holds (many equal ones):
+  // the same with keys, which are all different.  `before`: entries of earlier rounds.
+  auto exact_round = [&](int c, int before) {
+    rank_list(before);
+    const Key worst = best[cur][W - 1];
+    const int base = c * kPartElems;
+    fetch(c);
+    keep([](const float4 &) {});
+    Key km = 0;
+    each([&](int e, float v) {
+      const int i = index(base, e);
+      const Key k = i < p.vocab ? make_key(clean(v), static_cast<uint32_t>(i)) : 0;
+      km = k > km ? k : km;
+    });
+    Key kg = km;
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+      const Key y = shfl_xor_key(kg, o);
+      kg = y > kg ? y : kg;
+    }
+    if ((tid & 7) == 0) key_max[tid >> 3] = kg;
+    if (tid == 0) ties = listed = 0;
+    __syncthreads();
+    const Key mykey = key_max[lane];
+    int above = 0;
+    for (int o = 0; o < 32; ++o) above += key_max[o] > mykey || (key_max[o] == mykey && o < lane);
+    const Key bound1 = __shfl_sync(0xffffffffu, mykey, __ffs(__ballot_sync(0xffffffffu, above == W - 1)) - 1);
+    if (km && km >= bound1) list[atomicAdd(&ties, 1)] = km;
+    __syncthreads();
+    const int n1 = ties;
+    if (tid == 0 && n1 < W) key_max[0] = 0;  // fewer threads than W: all their keys
+    for (int a = tid; a < n1; a += kPartThreads) {
+      const Key k = list[a];
+      int over = 0;
+      for (int z = 0; z < n1; ++z) over += list[z] > k;
+      if (over == W - 1) key_max[0] = k;
     }
     __syncthreads();
+    const Key bound2 = key_max[0];  // W threads' keys at most lie above it
+    each([&](int e, float v) {
+      const int i = index(base, e);
+      const Key k = make_key(clean(v), static_cast<uint32_t>(i));
+      if (i < p.vocab && k >= bound2 && k > worst) list[atomicAdd(&listed, 1)] = k;
+    });
+    __syncthreads();
+    rank_list(listed);
+  };
+  // Entries, those before the latest round, and what `added` was: every thread
+  // keeps the same.  A round's entries are counted by its parity, so that the
+  // count can be read while the next round's are being added.
+  int n_list = 0, n_before = 0, seen[2] = {0, 0};
+  auto count_round = [&](int c) {
+    const int now = added[c & 1];
+    n_before = n_list;
+    n_list += now - (c & 1 ? seen[1] : seen[0]);
+    if (c & 1)
+      seen[1] = now;
+    else
+      seen[0] = now;
+  };
+  fetch(c0);
+  for (int c = c0;; ++c) {
+    const int base = c * kPartElems;
+    float mine = -INFINITY, part = NAN;  // part: the thread's terms of the sum, NaN: not yet
+    if (c < c1) {
+      // The largest (fmaxf passes over NaN) and, where there is a reference for
+      // it, the sum, straight from the registers.
+      uint64_t a = f2(0.f, 0.f), b = a;
+      const bool known = fabsf(ref) < 64.f;
+      if (known) {
+        const uint64_t l2 = f2(kLog2e, kLog2e), m2 = f2(-(ref * kLog2e), -(ref * kLog2e));
+        keep([&](const float4 &v) {
+          mine = fmaxf(fmaxf(fmaxf(mine, v.x), fmaxf(v.y, v.z)), v.w);
+          a = add2(a, ex2_2(fma2(f2(v.x, v.y), l2, m2)));
+          b = add2(b, ex2_2(fma2(f2(v.z, v.w), l2, m2)));
+        });
+      } else {
+        keep([&](const float4 &v) { mine = fmaxf(fmaxf(fmaxf(mine, v.x), fmaxf(v.y, v.z)), v.w); });
+      }
+      part = known ? halves(add2(a, b)) : NAN;
+      if (c + 1 < c1) fetch(c + 1);
+      // +inf is taken out here, NaN where the sum shows it
+      auto largest = [&]() {
+        float v = -INFINITY;
+        each([&](int, float y) { v = fmaxf(v, y); });
+        return v;
+      };
+      if (!(mine < INFINITY)) {
+        clean_all();
+        mine = largest();
+        part = NAN;
+      }
+      float g = mine;
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+      if ((tid & 7) == 0) group_max[c & 1][tid >> 3] = g;
+    }
+    __syncthreads();
+    if (c > c0) {
+      count_round(c - 1);
+      if (n_list > kList / 2 || c == c1) {
+        if (n_list > kList) {
+          exact_round(c - 1, n_before);
+          if (c < c1) {  // the round at hand again
+            fetch(c);
+            keep([](const float4 &) {});
+            clean_all();
+            if (c + 1 < c1) fetch(c + 1);
+          }
+        } else
+          rank_list(n_list);
+        n_list = 0;
+      }
+    }
+    if (c == c1) break;
+    // Every warp for itself: the round's maximum and the W-th largest group maximum.
+    const float gm = group_max[c & 1][lane];
+    const float top = unordered(__reduce_max_sync(0xffffffffu, ordered(gm)));
+    // Where the floor leaves more than a few groups, the round's own bound: its
+    // W-th largest group maximum.
+    float bound = floor;
+    const int over = __popc(__ballot_sync(0xffffffffu, !floored || gm > floor));
+    if (!floored || over > W) {
+      int rank = 0;
+#pragma unroll
+      for (int o = 0; o < 32; ++o) {
+        const float y = group_max[c & 1][o];
+        rank += y > gm || (y == gm && o < lane);
+      }
+      bound = __shfl_sync(0xffffffffu, gm, __ffs(__ballot_sync(0xffffffffu, rank == W - 1)) - 1);
+    }
+    // The sum, against a reference that moves only where a term could overflow.
+    if (top > -INFINITY && !(top < ref + 40.f)) {
+      if (ref > -INFINITY) sum *= exp(static_cast<double>(ref) - top);
+      ref = top;
+      part = NAN;
+    }
+    if (ref > -INFINITY) {
+      const bool near = fabsf(ref) < 64.f;
+      auto terms = [&]() {  // 0 where x is -inf
+        if (!near) {  // far from 0: the difference first
+          float d = 0.f;
+          each([&](int, float y) { d += ex2((y - ref) * kLog2e); });
+          return d;
+        }
+        const uint64_t l2 = f2(kLog2e, kLog2e), m2 = f2(-(ref * kLog2e), -(ref * kLog2e));
+        uint64_t a = f2(0.f, 0.f), b = a;
+#pragma unroll
+        for (int q = 0; q < kPerThread / 4; ++q) {
+          const float4 v = *place(q);
+          a = add2(a, ex2_2(fma2(f2(v.x, v.y), l2, m2)));
+          b = add2(b, ex2_2(fma2(f2(v.z, v.w), l2, m2)));
+        }
+        return halves(add2(a, b));
+      };
+      if (isnan(part)) part = terms();
+      if (isnan(part)) {
+        clean_all();
+        part = terms();
+      }
+      // 2^(m' - m log2e') to first order: the difference is below 2^-18
+      const double fix = near ? 1.0 + (static_cast<double>(ref * kLog2e) - static_cast<double>(ref) * static_cast<double>(kLog2e)) * 0.6931471805599453 : 1.0;
+      sum += static_cast<double>(part) * fix;
+    }
+    // Values below this round's bound are out, and those not above the floor:
+    // W earlier ones go before them.
+    // The threads that hold one, one after the other: a lane for each of the
+    // thread's elements.
+    const float *xf = reinterpret_cast<const float *>(xs);
+    for (unsigned who = __ballot_sync(0xffffffffu, mine >= bound && (!floored || mine > floor)); who; who &= who - 1) {
+      const int t = (tid & ~31) + __ffs(who) - 1;
+      const int i = base + (lane / kVec * kPartThreads + t) * kVec + lane % kVec;
+      const float v = clean(xf[(lane / 4 * kPartThreads + t) * 4 + lane % 4]);
+      if (v >= bound && (!floored || v > floor) && i < p.vocab) {
+        const int at = n_list + atomicAdd(&added[c & 1], 1) - (c & 1 ? seen[1] : seen[0]);
+        if (at < kList) list[at] = make_key(v, static_cast<uint32_t>(i));
+      }
+    }
+    __syncwarp();
+    const bool full = base + kPartThreads * kVec <= p.vocab;  // every group has a value of the row
+    if ((full && !floored) || bound > floor) floor = bound, floored = true;
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) sums[tid >> 5] = sum;
+  __syncthreads();
   const int64_t at = static_cast<int64_t>(row) * p.splits + blockIdx.x;
   if (tid < W) p.part_keys[at * W + tid] = best[cur][tid];
   if (tid == 0) {
-    p.part_max[at] = run_max;
-    p.part_sum[at] = run_sum;
+    double s = 0.0;
+#pragma unroll
+    for (int w = 0; w < kPartThreads / 32; ++w) s += sums[w];
+    p.part_max[at] = ref;
+    p.part_sum[at] = s;
   }
 }
 
-// One utterance: warp k joins beam k's parts, warp 0 the beams.
-__global__ void __launch_bounds__(32 * kBeamMax) beam_join_kernel(const __grid_constant__ BeamParams p) {
-  extern __shared__ __align__(8) Key parts[];  // [beams][splits][beams]
-  __shared__ double score[kBeamMax][kBeamMax];
-  __shared__ int token[kBeamMax][kBeamMax];
-  __shared__ int have[kBeamMax];
+// A candidate's place among all: better score first, then the lower beam, then
+// the larger key (a beam's own logits order its candidates).
+struct Cand {
+  Key score;  // the f64 score as an integer of the same order (never 0)
+  Key key;    // 0: no candidate
+  int beam;
+  __device__ __forceinline__ bool before(const Cand &o) const {
+    if (score != o.score) return score > o.score;
+    if (beam != o.beam) return beam < o.beam;
+    return key > o.key;
+  }
+};
+__device__ __forceinline__ Key ordered64(double x) {
+  const Key u = static_cast<Key>(__double_as_longlong(x + 0.0));  // -0 as +0
+  return u >> 63 ? ~u : u | Key{1} << 63;
+}
+__device__ __forceinline__ double unordered64(Key u) { return __longlong_as_double(static_cast<long long>(u >> 63 ? u & ~(Key{1} << 63) : ~u)); }
+
+// One utterance: of the W x S sorted lists of W keys each, those whose head is
+// among the W best heads hold all W best candidates; they are ranked by
+// counting.
+constexpr int kJoinThreads = 256;
+__global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_constant__ BeamParams p) {
+  __shared__ double lse[kBeamMax], base_score[kBeamMax];
+  __shared__ uint8_t done[kBeamMax];
+  __shared__ Cand head[kBeamMax * kBeamSplitsMax];
+  __shared__ Cand pick[kBeamMax * kBeamMax];
+  __shared__ int n_pick, w_head;
   pdl_wait();
   pdl_trigger();
-  const int W = p.beams, S = p.splits, b = blockIdx.x, k = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int row = b * W + k;
-  const bool done = p.finished && p.finished[row];
-  const float base = p.scores[row];
-  Key *mine = parts + static_cast<int64_t>(k) * S * W;
-  if (done) {
-    if (lane == 0) {
-      score[k][0] = isnan(base) ? -INFINITY : static_cast<double>(base);
-      token[k][0] = p.eos;
-      have[k] = 1;
+  const int W = p.beams, S = p.splits, b = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const Key *keys = p.part_keys + static_cast<int64_t>(b) * W * S * W;  // [beam][split][W]
+  const int lists = W * S, all = lists * W;
+  const Key first = tid < all ? keys[tid] : 0;  // on its way while the sums are joined
+  if (tid == 0) n_pick = 0, w_head = -1;
+  // log sum exp of each beam's row, over its parts (a lane each)
+  for (int k = warp; k < W; k += kJoinThreads / 32) {
+    const int row = b * W + k;
+    const bool fin = p.finished && p.finished[row];
+    const float base = p.scores[row];
+    double sum = 0.0;
+    float m = -INFINITY;
+    if (lane < S) {
+      m = p.part_max[static_cast<int64_t>(row) * S + lane];
+      sum = p.part_sum[static_cast<int64_t>(row) * S + lane];
     }
-  } else {
-    for (int x = lane; x < S * W; x += 32) mine[x] = p.part_keys[static_cast<int64_t>(row) * S * W + x];
-    // log sum exp of the row
-    const float m = lane < S ? p.part_max[static_cast<int64_t>(row) * S + lane] : -INFINITY;
     float top = m;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    double sum = 0.0;
-    if (m > -INFINITY) sum = p.part_sum[static_cast<int64_t>(row) * S + lane] * exp(static_cast<double>(m) - top);
+    sum = m > -INFINITY ? (m == top ? sum : sum * exp(static_cast<double>(m) - top)) : 0.0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const double lse = static_cast<double>(top) + log(sum);
-    __syncwarp();
-    // W times the largest head of the parts' lists (lane: a part)
-    int at = 0, found = 0;
-    for (int r = 0; r < W; ++r) {
-      const Key head = lane < S && at < W ? mine[lane * W + at] : 0;
-      Key best = head;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const Key y = shfl_xor_key(best, o);
-        best = y > best ? y : best;
-      }
-      if (best == 0) break;  // fewer tokens than beams
-      if (head == best) ++at;
-      if (lane == 0) {
-        const float x = unordered(static_cast<uint32_t>(best >> 32));
-        // every logit -inf: the sum is none, and the candidates count as -inf
-        const double s = x > -INFINITY ? static_cast<double>(base) + (static_cast<double>(x) - lse) : -INFINITY;
-        score[k][r] = isnan(s) || isnan(base) ? -INFINITY : s;
-        token[k][r] = static_cast<int>(~static_cast<uint32_t>(best));
-      }
-      ++found;
+    if (lane == 0) {
+      lse[k] = static_cast<double>(top) + log(sum);
+      base_score[k] = isnan(base) ? -INFINITY : static_cast<double>(base);
+      done[k] = fin;
     }
-    if (lane == 0) have[k] = found;
   }
   __syncthreads();
-  if (k) return;
-  int at = 0;
-  const int n = lane < W ? have[lane] : 0;
-  const bool was = lane < W && p.finished && p.finished[b * W + lane];  // before the outputs, which may lie there
-  for (int r = 0; r < W; ++r) {
-    double s = at < n ? score[lane][at] : -INFINITY;
-    int who = at < n ? lane : 64;  // past every beam
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const double y = __shfl_xor_sync(0xffffffffu, s, o);
-      const int z = __shfl_xor_sync(0xffffffffu, who, o);
-      if (y > s || (y == s && z < who)) {
-        s = y;
-        who = z;
+  auto candidate = [&](int k, Key key) {
+    Cand c;
+    c.beam = k;
+    c.key = key;
+    if (done[k]) {
+      c.score = ordered64(base_score[k]);
+    } else {
+      const float x = unordered(static_cast<uint32_t>(key >> 32));
+      // every logit -inf: there is no sum, and the candidates count as -inf
+      const double s = x > -INFINITY ? base_score[k] + (static_cast<double>(x) - lse[k]) : -INFINITY;
+      c.score = ordered64(isnan(s) ? -INFINITY : s);
+    }
+    return c;
+  };
+  // Entry i of the lists: a finished beam's only candidate stands first in its
+  // first list; the parts of its row were not written.
+  auto entry = [&](int i, Key key) -> Key {
+    const int k = i / (S * W);
+    return done[k] ? (i % (S * W) == 0 ? static_cast<Key>(~static_cast<uint32_t>(p.eos)) | Key{1} << 63 : 0) : key;
+  };
+  auto put = [&](const Cand &c, int above) {
+    const int out = b * W + above;
+    const int t = done[c.beam] ? p.eos : static_cast<int>(~static_cast<uint32_t>(c.key));
+    p.out_scores[out] = static_cast<float>(unordered64(c.score));
+    p.out_parents[out] = b * W + c.beam;
+    p.out_tokens[out] = t;
+    if (p.out_finished) p.out_finished[out] = done[c.beam] || t == p.eos;
+  };
+  if (all <= kJoinThreads) {  // few: each thread ranks its own among all
+    // score (0: none), then 31 - beam and the logit, then the inverted token
+    ulonglong2 *major = reinterpret_cast<ulonglong2 *>(pick);
+    uint32_t *minor = reinterpret_cast<uint32_t *>(head);
+    Cand mine{};
+    if (tid < all) {
+      const Key key = entry(tid, first);
+      if (key) mine = candidate(tid / (S * W), key);
+      major[tid] = make_ulonglong2(mine.score, static_cast<Key>(31 - mine.beam) << 32 | mine.key >> 32);
+      minor[tid] = static_cast<uint32_t>(mine.key);
+    }
+    __syncthreads();
+    if (mine.key) {
+      const Key m = static_cast<Key>(31 - mine.beam) << 32 | mine.key >> 32;
+      const uint32_t t = static_cast<uint32_t>(mine.key);
+      int above = 0;
+#pragma unroll 4
+      for (int z = 0; z < all; ++z) {
+        const ulonglong2 y = major[z];
+        above += (y.x > mine.score) | ((y.x == mine.score) & ((y.y > m) | ((y.y == m) & (minor[z] > t))));
       }
+      if (above < W) put(mine, above);
     }
-    if (lane == who) {
-      const int t = token[lane][at];
-      const int out = b * W + r;
-      p.out_scores[out] = static_cast<float>(s);
-      p.out_parents[out] = b * W + lane;
-      p.out_tokens[out] = t;
-      if (p.out_finished) p.out_finished[out] = was || t == p.eos;
-      ++at;
-    }
+    return;
+  }
+  for (int i = tid; i < lists; i += kJoinThreads) head[i] = candidate(i / S, entry(i * W, keys[static_cast<int64_t>(i) * W]));
+  __syncthreads();
+  // The W-th best head; fewer heads than W: all lists.
+  for (int i = tid; i < lists; i += kJoinThreads) {
+    if (head[i].key == 0) continue;
+    int above = 0;
+    for (int z = 0; z < lists; ++z) above += head[z].key != 0 && head[z].before(head[i]);
+    if (above == W - 1) w_head = i;
+  }
+  __syncthreads();
+  const int last = w_head;
+  const Cand floor_c = last >= 0 ? head[last] : Cand{};
+  for (int i = tid; i < all; i += kJoinThreads) {
+    const int l = i / W;
+    if (head[l].key == 0 || (last >= 0 && floor_c.before(head[l]))) continue;
+    const Key key = entry(i, keys[i]);
+    if (key == 0) continue;
+    const Cand c = candidate(l / S, key);
+    if (last >= 0 && floor_c.before(c)) continue;
+    pick[atomicAdd(&n_pick, 1)] = c;
+  }
+  __syncthreads();
+  const int n = n_pick;
+  for (int i = tid; i < n; i += kJoinThreads) {
+    const Cand c = pick[i];
+    int above = 0;
+    for (int z = 0; z < n; ++z) above += pick[z].before(c);
+    if (above < W) put(c, above);
   }
 }
 
-// dst[r] = src[parents[r]]: a CTA holds one strip of every row of one state,
-// and reads all rows before it writes any, so dst may be src.
+// dst[r] = src[parents[r]] into other memory: a warp a row and 2 KB of it.
+constexpr int kCopyBytes = 2048;
+template <typename T>
+__global__ void __launch_bounds__(256) beam_gather_kernel(const __grid_constant__ ReorderParams p) {
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31;
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int r = static_cast<int>(unit % p.rows);
+  const int strip = static_cast<int>(unit / p.rows);
+  if (strip >= p.strip0[p.count]) return;
+  int i = 0;
+  while (i + 1 < p.count && strip >= p.strip0[i + 1]) ++i;
+  const int64_t lo = static_cast<int64_t>(strip - p.strip0[i]) * kCopyBytes;
+  const int64_t left = p.row_bytes[i] - lo;
+  const int n = static_cast<int>((left < kCopyBytes ? left : kCopyBytes) / static_cast<int>(sizeof(T)));
+  int from = __ldg(p.parents + r);
+  if (from < 0 || from >= p.rows) from = r;  // out of range: the row's own
+  const T *src = reinterpret_cast<const T *>(static_cast<const char *>(p.src[i]) + from * p.src_ld[i] + lo);
+  T *dst = reinterpret_cast<T *>(static_cast<char *>(p.dst[i]) + r * p.dst_ld[i] + lo);
+  if constexpr (sizeof(T) == 16) {
+    T v[kCopyBytes / 512];
+#pragma unroll
+    for (int u = 0; u < kCopyBytes / 512; ++u)
+      if (lane + 32 * u < n) v[u] = src[lane + 32 * u];
+#pragma unroll
+    for (int u = 0; u < kCopyBytes / 512; ++u)
+      if (lane + 32 * u < n) dst[lane + 32 * u] = v[u];
+  } else {
+    for (int x = lane; x < n; x += 32) dst[x] = src[x];
+  }
+}
+
+// The same in place (or between any two): a CTA holds one strip of every row of one
+// state, and reads all rows before it writes any.
 template <typename T>
 __global__ void __launch_bounds__(256) beam_reorder_kernel(const __grid_constant__ ReorderParams p) {
   extern __shared__ __align__(16) uint8_t strip_raw[];
@@ -315,11 +600,10 @@ __global__ void __launch_bounds__(256) beam_reorder_kernel(const __grid_constant
 
 }  // namespace
 
-// CTAs of a row: enough that all rows' CTAs fill the GPU four times over, each
-// with at least one round of logits.
+// CTAs of a row: one wave of four CTAs an SM, each with at least one round of logits.
 int beam_splits(int sm_count, int rows, int vocab) {
   const int rounds = (vocab + kPartElems - 1) / kPartElems;
-  int s = (4 * sm_count + rows - 1) / (rows > 0 ? rows : 1);
+  int s = 4 * sm_count / (rows > 0 ? rows : 1);
   s = s < rounds ? s : rounds;
   return s < 1 ? 1 : s > kBeamSplitsMax ? kBeamSplitsMax : s;
 }
@@ -329,19 +613,17 @@ size_t beam_workspace(int rows, int beams, int splits) {
 
 cudaError_t launch_beam_select(const BeamParams &p, cudaStream_t s) {
   const int rows = p.items * p.beams;
-  const bool vec = (reinterpret_cast<uintptr_t>(p.logits) | static_cast<uintptr_t>(p.ld * (p.bf16 ? 2 : 4))) % 16 == 0;
+  const bool vec = (reinterpret_cast<uintptr_t>(p.logits) | static_cast<uintptr_t>(p.ld * (p.bf16 ? 2 : 4))) % 16 == 0 &&
+                   p.vocab % (p.bf16 ? 8 : 4) == 0;
   const dim3 grid(p.splits, rows);
-  cudaError_t e = p.bf16 ? vec ? launch_pdl(beam_part_kernel<true, true>, grid, dim3(kPartThreads), 0, s, 1, p)
-                               : launch_pdl(beam_part_kernel<true, false>, grid, dim3(kPartThreads), 0, s, 1, p)
-                  : vec ? launch_pdl(beam_part_kernel<false, true>, grid, dim3(kPartThreads), 0, s, 1, p)
-                        : launch_pdl(beam_part_kernel<false, false>, grid, dim3(kPartThreads), 0, s, 1, p);
+  constexpr size_t smem = kPartElems * 4;
+  static_assert(smem + 16 * 1024 <= 48 * 1024, "no attribute is needed");
+  cudaError_t e = p.bf16 ? vec ? launch_pdl(beam_part_kernel<true, true>, grid, dim3(kPartThreads), smem, s, 1, p)
+                               : launch_pdl(beam_part_kernel<true, false>, grid, dim3(kPartThreads), smem, s, 1, p)
+                  : vec ? launch_pdl(beam_part_kernel<false, true>, grid, dim3(kPartThreads), smem, s, 1, p)
+                        : launch_pdl(beam_part_kernel<false, false>, grid, dim3(kPartThreads), smem, s, 1, p);
   if (e != cudaSuccess) return e;
-  const size_t smem = static_cast<size_t>(p.beams) * p.splits * p.beams * 8;
-  if (smem > 32 * 1024) {  // next to the kernel's static arrays
-    e = cudaFuncSetAttribute(beam_join_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBeamMax * kBeamSplitsMax * kBeamMax * 8);
-    if (e != cudaSuccess) return e;
-  }
-  return launch_pdl(beam_join_kernel, dim3(p.items), dim3(32 * p.beams), smem, s, 1, p);
+  return launch_pdl(beam_join_kernel, dim3(p.items), dim3(kJoinThreads), 0, s, 1, p);
 }
 
 cudaError_t launch_beam_reorder(ReorderParams &p, cudaStream_t s) {
@@ -349,6 +631,21 @@ cudaError_t launch_beam_reorder(ReorderParams &p, cudaStream_t s) {
   for (int i = 0; i < p.count; ++i)
     bits |= reinterpret_cast<uintptr_t>(p.src[i]) | reinterpret_cast<uintptr_t>(p.dst[i]) | static_cast<uint64_t>(p.row_bytes[i]) |
             static_cast<uint64_t>(p.src_ld[i]) | static_cast<uint64_t>(p.dst_ld[i]);
+  bool in_place = false;
+  for (int i = 0; i < p.count; ++i) in_place |= p.src[i] == p.dst[i];
+  if (!in_place) {
+    int n = 0;
+    for (int i = 0; i < p.count; ++i) {
+      p.strip0[i] = n;
+      n += static_cast<int>((p.row_bytes[i] + kCopyBytes - 1) / kCopyBytes);
+    }
+    p.strip0[p.count] = n;
+    const int64_t blocks = (static_cast<int64_t>(n) * p.rows + 7) / 8;
+    if (blocks <= INT32_MAX) {
+      auto go = [&](auto kern) { return launch_pdl(kern, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, 1, static_cast<const ReorderParams &>(p)); };
+      return bits % 16 == 0 ? go(beam_gather_kernel<uint4>) : bits % 4 == 0 ? go(beam_gather_kernel<uint32_t>) : bits % 2 == 0 ? go(beam_gather_kernel<uint16_t>) : go(beam_gather_kernel<uint8_t>);
+    }
+  }
   // strips of about 16 KB over all rows, of 16 bytes of a row at least
   int strip = 16384 / p.rows / 16 * 16;
   p.strip_bytes = strip < 16 ? 16 : strip;

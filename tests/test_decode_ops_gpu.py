@@ -560,6 +560,25 @@ def test_beam_select_ties_and_masks(dt, beams, kind):
         assert np.all(same | (np.abs(got[0][0].numpy() - s) <= np.abs(s) * 2.0 ** -24 + 2.0 ** -19))
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("beams", [1, 2, 8, 32])
+def test_beam_select_over_many_rounds(dt, beams):
+    """Rows of several rounds a CTA where the best come early, late, scattered or in runs of equal values."""
+    from nspeech_b200.beam import beam_select
+    vocab, rng = 150001, np.random.default_rng(3)
+    rows = [np.linspace(5, -5, vocab), np.linspace(-5, 5, vocab), np.sin(np.arange(vocab) * 0.37) * 6, np.repeat(rng.standard_normal(151), 1000)[:vocab],
+            np.where(np.arange(vocab) % 4096 == 5, 3.0, -1.0), np.where(np.arange(vocab) > 140000, 0.5, 0.25), rng.standard_normal(vocab) * 4]
+    x = np.stack([rows[(b * 5 + i) % len(rows)] for i in range(3) for b in range(beams)]).reshape(3, beams, vocab).astype(np.float32)
+    x[:, :, 70000:90000:7] = -np.inf
+    lt = torch.from_numpy(x).to(DT[dt])
+    scores = -np.arange(3 * beams, dtype=np.float32).reshape(3, beams) / 64
+    got = [t.cpu() for t in beam_select(lt.cuda(), torch.from_numpy(scores).cuda())]
+    for i in range(3):
+        want = beam64(lt[i].float().numpy(), scores[i], np.zeros(beams, bool), -1)
+        assert got[1][i].tolist() == [i * beams + b for _, b, _ in want]
+        assert got[2][i].tolist() == [t for _, _, t in want]
+
+
 def test_beam_select_strided_rows_and_outputs_in_place():
     from nspeech_b200.beam import beam_select
     g = torch.Generator(device="cuda").manual_seed(2)
