@@ -84,13 +84,10 @@ __global__ void __launch_bounds__(kBlock) cache_reserve_kernel(const CacheView c
   int *tail = reinterpret_cast<int *>(sh + words), *start = tail + n;
   pdl_wait();
   pdl_trigger();
-  if (c.state[kStateStatus]) {
-    if (threadIdx.x == 0) c.state[kStateCopies] = 0;
-    return;
-  }
+  const int status = c.state[kStateStatus];
   const int P = 1 << c.page_shift;
   const int64_t room = static_cast<int64_t>(c.max_pages) << c.page_shift;
-  if (threadIdx.x == 0) bad = copies = 0;
+  if (threadIdx.x == 0) copies = 0, bad = status;
   held_bits(c, bits);
   for (int i = threadIdx.x; i < n; i += kBlock) {
     const int old = c.lens[first + i], add = count_of(offsets, uniform, i);
@@ -142,7 +139,7 @@ __global__ void __launch_bounds__(kBlock) cache_reserve_kernel(const CacheView c
   __syncthreads();
   if (bad || total > free_pages) {
     if (threadIdx.x == 0) {
-      c.state[kStateStatus] = bad ? bad : kCacheOutOfPages;
+      if (!status) c.state[kStateStatus] = bad ? bad : kCacheOutOfPages;
       c.state[kStateCopies] = 0;
     }
     return;
@@ -210,33 +207,59 @@ __global__ void __launch_bounds__(128) cache_copy_kernel(const CacheView c) {
   }
 }
 
-// New tokens into their places: 16 rows of one layer a CTA.  Within a head a
-// page's rows are adjacent, so the threads go along rows first.
-constexpr int kWriteRows = 16;
-template <typename T>
+// The last i in [0, n) with offsets[i] <= r, by a whole warp: 32 probes a step.
+__device__ __forceinline__ int slot_of(const int *offsets, int n, int r) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, len = n;
+  while (len > 1) {
+    const int step = (len + 31) / 32;
+    const int i = lane * step;
+    const unsigned m = __ballot_sync(0xffffffffu, i < len && __ldg(offsets + lo + i) <= r);
+    const int at = max(__popc(m) - 1, 0) * step;  // the probes that hold come first
+    lo += at;
+    len = min(step, len - at);
+  }
+  return lo;
+}
+
+// New tokens into their places: ROWS rows of one layer a CTA.  Within a head a
+// page's rows are adjacent, so the threads go along rows first; their first
+// loads are under way while the rows' places are looked up.
+template <typename T, int ROWS>
 __global__ void __launch_bounds__(256) cache_write_kernel(const CacheView c, const char *__restrict__ k, const char *__restrict__ v,
                                                           int64_t k_ts, int64_t k_hs, int64_t k_ls, int64_t v_ts, int64_t v_hs,
                                                           int64_t v_ls, int layer0, int rows, const int *__restrict__ offsets,
                                                           int uniform, int first, int n) {
-  __shared__ int64_t place[kWriteRows];  // page row of head 0 (in rows of `dim`), -1: none
+  __shared__ int64_t place[ROWS];  // page row of head 0 (in rows of `dim`), -1: none
   pdl_wait();
   pdl_trigger();
-  if (c.state[kStateStatus]) return;
-  const int row0 = blockIdx.x * kWriteRows, layer = blockIdx.y;
-  if (threadIdx.x < kWriteRows) {
-    const int r = row0 + threadIdx.x;
+  const int row0 = blockIdx.x * ROWS, layer = blockIdx.y;
+  const int units = c.dim * c.size / static_cast<int>(sizeof(T));  // of a row of one head
+  const int row_bytes = c.dim * c.size;
+  const int all = units * ROWS * c.kv_heads;
+  auto source = [&](const char *base, int64_t ts, int64_t hs, int64_t ls, int x) {
+    const int u = x % units, r = x / units % ROWS, h = x / (units * ROWS);
+    return reinterpret_cast<const T *>(base + (layer * ls + (row0 + r) * ts + h * hs) * c.size + u * sizeof(T));
+  };
+  constexpr int U = 2;
+  T kk[U], vv[U];
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const int x = threadIdx.x + 256 * i;
+    if (x < all && row0 + x / units % ROWS < rows) {
+      kk[i] = *source(k, k_ts, k_hs, k_ls, x);
+      vv[i] = *source(v, v_ts, v_hs, v_ls, x);
+    }
+  }
+  const int status = c.state[kStateStatus];
+  for (int j = threadIdx.x >> 5; j < ROWS; j += 8) {
+    const int r = row0 + j;
     int64_t at = -1;
     int fault = 0;
     if (r < rows) {
       int i, begin, end;
       if (offsets) {
-        int lo = 0, hi = n;  // the last i with offsets[i] <= r
-        while (hi - lo > 1) {
-          const int mid = (lo + hi) / 2;
-          if (__ldg(offsets + mid) <= r) lo = mid;
-          else hi = mid;
-        }
-        i = lo;
+        i = slot_of(offsets, n, r);
         begin = __ldg(offsets + i);
         end = __ldg(offsets + i + 1);
       } else {
@@ -256,66 +279,74 @@ __global__ void __launch_bounds__(256) cache_write_kernel(const CacheView c, con
         }
       }
     }
-    place[threadIdx.x] = at;
-    if (fault) atomicOr(c.state + kStateStatus, fault);
+    if ((threadIdx.x & 31) == 0) {
+      place[j] = status ? -1 : at;
+      if (fault && !status) atomicOr(c.state + kStateStatus, fault);
+    }
   }
   __syncthreads();
-  const int units = c.dim * c.size / static_cast<int>(sizeof(T));  // of a row of one head
   const int64_t base = static_cast<int64_t>(layer0 + layer) * c.pages * c.kv_heads << c.page_shift;
-  const int row_bytes = c.dim * c.size;
-  for (int x = threadIdx.x; x < units * kWriteRows * c.kv_heads; x += blockDim.x) {
-    const int u = x % units, r = x / units % kWriteRows, h = x / (units * kWriteRows);
-    if (place[r] < 0) continue;
+  auto put = [&](int x, const T &a, const T &b) {
+    const int u = x % units, r = x / units % ROWS, h = x / (units * ROWS);
     const int64_t to = (base + place[r] + (static_cast<int64_t>(h) << c.page_shift)) * row_bytes + u * sizeof(T);
-    const int64_t tok = row0 + r;
-    *reinterpret_cast<T *>(static_cast<char *>(c.k) + to) =
-        *reinterpret_cast<const T *>(k + (layer * k_ls + tok * k_ts + h * k_hs) * c.size + u * sizeof(T));
-    *reinterpret_cast<T *>(static_cast<char *>(c.v) + to) =
-        *reinterpret_cast<const T *>(v + (layer * v_ls + tok * v_ts + h * v_hs) * c.size + u * sizeof(T));
+    *reinterpret_cast<T *>(static_cast<char *>(c.k) + to) = a;
+    *reinterpret_cast<T *>(static_cast<char *>(c.v) + to) = b;
+  };
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const int x = threadIdx.x + 256 * i;
+    if (x < all && place[x / units % ROWS] >= 0) put(x, kk[i], vv[i]);
   }
+#pragma unroll 2
+  for (int x = threadIdx.x + 256 * U; x < all; x += 256)
+    if (place[x / units % ROWS] >= 0) {
+      const T a = *source(k, k_ts, k_hs, k_ls, x), b = *source(v, v_ts, v_hs, v_ls, x);
+      put(x, a, b);
+    }
 }
 
 // Slots [first, first + n) become what the slots src[i] were.  A CTA owns a
 // few columns of the table for all n rows and reads them before it writes
 // any, so sources may be among the rows written and repeat.
 __global__ void __launch_bounds__(256) cache_fork_kernel(const CacheView c, const int *__restrict__ src, int first, int n, int cols) {
-  extern __shared__ int fork_sh[];  // [n][cols]
+  extern __shared__ int fork_sh[];  // sources [n], new entries [n][cols]
+  int *from = fork_sh, *entry = fork_sh + n;
   pdl_wait();
   pdl_trigger();
-  if (c.state[kStateStatus]) return;
+  const int status = c.state[kStateStatus];
   const int col0 = blockIdx.x * cols;
   const int width = min(cols, c.max_pages - col0);
   const bool lens_too = blockIdx.x == gridDim.x - 1;  // one more CTA moves the lengths
-  auto source = [&](int i) { return src ? __ldg(src + i) : -1; };
   // Every CTA looks at all sources, so that a bad one leaves all columns alone.
-  int wrong = 0;
+  int wrong = status;
   for (int i = threadIdx.x; i < n; i += blockDim.x) {
-    const int f = source(i);
+    const int f = src ? __ldg(src + i) : -1;
+    from[i] = f;
     wrong |= f < -1 || f >= c.slots;
   }
   if (__syncthreads_or(wrong)) {
-    if (lens_too && threadIdx.x == 0) atomicOr(c.state + kStateStatus, kCacheBadIndex);
+    if (lens_too && threadIdx.x == 0 && !status) atomicOr(c.state + kStateStatus, kCacheBadIndex);
     return;
   }
   if (lens_too) {
-    for (int i = threadIdx.x; i < n; i += blockDim.x) {
-      const int f = source(i);
-      fork_sh[i] = f < 0 ? 0 : c.lens[f];
-    }
+    for (int i = threadIdx.x; i < n; i += blockDim.x) entry[i] = from[i] < 0 ? 0 : c.lens[from[i]];
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += blockDim.x) c.lens[first + i] = fork_sh[i];
+    for (int i = threadIdx.x; i < n; i += blockDim.x) c.lens[first + i] = entry[i];
     return;
   }
+  int *rows = c.table + static_cast<int64_t>(first) * c.max_pages + col0;
+#pragma unroll 4
   for (int x = threadIdx.x; x < n * cols; x += blockDim.x) {
-    const int i = x / cols, col = x % cols, f = source(i);
-    fork_sh[x] = f < 0 || col >= width ? -1 : c.table[static_cast<int64_t>(f) * c.max_pages + col0 + col];
+    const int i = x / cols, col = x % cols, f = from[i];
+    entry[x] = f < 0 || col >= width ? -1 : c.table[static_cast<int64_t>(f) * c.max_pages + col0 + col];
   }
   __syncthreads();
+#pragma unroll 4
   for (int x = threadIdx.x; x < n * cols; x += blockDim.x) {
     const int i = x / cols, col = x % cols;
     if (col >= width) continue;
-    int *e = c.table + static_cast<int64_t>(first + i) * c.max_pages + col0 + col;
-    const int was = *e, is = fork_sh[x];
+    int *e = rows + static_cast<int64_t>(i) * c.max_pages + col;
+    const int was = *e, is = entry[x];
     if (was == is) continue;
     if (is >= 0 && is < c.pages) atomicAdd(c.refs + is, 1);
     if (was >= 0 && was < c.pages) atomicSub(c.refs + was, 1);
@@ -395,7 +426,7 @@ __global__ void __launch_bounds__(kBlock) cache_plan_kernel(const CacheView c) {
 }
 
 // The moves' data and the table's new page numbers.
-constexpr int kMoveBytes = 16384;
+constexpr int kMoveBytes = 24576;  // at most, of a CTA's turn
 __global__ void __launch_bounds__(256) cache_move_kernel(const CacheView c) {
   pdl_wait();
   pdl_trigger();
@@ -410,16 +441,17 @@ __global__ void __launch_bounds__(256) cache_move_kernel(const CacheView c) {
   }
   const int64_t page_bytes = (static_cast<int64_t>(c.dim) * c.kv_heads << c.page_shift) * c.size;  // a multiple of 16
   const int pieces = static_cast<int>((page_bytes + kMoveBytes - 1) / kMoveBytes);
+  const int64_t piece_bytes = ((page_bytes + pieces - 1) / pieces + 15) / 16 * 16;  // equal ones
   const int64_t units = static_cast<int64_t>(moves) * c.layers * 2 * pieces;
   for (int64_t x = blockIdx.x; x < units; x += gridDim.x) {
     const int piece = static_cast<int>(x % pieces);
     const int64_t y = x / pieces;
     const int side = static_cast<int>(y & 1), layer = static_cast<int>((y >> 1) % c.layers), i = static_cast<int>((y >> 1) / c.layers);
     char *pool = static_cast<char *>(side ? c.v : c.k);
-    const int64_t lo = static_cast<int64_t>(piece) * kMoveBytes;
+    const int64_t lo = piece * piece_bytes;
     const uint4 *src = reinterpret_cast<const uint4 *>(pool + (static_cast<int64_t>(layer) * c.pages + from[i]) * page_bytes + lo);
     uint4 *dst = reinterpret_cast<uint4 *>(pool + (static_cast<int64_t>(layer) * c.pages + to[i]) * page_bytes + lo);
-    const int n = static_cast<int>((page_bytes - lo < kMoveBytes ? page_bytes - lo : kMoveBytes) / 16);
+    const int n = static_cast<int>((page_bytes - lo < piece_bytes ? page_bytes - lo : piece_bytes) / 16);
     constexpr int U = kMoveBytes / 16 / 256;
     uint4 r[U];
 #pragma unroll
@@ -459,22 +491,25 @@ cudaError_t launch_cache_reserve(const CacheView &c, const int *offsets, int uni
 cudaError_t launch_cache_write(const CacheView &c, const void *k, const void *v, int64_t ts, int64_t hs, int64_t ls, int64_t v_ts,
                                int64_t v_hs, int64_t v_ls, int layer, int layers, int rows, const int *offsets, int uniform,
                                int first, int n, cudaStream_t s) {
-  const dim3 grid((rows + kWriteRows - 1) / kWriteRows, layers);
   auto fits = [&](int unit) {
     const int64_t x = reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | (ts * c.size) | (hs * c.size) | (ls * c.size) |
                       (v_ts * c.size) | (v_hs * c.size) | (v_ls * c.size) | (static_cast<int64_t>(c.dim) * c.size);
     return x % unit == 0;
   };
-  auto go = [&](auto kern) {
-    return launch_pdl(kern, grid, dim3(256), 0, s, 1, c, static_cast<const char *>(k), static_cast<const char *>(v), ts, hs, ls, v_ts,
-                      v_hs, v_ls, layer, rows, offsets, uniform, first, n);
+  auto go = [&](auto kern, int each) {
+    return launch_pdl(kern, dim3((rows + each - 1) / each, layers), dim3(256), 0, s, 1, c, static_cast<const char *>(k),
+                      static_cast<const char *>(v), ts, hs, ls, v_ts, v_hs, v_ls, layer, rows, offsets, uniform, first, n);
   };
-  return fits(16) ? go(cache_write_kernel<uint4>) : fits(4) ? go(cache_write_kernel<uint32_t>) : go(cache_write_kernel<uint16_t>);
+  // A step's few tokens are spread over more CTAs.
+  const bool few = static_cast<int64_t>(rows) * layers < 16 * 1024;
+  if (fits(16)) return few ? go(cache_write_kernel<uint4, 4>, 4) : go(cache_write_kernel<uint4, 16>, 16);
+  return fits(4) ? go(cache_write_kernel<uint32_t, 16>, 16) : go(cache_write_kernel<uint16_t, 16>, 16);
 }
 
 cudaError_t launch_cache_fork(const CacheView &c, const int *src, int first, int n, cudaStream_t s) {
-  const int cols = n <= 1024 ? 32 : 8;  // at most 128 KB of shared memory
-  const size_t smem = static_cast<size_t>(n) * cols * 4;
+  // Few columns a CTA: two entries a thread, and whole 32-byte sectors; at most 144 KB of shared memory.
+  const int cols = n <= 16 ? 32 : n <= 32 ? 16 : 8;
+  const size_t smem = static_cast<size_t>(n) * (cols + 1) * 4;
   const cudaError_t e = set_smem<cache_fork_kernel>(smem);
   if (e != cudaSuccess) return e;
   return launch_pdl(cache_fork_kernel, dim3((c.max_pages + cols - 1) / cols + 1), dim3(256), smem, s, 1, c, src, first, n, cols);
