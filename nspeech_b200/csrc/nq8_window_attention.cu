@@ -12,7 +12,7 @@
 // rounded to bf16 as the MMA's operand.  Few rows (a decoder's token): the
 // four warps take different keys of each tile and join at the end, so a step
 // streams K and V at the rate of memory instead of idling three warps.
-// f32: products in f32 FMA (no tensor-core form holds 24 bits).
+// f32: products as three tf32 products, or by FMA for single tokens.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -49,12 +49,41 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
                : "memory");
 }
 
-// Element offset of key j's row for kv head h; -1 where the key's page is
-// missing or the key is outside the tile's keys (its row reads as zeros).
+// The keys that a row tile sees, one after the other: the sinks [0, s_end),
+// then the window from lo on.  Tiles are cut from this list, so a few sinks
+// cost no tile of their own.
+struct KeyList {
+  int lo, s_end, n;
+  int tiles;
+  __device__ __forceinline__ int key(int u) const { return u < s_end ? u : u - s_end + lo; }
+};
+template <int KT>
+__device__ __forceinline__ KeyList list_of(const WinAttnParams &p, const Seq &s, int i_first, int i_last) {
+  const Keys k = keys_of<1>(p, s, i_first, i_last);
+  KeyList l{k.lo, k.s_end, k.s_end + max(0, k.hi - k.lo + 1), 0};
+  l.tiles = (l.n + KT - 1) / KT;
+  return l;
+}
+// Whether every row between positions pos_lo and pos_hi sees all of the list's
+// entries [u, u + KT).
+template <int KT>
+__device__ __forceinline__ bool all_see(const WinAttnParams &p, const Seq &s, const KeyList &k, int u, int pos_lo, int pos_hi) {
+  const int j = k.key(u);
+  return u >= k.s_end && u + KT <= k.n && j + KT - 1 <= (p.right >= kWinUnlimited ? s.nk - 1 : min(s.nk - 1, pos_lo + p.right)) &&
+         (p.left >= kWinUnlimited || j >= pos_hi - p.left);
+}
+// Whether a row at position `at` sees the list's entry u.
+__device__ __forceinline__ bool sees(const WinAttnParams &p, const KeyList &k, int u, int at) {
+  const int j = k.key(u);
+  return u < k.n && (p.right >= kWinUnlimited || j <= at + p.right) && (p.left >= kWinUnlimited || j >= at - p.left || j < p.sinks);
+}
+
+// Element offset of the row of entry u for kv head h; -1 past the list's end
+// and where the key's page is missing (the row reads as zeros).
 template <bool PAGED>
-__device__ __forceinline__ int64_t key_row(const WinAttnParams &p, const Keys &k, const Seq &s, const int *table, int h,
-                                           int j, bool v) {
-  if (!key_there(k, j)) return -1;
+__device__ __forceinline__ int64_t key_row(const WinAttnParams &p, const KeyList &k, const Seq &s, const int *table, int h, int u, bool v) {
+  if (u >= k.n) return -1;
+  const int j = k.key(u);
   if constexpr (PAGED) {
     const int pg = __ldg(table + (j >> p.page_shift));
     if (pg < 0 || pg >= p.pages) return -1;
@@ -140,7 +169,7 @@ __global__ void __launch_bounds__(kThreads) win_attn_mma(const __grid_constant__
   const int h = blockIdx.y, G = p.group;
   const int n_rows = s.nq * G;
   const int r_last = min(row0 + R, n_rows) - 1;
-  const Keys k = keys_of<KT>(p, s, row0 / G, r_last / G);
+  const KeyList k = list_of<KT>(p, s, row0 / G, r_last / G);
   const int t0 = static_cast<int>(static_cast<int64_t>(k.tiles) * blockIdx.z / p.splits);
   const int t1 = static_cast<int>(static_cast<int64_t>(k.tiles) * (blockIdx.z + 1) / p.splits);
   const int nt = t1 - t0;
@@ -152,7 +181,7 @@ __global__ void __launch_bounds__(kThreads) win_attn_mma(const __grid_constant__
     if constexpr (PAGED) {
       if (warp < 2 && t < nt) {
         const int slot = t % L::kRing;
-        const int j = tile_base<KT>(k, t0 + t) + tid;
+        const int j = (t0 + t) * KT + tid;
         const int64_t o = key_row<true>(p, k, s, table, h, j, false);
         row_off[slot * KT + tid] = o;
         const unsigned m = __ballot_sync(0xffffffffu, o < 0);
@@ -179,7 +208,7 @@ __global__ void __launch_bounds__(kThreads) win_attn_mma(const __grid_constant__
   auto sw = [](int row, int c) { return static_cast<uint32_t>(row * (DP * 2) + ((c ^ (row & 7)) << 4)); };
   auto load_tile = [&](int t) {
     if (t < nt) {
-      const int st = t % STAGES, slot = t % L::kRing, base = tile_base<KT>(k, t0 + t);
+      const int st = t % STAGES, slot = t % L::kRing, base = (t0 + t) * KT;
       const uint32_t ks = sb + L::kOffK + st * L::kTileBytes, vs = sb + L::kOffV + st * L::kTileBytes;
       const int c = tid % CH;
 #pragma unroll
@@ -237,7 +266,7 @@ __global__ void __launch_bounds__(kThreads) win_attn_mma(const __grid_constant__
     }
     load_tile(t + STAGES - 1);
     rows_of_tile(t + STAGES);
-    const int st = t % STAGES, slot = t % L::kRing, base = tile_base<KT>(k, t0 + t);
+    const int st = t % STAGES, slot = t % L::kRing, base = (t0 + t) * KT;
     const uint32_t ks = sb + L::kOffK + st * L::kTileBytes, vs = sb + L::kOffV + st * L::kTileBytes;
     float sc[KW / 8][4];
 #pragma unroll
@@ -261,9 +290,7 @@ __global__ void __launch_bounds__(kThreads) win_attn_mma(const __grid_constant__
       hole[0] = holes[slot * 2];
       hole[1] = holes[slot * 2 + 1];
     }
-    // every row of the tile sees every key of it
-    const bool inside = base + KT - 1 <= k.hi && base + KT - 1 <= min(s.nk - 1, p.right >= kWinUnlimited ? s.nk - 1 : pos_lo + p.right) &&
-                        (p.left >= kWinUnlimited || base >= pos_hi - p.left || base + KT <= p.sinks) && !(hole[0] | hole[1]);
+    const bool inside = all_see<KT>(p, s, k, base, pos_lo, pos_hi) && !(hole[0] | hole[1]);
     float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int n = 0; n < KW / 8; ++n)
@@ -271,10 +298,8 @@ __global__ void __launch_bounds__(kThreads) win_attn_mma(const __grid_constant__
       for (int e = 0; e < 4; ++e) {
         float x = sc[n][e] * p.sl2;
         if (!inside) {
-          const int jl = wk * KW + 8 * n + 2 * (lane & 3) + (e & 1), j = base + jl;
-          const int at = pos[e >> 1];
-          const bool see = key_there(k, j) && (p.right >= kWinUnlimited || j <= at + p.right) &&
-                           (p.left >= kWinUnlimited || j >= at - p.left || j < p.sinks) && !((hole[jl >> 5] >> (jl & 31)) & 1u);
+          const int jl = wk * KW + 8 * n + 2 * (lane & 3) + (e & 1);
+          const bool see = sees(p, k, base + jl, pos[e >> 1]) && !((hole[jl >> 5] >> (jl & 31)) & 1u);
           x = see ? x : -INFINITY;
         }
         sc[n][e] = x;
@@ -417,15 +442,22 @@ __global__ void __launch_bounds__(kThreads) win_attn_mma(const __grid_constant__
 }
 
 // ----------------------------------------------------------------------- f32
-// Tile form: 64 rows x 32 keys, 4 x 4 scores and 4 x DP / 8 outputs a thread.
+// Tile form, on the tensor cores: a product of two f32 as three tf32 products,
+// x y = xh yh + xh yl + xl yh with xh = x rounded to tf32 (11 bits) and xl =
+// x - xh (exact, taken at 11 bits): 2^-20 of |x y| at most is lost, 2^-22 on
+// the mean.  The tensor cores add with truncation, so their sums are kept
+// short: the large and the small products apart, and an output's sum over the
+// 32 keys of a tile is added to the running one in f32.  (FMA form of the same
+// tile: bound by shared memory, 128-bit loads of operands that only 16
+// products each use; 32 segments of up to 1501 tokens 544 us, this 1XX us.)
 template <int DP>
 struct F32Smem {
-  static constexpr int kR = 64, kKT = 32, kP = DP + 4, kPP = kKT + 4;
-  static constexpr int kOffQ = 0;
-  static constexpr int kOffK = kOffQ + kR * kP * 4;
-  static constexpr int kOffV = kOffK + 2 * kKT * kP * 4;
-  static constexpr int kOffP = kOffV + 2 * kKT * kP * 4;
-  static constexpr int kOffRow = kOffP + kR * kPP * 4;
+  static constexpr int kKT = 32, kP = DP + 4;  // pitch: rows 16 bytes apart in the banks
+  static constexpr int kTileBytes = kKT * kP * 4;
+  static constexpr int kOffK = 0;
+  static constexpr int kOffV = 2 * kTileBytes;
+  static constexpr int kOffQ = 4 * kTileBytes;
+  static constexpr int kOffRow = kOffQ + 64 * kP * 4;
   static constexpr int kBytes = kOffRow + 3 * kKT * 8;
 };
 
@@ -444,34 +476,44 @@ __device__ __forceinline__ void copy4(float *dst, const float *src, bool there, 
     *reinterpret_cast<float4 *>(dst) = x;
   }
 }
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void split_tf32(uint32_t x, uint32_t &hi, uint32_t &lo) {
+  hi = (x + 0x1000u) & 0xffffe000u;  // to nearest
+  lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi));
+}
 
-template <int DP, bool PAGED, bool VEC>
-__global__ void __launch_bounds__(kThreads) win_attn_f32(const __grid_constant__ WinAttnParams p) {
+template <int DP, int WR, bool PAGED, bool VEC>
+__global__ void __launch_bounds__(kThreads) win_attn_tf32(const __grid_constant__ WinAttnParams p) {
   using L = F32Smem<DP>;
-  constexpr int R = L::kR, KT = L::kKT, P = L::kP, PP = L::kPP, CH = DP / 4, NC = DP / 32;
+  constexpr int KT = L::kKT, WK = 4 / WR, KW = KT / WK, R = 16 * WR, P = L::kP, CH = DP / 4;
   extern __shared__ __align__(128) uint8_t smem[];
-  float *qs = reinterpret_cast<float *>(smem + L::kOffQ), *ps = reinterpret_cast<float *>(smem + L::kOffP);
+  const uint32_t sb = smem_u32(smem);
   int64_t *row_off = reinterpret_cast<int64_t *>(smem + L::kOffRow);
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_wait();
   pdl_trigger();
   int b, row0;
   if (!find_tile(p, gridDim.x - 1 - blockIdx.x, R, b, row0)) return;
   const Seq s = seq_of(p, b);
   const int h = blockIdx.y, G = p.group, n_rows = s.nq * G, r_last = min(row0 + R, n_rows) - 1;
-  const Keys k = keys_of<KT>(p, s, row0 / G, r_last / G);
+  const KeyList k = list_of<KT>(p, s, row0 / G, r_last / G);
   const int t0 = static_cast<int>(static_cast<int64_t>(k.tiles) * blockIdx.z / p.splits);
   const int nt = static_cast<int>(static_cast<int64_t>(k.tiles) * (blockIdx.z + 1) / p.splits) - t0;
   const int *table = PAGED ? p.table + static_cast<int64_t>(b) * p.table_ld : nullptr;
   const float *kp = static_cast<const float *>(p.k), *vp = static_cast<const float *>(p.v), *qp = static_cast<const float *>(p.q);
   auto rows_of_tile = [&](int t) {
-    if (PAGED && tid < KT && t < nt) row_off[(t % 3) * KT + tid] = key_row<true>(p, k, s, table, h, tile_base<KT>(k, t0 + t) + tid, false);
+    if (PAGED && tid < KT && t < nt) row_off[(t % 3) * KT + tid] = key_row<true>(p, k, s, table, h, (t0 + t) * KT + tid, false);
   };
   auto load_tile = [&](int t) {
     if (t < nt) {
       float *ks = reinterpret_cast<float *>(smem + L::kOffK) + (t & 1) * KT * P;
       float *vs = reinterpret_cast<float *>(smem + L::kOffV) + (t & 1) * KT * P;
-      const int c = (tid % CH) * 4, base = tile_base<KT>(k, t0 + t);
+      const int c = (tid % CH) * 4, base = (t0 + t) * KT;
 #pragma unroll
       for (int r = tid / CH; r < KT; r += kThreads / CH) {
         int64_t ok, ov;
@@ -487,6 +529,7 @@ __global__ void __launch_bounds__(kThreads) win_attn_f32(const __grid_constant__
     }
     cp_commit();
   };
+  float *qs = reinterpret_cast<float *>(smem + L::kOffQ);
   for (int x = tid; x < R * CH; x += kThreads) {
     const int r = x / CH, c = (x % CH) * 4, rr = row0 + r;
     const bool there = rr < n_rows;
@@ -497,128 +540,201 @@ __global__ void __launch_bounds__(kThreads) win_attn_f32(const __grid_constant__
   rows_of_tile(1);
   __syncthreads();
   load_tile(0);
-  const int ty = tid >> 3, tx = tid & 7;  // rows ty + 16 i, keys tx + 8 j, columns 4 tx + 32 j
-  int pos[4];
+  const int wr = warp % WR, wk = warp / WR;
+  const int qr = lane >> 2, qc = lane & 3;  // this thread's rows qr, qr + 8 of the warp's 16
+  int pos[2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) pos[i] = s.nk - s.nq + min(row0 + ty + 16 * i, n_rows - 1) / G;
-  float m[4], l[4], o[4][4 * NC];
+  for (int x = 0; x < 2; ++x) pos[x] = s.nk - s.nq + min(row0 + 16 * wr + qr + 8 * x, n_rows - 1) / G;
+  const int pos_lo = s.nk - s.nq + row0 / G, pos_hi = s.nk - s.nq + r_last / G;
+  float o[DP / 8][4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    m[i] = -INFINITY;
-    l[i] = 0.f;
+  for (int d = 0; d < DP / 8; ++d)
 #pragma unroll
-    for (int c = 0; c < 4 * NC; ++c) o[i][c] = 0.f;
-  }
+    for (int e = 0; e < 4; ++e) o[d][e] = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  const uint32_t q_at = sb + L::kOffQ + ((16 * wr + (lane & 7) + ((lane >> 3) & 1) * 8) * P + (lane >> 4) * 4) * 4;
   for (int t = 0; t < nt; ++t) {
     load_tile(t + 1);
     cp_wait<1>();
     __syncthreads();
     rows_of_tile(t + 2);
-    const float *ks = reinterpret_cast<const float *>(smem + L::kOffK) + (t & 1) * KT * P;
+    const uint32_t ks = sb + L::kOffK + (t & 1) * L::kTileBytes;
     const float *vs = reinterpret_cast<const float *>(smem + L::kOffV) + (t & 1) * KT * P;
-    const int base = tile_base<KT>(k, t0 + t);
-    float sc[4][4];
+    const int base = (t0 + t) * KT;
+    // Scores: KW / 8 tiles of 8 keys.
+    constexpr int N = KW / 8;
+    float hi[N][4], lo[N][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int n = 0; n < N; ++n)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sc[i][j] = 0.f;
-#pragma unroll 4
-    for (int d = 0; d < DP; d += 4) {
-      float4 a[4], c[4];
+      for (int e = 0; e < 4; ++e) hi[n][e] = lo[n][e] = 0.f;
+    auto products = [&](int n, const uint32_t (&ah)[4], const uint32_t (&al)[4], uint32_t x0, uint32_t x1) {
+      uint32_t h0, l0, h1, l1;
+      split_tf32(x0, h0, l0);
+      split_tf32(x1, h1, l1);
+      mma_tf32(hi[n], ah, h0, h1);
+      mma_tf32(lo[n], ah, l0, l1);
+      mma_tf32(lo[n], al, h0, h1);
+    };
+    if constexpr (N >= 2) {
+      const uint32_t k_at = ks + ((wk * KW + (lane & 7) + ((lane >> 4) << 3)) * P + ((lane >> 3) & 1) * 4) * 4;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4 *>(qs + (ty + 16 * i) * P + d);
+      for (int kk = 0; kk < DP / 8; ++kk) {
+        uint32_t a[4], ah[4], al[4];
+        ldsm4(a, q_at + kk * 32);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) c[j] = *reinterpret_cast<const float4 *>(ks + (tx + 8 * j) * P + d);
+        for (int e = 0; e < 4; ++e) split_tf32(a[e], ah[e], al[e]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          sc[i][j] = fmaf(a[i].x, c[j].x, sc[i][j]);
-          sc[i][j] = fmaf(a[i].y, c[j].y, sc[i][j]);
-          sc[i][j] = fmaf(a[i].z, c[j].z, sc[i][j]);
-          sc[i][j] = fmaf(a[i].w, c[j].w, sc[i][j]);
+        for (int n = 0; n < N; n += 2) {
+          uint32_t f[4];
+          ldsm4(f, k_at + n * 8 * P * 4 + kk * 32);
+          products(n, ah, al, f[0], f[1]);
+          products(n + 1, ah, al, f[2], f[3]);
         }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float top = m[i];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int key = base + tx + 8 * j;
-        bool see = key_there(k, key) && (p.right >= kWinUnlimited || key <= pos[i] + p.right) &&
-                   (p.left >= kWinUnlimited || key >= pos[i] - p.left || key < p.sinks);
-        if (PAGED) see = see && row_off[(t % 3) * KT + tx + 8 * j] >= 0;
-        sc[i][j] = see ? sc[i][j] * p.sl2 : -INFINITY;
-        top = fmaxf(top, sc[i][j]);
       }
+    } else {
+      const uint32_t k_at = ks + ((wk * KW + (lane & 7)) * P + (lane >> 3) * 4) * 4;
 #pragma unroll
-      for (int x = 1; x < 8; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-      const float ref = top == -INFINITY ? 0.f : top;
-      const float f = exp2f(m[i] - ref);
-      m[i] = top;
-      l[i] *= f;
+      for (int kk = 0; kk < DP / 8; kk += 2) {
+        uint32_t f[4];
+        ldsm4(f, k_at + kk * 32);
 #pragma unroll
-      for (int c = 0; c < 4 * NC; ++c) o[i][c] *= f;
+        for (int x = 0; x < 2; ++x) {
+          uint32_t a[4], ah[4], al[4];
+          ldsm4(a, q_at + (kk + x) * 32);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float e = exp2f(sc[i][j] - ref);
-        l[i] += e;
-        ps[(ty + 16 * i) * PP + tx + 8 * j] = e;
+          for (int e = 0; e < 4; ++e) split_tf32(a[e], ah[e], al[e]);
+          products(0, ah, al, f[2 * x], f[2 * x + 1]);
+        }
       }
     }
-    __syncwarp();  // a row's eight threads are of one warp
-#pragma unroll 2
-    for (int j = 0; j < KT; j += 4) {
-      float4 e[4];
+    bool inside = all_see<KT>(p, s, k, base, pos_lo, pos_hi);
+    if constexpr (PAGED) inside = __all_sync(0xffffffffu, inside && row_off[(t % 3) * KT + lane] >= 0);
+    float top[2] = {m[0], m[1]};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) e[i] = *reinterpret_cast<const float4 *>(ps + (ty + 16 * i) * PP + j);
+    for (int n = 0; n < N; ++n)
 #pragma unroll
-      for (int jj = 0; jj < 4; ++jj)
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          const float4 x = *reinterpret_cast<const float4 *>(vs + (j + jj) * P + 32 * c + 4 * tx);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float w = jj == 0 ? e[i].x : jj == 1 ? e[i].y : jj == 2 ? e[i].z : e[i].w;
-            o[i][4 * c] = fmaf(w, x.x, o[i][4 * c]);
-            o[i][4 * c + 1] = fmaf(w, x.y, o[i][4 * c + 1]);
-            o[i][4 * c + 2] = fmaf(w, x.z, o[i][4 * c + 2]);
-            o[i][4 * c + 3] = fmaf(w, x.w, o[i][4 * c + 3]);
-          }
+      for (int e = 0; e < 4; ++e) {
+        float x = (hi[n][e] + lo[n][e]) * p.sl2;
+        if (!inside) {
+          const int jl = wk * KW + 8 * n + 2 * qc + (e & 1);
+          bool see = sees(p, k, base + jl, pos[e >> 1]);
+          if constexpr (PAGED) see = see && row_off[(t % 3) * KT + jl] >= 0;
+          x = see ? x : -INFINITY;
         }
+        hi[n][e] = x;
+        top[e >> 1] = fmaxf(top[e >> 1], x);
+      }
+    float ref[2], f[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 1));
+      top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 2));
+      ref[x] = top[x] == -INFINITY ? 0.f : top[x];
+      f[x] = ex2(m[x] - ref[x]);
+      l[x] *= f[x];
+      m[x] = top[x];
+    }
+    // Weights as the A operand: this thread's keys 2 qc and 2 qc + 1 stand in
+    // columns qc and qc + 4, for V alike.
+    uint32_t ah[N][4], al[N][4];
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float w = ex2(hi[n][e] - ref[e >> 1]);
+        l[e >> 1] += w;
+        constexpr int to[4] = {0, 2, 1, 3};
+        split_tf32(__float_as_uint(w), ah[n][to[e]], al[n][to[e]]);
+      }
+#pragma unroll
+    for (int d = 0; d < DP / 8; ++d) {
+      float big[4] = {0.f, 0.f, 0.f, 0.f}, small[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const float *v = vs + (wk * KW + 8 * n + 2 * qc) * P + 8 * d + qr;
+        uint32_t h0, l0, h1, l1;
+        split_tf32(__float_as_uint(v[0]), h0, l0);
+        split_tf32(__float_as_uint(v[P]), h1, l1);
+        mma_tf32(big, ah[n], h0, h1);
+        mma_tf32(small, ah[n], l0, l1);
+        mma_tf32(small, al[n], h0, h1);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[d][e] = fmaf(o[d][e], f[e >> 1], big[e] + small[e]);
     }
     __syncthreads();
   }
   cp_wait<0>();
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
+    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
+  }
   const int heads = p.kv_heads * G;
   const int64_t all = static_cast<int64_t>(p.q_rows) * heads;
+  float *outp = static_cast<float *>(p.out);
+  if constexpr (WK == 1) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+    for (int x = 0; x < 2; ++x) {
+      const int r = row0 + 16 * wr + qr + 8 * x;
+      if (r >= n_rows) continue;
+      const int i = r / G, hq = h * G + r % G;
+      const int64_t row = blockIdx.z * all + static_cast<int64_t>(s.q0 + i) * heads + hq;
+      if (p.splits > 1 && qc == 0) p.part_ml[row] = make_float2(m[x], l[x]);
+      const float inv = p.splits > 1 ? 1.f : l[x] > 0.f ? 1.f / l[x] : (l[x] == 0.f ? 0.f : l[x]);
+      float *out = p.splits > 1 ? p.part_o + row * DP : outp + (s.q0 + static_cast<int64_t>(i)) * p.o_ts + hq * p.o_hs;
+      const int width = p.splits > 1 ? DP : p.dim;
 #pragma unroll
-    for (int x = 1; x < 8; x <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], x);
-    const int rr = row0 + ty + 16 * i;
-    if (rr >= n_rows) continue;
-    const int tok = rr / G, hq = h * G + rr % G;
-    if (p.splits > 1) {
-      const int64_t row = blockIdx.z * all + static_cast<int64_t>(s.q0 + tok) * heads + hq;
-      if (tx == 0) p.part_ml[row] = make_float2(m[i], l[i]);
-#pragma unroll
-      for (int c = 0; c < NC; ++c)
-        *reinterpret_cast<float4 *>(p.part_o + row * DP + 32 * c + 4 * tx) = make_float4(o[i][4 * c], o[i][4 * c + 1], o[i][4 * c + 2], o[i][4 * c + 3]);
-    } else {
-      const float inv = l[i] > 0.f ? 1.f / l[i] : (l[i] == 0.f ? 0.f : l[i]);
-      float *out = static_cast<float *>(p.out) + (s.q0 + static_cast<int64_t>(tok)) * p.o_ts + hq * p.o_hs;
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const int col = 32 * c + 4 * tx;
+      for (int d = 0; d < DP / 8; ++d) {
+        const int c = 8 * d + 2 * qc;
         if constexpr (VEC) {
-          if (col < p.dim)
-            *reinterpret_cast<float4 *>(out + col) = make_float4(o[i][4 * c] * inv, o[i][4 * c + 1] * inv, o[i][4 * c + 2] * inv, o[i][4 * c + 3] * inv);
+          if (c < width) *reinterpret_cast<float2 *>(out + c) = make_float2(o[d][2 * x] * inv, o[d][2 * x + 1] * inv);
         } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (col + e < p.dim) out[col + e] = o[i][4 * c + e] * inv;
+          if (c < width) out[c] = o[d][2 * x] * inv;
+          if (c + 1 < width) out[c + 1] = o[d][2 * x + 1] * inv;
         }
+      }
+    }
+  } else {
+    // Join the WK warps of each 16 rows through shared memory.
+    float *jo = reinterpret_cast<float *>(smem);                // [4 warps][16][P]
+    float2 *jml = reinterpret_cast<float2 *>(smem + L::kOffQ);  // [4 warps][16]
+    static_assert(64 * P * 4 <= L::kOffQ, "the warps' join fits the key tiles");
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int r = 16 * warp + qr + 8 * x;
+      if (qc == 0) jml[r] = make_float2(m[x], l[x]);
+#pragma unroll
+      for (int d = 0; d < DP / 8; ++d) *reinterpret_cast<float2 *>(jo + r * P + 8 * d + 2 * qc) = make_float2(o[d][2 * x], o[d][2 * x + 1]);
+    }
+    __syncthreads();
+    constexpr int kPer = kThreads / R;
+    const int r = tid / kPer, rr = row0 + r;
+    if (rr < n_rows) {
+      const int w0 = r / 16;
+      float mm = -INFINITY, ll = 0.f, f[WK];
+#pragma unroll
+      for (int x = 0; x < WK; ++x) mm = fmaxf(mm, jml[16 * (w0 + WR * x) + r % 16].x);
+#pragma unroll
+      for (int x = 0; x < WK; ++x) {
+        const float2 ml = jml[16 * (w0 + WR * x) + r % 16];
+        f[x] = ml.x == -INFINITY ? 0.f : ex2(ml.x - mm);
+        ll += ml.y * f[x];
+      }
+      const int i = rr / G, hq = h * G + rr % G;
+      const int64_t row = blockIdx.z * all + static_cast<int64_t>(s.q0 + i) * heads + hq;
+      if (p.splits > 1 && tid % kPer == 0) p.part_ml[row] = make_float2(mm, ll);
+      const float inv = p.splits > 1 ? 1.f : ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
+      float *out = p.splits > 1 ? p.part_o + row * DP : outp + (s.q0 + static_cast<int64_t>(i)) * p.o_ts + hq * p.o_hs;
+      const int width = p.splits > 1 ? DP : p.dim;
+      for (int c = tid % kPer; c < width; c += kPer) {
+        float v = 0.f;
+#pragma unroll
+        for (int x = 0; x < WK; ++x)
+          if (f[x] != 0.f) v = fmaf(jo[(16 * (w0 + WR * x) + r % 16) * P + c], f[x], v);  // 0: a part without a visible key
+        out[c] = v * inv;
       }
     }
   }
@@ -640,7 +756,7 @@ __global__ void __launch_bounds__(kThreads) win_attn_f32_rows(const __grid_const
   if (!find_tile(p, gridDim.x - 1 - blockIdx.x, R, b, row0)) return;
   const Seq s = seq_of(p, b);
   const int h = blockIdx.y, G = p.group, n_rows = s.nq * G, r_last = min(row0 + R, n_rows) - 1;
-  const Keys k = keys_of<KT>(p, s, row0 / G, r_last / G);
+  const KeyList k = list_of<KT>(p, s, row0 / G, r_last / G);
   const int t0 = static_cast<int>(static_cast<int64_t>(k.tiles) * blockIdx.z / p.splits);
   const int t1 = static_cast<int>(static_cast<int64_t>(k.tiles) * (blockIdx.z + 1) / p.splits);
   const int *table = PAGED ? p.table + static_cast<int64_t>(b) * p.table_ld : nullptr;
@@ -669,26 +785,25 @@ __global__ void __launch_bounds__(kThreads) win_attn_f32_rows(const __grid_const
     m[r] = -INFINITY;
     l[r] = 0.f;
   }
-  // this lane's key rows of tile t
-  auto rows_of = [&](int t, int64_t (&off)[U]) {
-    const int base = t < t1 ? tile_base<KT>(k, t) : 0;
-#pragma unroll
-    for (int u = 0; u < U; ++u) off[u] = t < t1 ? key_row<PAGED>(p, k, s, table, h, base + u * KPL + sub, false) : -1;
+  // A lane for each of a tile's keys: where its rows are (-1: nowhere), handed
+  // to the lanes that load them.
+  auto row_of = [&](int t, bool v) -> int64_t {
+    return lane < KT && t < t1 ? key_row<PAGED>(p, k, s, table, h, t * KT + lane, v) : -1;
   };
-  int64_t off[U];
-  rows_of(t0 + warp, off);
+  int64_t mine = row_of(t0 + warp, false);
   for (int t = t0 + warp; t < t1; t += 4) {
-    const int base = tile_base<KT>(k, t);
+    const int64_t mine_v = PAGED || mine < 0 ? mine : row_of(t, true);
     float4 kk[U], vv[U];
-    bool there[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      there[u] = off[u] >= 0;
-      const int64_t ov = PAGED ? off[u] : key_row<PAGED>(p, k, s, table, h, base + u * KPL + sub, true);
-      kk[u] = fetch(kp + (there[u] ? off[u] : 0), there[u]);
-      vv[u] = fetch(vp + (there[u] ? ov : 0), there[u]);
+      const int64_t ok = __shfl_sync(0xffffffffu, mine, u * KPL + sub), ov = PAGED ? ok : __shfl_sync(0xffffffffu, mine_v, u * KPL + sub);
+      kk[u] = fetch(kp + (ok < 0 ? 0 : ok), ok >= 0);
+      vv[u] = fetch(vp + (ok < 0 ? 0 : ov), ok >= 0);
     }
-    rows_of(t + 4, off);
+    unsigned see[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) see[r] = __ballot_sync(0xffffffffu, mine >= 0 && sees(p, k, t * KT + lane, pos[r])) >> sub;
+    mine = row_of(t + 4, false);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       float sc[U], top = -INFINITY;
@@ -700,10 +815,7 @@ __global__ void __launch_bounds__(kThreads) win_attn_f32_rows(const __grid_const
         x = fmaf(q[r].w, kk[u].w, x);
 #pragma unroll
         for (int y = LPK / 2; y > 0; y >>= 1) x += __shfl_xor_sync(0xffffffffu, x, y);
-        const int key = base + u * KPL + sub;
-        const bool see = there[u] && (p.right >= kWinUnlimited || key <= pos[r] + p.right) &&
-                         (p.left >= kWinUnlimited || key >= pos[r] - p.left || key < p.sinks);
-        sc[u] = see ? x * p.sl2 : -INFINITY;
+        sc[u] = see[r] >> (u * KPL) & 1u ? x * p.sl2 : -INFINITY;
         top = fmaxf(top, sc[u]);
       }
       top = fmaxf(top, m[r]);  // each lane group keeps its own keys' maximum
@@ -789,7 +901,9 @@ cudaError_t launch_form(const WinAttnParams &p, int f32, const WinAttnPlan &pl, 
     if (pl.rows == 1) return launch_smem<win_attn_f32_rows<DP, 1, PAGED, VEC>>(grid, 0, stream, p);
     if (pl.rows == 2) return launch_smem<win_attn_f32_rows<DP, 2, PAGED, VEC>>(grid, 0, stream, p);
     if (pl.rows == 4) return launch_smem<win_attn_f32_rows<DP, 4, PAGED, VEC>>(grid, 0, stream, p);
-    return launch_smem<win_attn_f32<DP, PAGED, VEC>>(grid, F32Smem<DP>::kBytes, stream, p);
+    if (pl.rows == 16) return launch_smem<win_attn_tf32<DP, 1, PAGED, VEC>>(grid, F32Smem<DP>::kBytes, stream, p);
+    if (pl.rows == 32) return launch_smem<win_attn_tf32<DP, 2, PAGED, VEC>>(grid, F32Smem<DP>::kBytes, stream, p);
+    return launch_smem<win_attn_tf32<DP, 4, PAGED, VEC>>(grid, F32Smem<DP>::kBytes, stream, p);
   }
   if (pl.rows == 16) return launch_smem<win_attn_mma<DP, 1, kDeep, PAGED, VEC>>(grid, MmaSmem<DP, kDeep>::kBytes, stream, p);
   if (pl.rows == 32) return launch_smem<win_attn_mma<DP, 2, kDeep, PAGED, VEC>>(grid, MmaSmem<DP, kDeep>::kBytes, stream, p);
@@ -818,7 +932,7 @@ WinAttnPlan win_attn_plan(int sm_count, int f32, bool tensor, bool uniform, int 
   if (tensor) {
     pl.rows = 2 * (128 / group * group);
   } else if (f32) {
-    pl.rows = mean <= 1 ? 1 : mean <= 2 ? 2 : mean <= 4 ? 4 : 64;
+    pl.rows = mean <= 1 ? 1 : mean <= 2 ? 2 : mean <= 4 ? 4 : mean <= 16 ? 16 : mean <= 32 ? 32 : 64;
   } else {
     pl.rows = mean <= 16 ? 16 : mean <= 32 ? 32 : 64;
   }
@@ -830,11 +944,14 @@ WinAttnPlan win_attn_plan(int sm_count, int f32, bool tensor, bool uniform, int 
     keys = keys < static_cast<int64_t>(left) + right + sinks + pl.rows ? keys : static_cast<int64_t>(left) + right + sinks + pl.rows;
   const int64_t each = (rows + pl.rows - 1) / pl.rows;
   const int64_t have = (each > seqs ? each : seqs) * kv_heads;
-  // Two CTAs an SM of the warp-level forms, of at least 256 keys; one of the
-  // tensor-core form, of at least 1024 (it fills and drains in the time of 256).
-  const int64_t want = tensor ? sm_count : 2LL * sm_count;
+  // CTAs an SM that a split aims at, and the keys that each takes at least: the
+  // f32 row form (little shared memory, loads straight to registers) six of
+  // 128, the other warp-level forms two of 256, the tensor-core form one of
+  // 1024 (it fills and drains in the time of 256).
+  const bool rows_form = f32 && pl.rows <= 4;
+  const int64_t want = static_cast<int64_t>(tensor ? 1 : rows_form ? 6 : 2) * sm_count;
   int64_t z = have > 0 ? want / have : 1;
-  const int64_t most = keys / (tensor ? 1024 : 256);
+  const int64_t most = keys / (tensor ? 1024 : rows_form ? 128 : 256);
   z = z < most ? z : most;
   pl.splits = static_cast<int>(z < 1 ? 1 : z > 64 ? 64 : z);
   const int dp = dim <= 64 ? 64 : 128;

@@ -100,13 +100,5 @@ __device__ __forceinline__ Keys keys_of(const WinAttnParams &p, const Seq &s, in
   k.tiles = k.sink_tiles + (k.hi >= k.lo ? (k.hi - k.lo + KT) / KT : 0);
   return k;
 }
-template <int KT>
-__device__ __forceinline__ int tile_base(const Keys &k, int t) {
-  return t < k.sink_tiles ? t * KT : k.lo + (t - k.sink_tiles) * KT;
-}
-__device__ __forceinline__ bool key_there(const Keys &k, int j) {
-  return j <= k.hi && (j >= k.lo || j < k.s_end);
-}
-
 }  // namespace win
 }  // namespace nq
