@@ -64,6 +64,12 @@ __device__ __forceinline__ KeyList list_of(const WinAttnParams &p, const Seq &s,
   l.tiles = (l.n + KT - 1) / KT;
   return l;
 }
+// Tiles of a list that one of its `splits` CTAs takes: an equal share, but not
+// less than split_keys, so that short sequences take fewer CTAs.
+template <int KT>
+__device__ __forceinline__ int share_of(const WinAttnParams &p, int tiles) {
+  return max((tiles + p.splits - 1) / p.splits, p.split_keys / KT);
+}
 // Whether every row between positions pos_lo and pos_hi sees all of the list's
 // entries [u, u + KT).
 template <int KT>
@@ -137,7 +143,7 @@ __global__ void __launch_bounds__(kThreads) win_attn_join(const __grid_constant_
 
 // ---------------------------------------------------------------------- bf16
 // WR warps along the rows (16 each), WK = 4 / WR along the keys of a tile.
-template <int DP, int STAGES>
+template <int DP, int R, int STAGES>
 struct MmaSmem {
   static constexpr int kKT = 64;
   static constexpr int kTileBytes = kKT * DP * 2;
@@ -145,14 +151,14 @@ struct MmaSmem {
   static constexpr int kOffK = 0;
   static constexpr int kOffV = STAGES * kTileBytes;
   static constexpr int kOffQ = 2 * STAGES * kTileBytes;
-  static constexpr int kOffRow = kOffQ + 64 * DP * 2;
+  static constexpr int kOffRow = kOffQ + (R * DP * 2 > 512 ? R * DP * 2 : 512);  // the join's 64 maxima and sums lie there too
   static constexpr int kOffHole = kOffRow + kRing * kKT * 8;
   static constexpr int kBytes = kOffHole + kRing * 8;
 };
 
 template <int DP, int WR, int STAGES, bool PAGED, bool VEC>
 __global__ void __launch_bounds__(kThreads) win_attn_mma(const __grid_constant__ WinAttnParams p) {
-  using L = MmaSmem<DP, STAGES>;
+  using L = MmaSmem<DP, 16 * WR, STAGES>;
   constexpr int KT = L::kKT, WK = 4 / WR, KW = KT / WK, R = 16 * WR, CH = DP / 8;
   static_assert(4 * 16 * (DP + 4) * 4 <= 2 * STAGES * L::kTileBytes, "the warps' join fits the key tiles");
   extern __shared__ __align__(128) uint8_t smem[];
@@ -170,8 +176,7 @@ __global__ void __launch_bounds__(kThreads) win_attn_mma(const __grid_constant__
   const int n_rows = s.nq * G;
   const int r_last = min(row0 + R, n_rows) - 1;
   const KeyList k = list_of<KT>(p, s, row0 / G, r_last / G);
-  const int t0 = static_cast<int>(static_cast<int64_t>(k.tiles) * blockIdx.z / p.splits);
-  const int t1 = static_cast<int>(static_cast<int64_t>(k.tiles) * (blockIdx.z + 1) / p.splits);
+  const int share = share_of<KT>(p, k.tiles), t0 = min(static_cast<int>(blockIdx.z) * share, k.tiles), t1 = min(t0 + share, k.tiles);
   const int nt = t1 - t0;
   const int *table = PAGED ? p.table + static_cast<int64_t>(b) * p.table_ld : nullptr;
   const __nv_bfloat16 *kp = static_cast<const __nv_bfloat16 *>(p.k), *vp = static_cast<const __nv_bfloat16 *>(p.v);
@@ -502,8 +507,7 @@ __global__ void __launch_bounds__(kThreads) win_attn_tf32(const __grid_constant_
   const Seq s = seq_of(p, b);
   const int h = blockIdx.y, G = p.group, n_rows = s.nq * G, r_last = min(row0 + R, n_rows) - 1;
   const KeyList k = list_of<KT>(p, s, row0 / G, r_last / G);
-  const int t0 = static_cast<int>(static_cast<int64_t>(k.tiles) * blockIdx.z / p.splits);
-  const int nt = static_cast<int>(static_cast<int64_t>(k.tiles) * (blockIdx.z + 1) / p.splits) - t0;
+  const int share = share_of<KT>(p, k.tiles), t0 = min(static_cast<int>(blockIdx.z) * share, k.tiles), nt = min(share, k.tiles - t0);
   const int *table = PAGED ? p.table + static_cast<int64_t>(b) * p.table_ld : nullptr;
   const float *kp = static_cast<const float *>(p.k), *vp = static_cast<const float *>(p.v), *qp = static_cast<const float *>(p.q);
   auto rows_of_tile = [&](int t) {
@@ -757,8 +761,7 @@ __global__ void __launch_bounds__(kThreads) win_attn_f32_rows(const __grid_const
   const Seq s = seq_of(p, b);
   const int h = blockIdx.y, G = p.group, n_rows = s.nq * G, r_last = min(row0 + R, n_rows) - 1;
   const KeyList k = list_of<KT>(p, s, row0 / G, r_last / G);
-  const int t0 = static_cast<int>(static_cast<int64_t>(k.tiles) * blockIdx.z / p.splits);
-  const int t1 = static_cast<int>(static_cast<int64_t>(k.tiles) * (blockIdx.z + 1) / p.splits);
+  const int share = share_of<KT>(p, k.tiles), t0 = min(static_cast<int>(blockIdx.z) * share, k.tiles), t1 = min(t0 + share, k.tiles);
   const int *table = PAGED ? p.table + static_cast<int64_t>(b) * p.table_ld : nullptr;
   const float *kp = static_cast<const float *>(p.k), *vp = static_cast<const float *>(p.v), *qp = static_cast<const float *>(p.q);
   auto fetch = [&](const float *src, bool there) {
@@ -905,9 +908,9 @@ cudaError_t launch_form(const WinAttnParams &p, int f32, const WinAttnPlan &pl, 
     if (pl.rows == 32) return launch_smem<win_attn_tf32<DP, 2, PAGED, VEC>>(grid, F32Smem<DP>::kBytes, stream, p);
     return launch_smem<win_attn_tf32<DP, 4, PAGED, VEC>>(grid, F32Smem<DP>::kBytes, stream, p);
   }
-  if (pl.rows == 16) return launch_smem<win_attn_mma<DP, 1, kDeep, PAGED, VEC>>(grid, MmaSmem<DP, kDeep>::kBytes, stream, p);
-  if (pl.rows == 32) return launch_smem<win_attn_mma<DP, 2, kDeep, PAGED, VEC>>(grid, MmaSmem<DP, kDeep>::kBytes, stream, p);
-  return launch_smem<win_attn_mma<DP, 4, 2, PAGED, VEC>>(grid, MmaSmem<DP, 2>::kBytes, stream, p);
+  if (pl.rows == 16) return launch_smem<win_attn_mma<DP, 1, kDeep, PAGED, VEC>>(grid, MmaSmem<DP, 16, kDeep>::kBytes, stream, p);
+  if (pl.rows == 32) return launch_smem<win_attn_mma<DP, 2, kDeep, PAGED, VEC>>(grid, MmaSmem<DP, 32, kDeep>::kBytes, stream, p);
+  return launch_smem<win_attn_mma<DP, 4, 2, PAGED, VEC>>(grid, MmaSmem<DP, 64, 2>::kBytes, stream, p);
 }
 
 bool aligned16(const void *x, int64_t a, int64_t b, int size) {
@@ -951,8 +954,16 @@ WinAttnPlan win_attn_plan(int sm_count, int f32, bool tensor, bool uniform, int 
   const bool rows_form = f32 && pl.rows <= 4;
   const int64_t want = static_cast<int64_t>(tensor ? 1 : rows_form ? 6 : 2) * sm_count;
   int64_t z = have > 0 ? want / have : 1;
-  const int64_t most = keys / (tensor ? 1024 : rows_form ? 128 : 256);
+  pl.split_keys = tensor ? 1024 : rows_form ? 128 : 256;
+  const int64_t most = keys / pl.split_keys;
   z = z < most ? z : most;
+  // Few rows over long contexts: pieces of 1024 keys, so that sequences of
+  // unlike lengths keep all SMs busy to the end (64 sequences of 2048 to 8192
+  // tokens, 32/8 heads of 128: 540 us whole, XXX us in pieces).
+  if (!tensor && pl.rows <= 32 && keys >= 2048 && z < (keys + 1023) / 1024) {
+    z = (keys + 1023) / 1024;
+    pl.split_keys = 1024;
+  }
   pl.splits = static_cast<int>(z < 1 ? 1 : z > 64 ? 64 : z);
   const int dp = dim <= 64 ? 64 : 128;
   pl.workspace = pl.splits > 1 ? static_cast<size_t>(pl.splits) * q_rows * kv_heads * group * (dp * 4 + 8) : 0;

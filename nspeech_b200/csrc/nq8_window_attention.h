@@ -40,7 +40,7 @@ struct WinAttnParams {
   int table_ld, pages, page_shift, max_pages;
   // Split of a row tile's keys over gridDim.z CTAs: unnormalised outputs,
   // row maxima (log2 units) and sums, joined by a second kernel.
-  int splits;
+  int splits, split_keys;  // CTAs of a tile's keys, and the keys that each takes at least
   float *part_o;           // [splits][q_rows * query heads][dim padded to 64 or 128]
   float2 *part_ml;         // [splits][q_rows * query heads]
   DevCtl ctl;
@@ -49,7 +49,7 @@ struct WinAttnParams {
 // What a call runs as; a function of its sizes alone.
 struct WinAttnPlan {
   int rows;    // query rows (token, head of a group) of a CTA
-  int splits;
+  int splits, split_keys;
   int tiles;   // CTAs along x: an upper bound of the row tiles of all sequences
   size_t workspace;
 };
