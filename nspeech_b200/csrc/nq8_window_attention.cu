@@ -899,7 +899,7 @@ cudaError_t launch_smem(dim3 grid, size_t smem, cudaStream_t stream, const WinAt
 template <int DP, bool PAGED, bool VEC>
 cudaError_t launch_form(const WinAttnParams &p, int f32, const WinAttnPlan &pl, cudaStream_t stream) {
   const dim3 grid(pl.tiles, p.kv_heads, p.splits);
-  constexpr int kDeep = DP == 64 ? 4 : 3;
+  constexpr int kDeep = DP == 64 ? 3 : 2;  // three CTAs an SM and more (with one stage more, two CTAs: 311 for 258 us at 64 x 8192 tokens, 32/8 heads of 128)
   if (f32) {
     if (pl.rows == 1) return launch_smem<win_attn_f32_rows<DP, 1, PAGED, VEC>>(grid, 0, stream, p);
     if (pl.rows == 2) return launch_smem<win_attn_f32_rows<DP, 2, PAGED, VEC>>(grid, 0, stream, p);
@@ -939,8 +939,9 @@ WinAttnPlan win_attn_plan(int sm_count, int f32, bool tensor, bool uniform, int 
   } else {
     pl.rows = mean <= 16 ? 16 : mean <= 32 ? 32 : 64;
   }
-  // every sequence's last tile may be a part of one
-  pl.tiles = static_cast<int>(uniform ? seqs * ((mean + pl.rows - 1) / pl.rows) : rows / pl.rows + seqs);
+  // every sequence's last tile may hold as little as one row
+  const int64_t bound = (rows + static_cast<int64_t>(seqs) * (pl.rows - 1)) / pl.rows;
+  pl.tiles = static_cast<int>(uniform ? seqs * ((mean + pl.rows - 1) / pl.rows) : bound < rows ? bound : rows);
   // Keys of a tile at most, and the CTAs that the call has without a split.
   int64_t keys = key_bound;
   if (left < kWinUnlimited && right < kWinUnlimited)
@@ -957,12 +958,14 @@ WinAttnPlan win_attn_plan(int sm_count, int f32, bool tensor, bool uniform, int 
   pl.split_keys = tensor ? 1024 : rows_form ? 128 : 256;
   const int64_t most = keys / pl.split_keys;
   z = z < most ? z : most;
-  // Few rows over long contexts: pieces of 1024 keys, so that sequences of
-  // unlike lengths keep all SMs busy to the end (64 sequences of 2048 to 8192
-  // tokens, 32/8 heads of 128: 540 us whole, XXX us in pieces).
-  if (!tensor && pl.rows <= 32 && keys >= 2048 && z < (keys + 1023) / 1024) {
-    z = (keys + 1023) / 1024;
-    pl.split_keys = 1024;
+  // Few rows over long contexts: pieces of 1024 keys (f32: 384), so that
+  // sequences of unlike lengths keep all SMs busy to the end (64 sequences of
+  // 2048 to 8192 tokens, 32/8 heads of 128: 258 us, pieces of 512 keys 281; f32,
+  // 32 sequences of up to 4000 tokens, 8 heads of 128: 131 us, of 1024 160).
+  const int64_t piece = f32 ? 384 : 1024;
+  if (!tensor && pl.rows <= 32 && keys >= 2 * piece && z < (keys + piece - 1) / piece) {
+    z = (keys + piece - 1) / piece;
+    pl.split_keys = static_cast<int>(piece);
   }
   pl.splits = static_cast<int>(z < 1 ? 1 : z > 64 ? 64 : z);
   const int dp = dim <= 64 ? 64 : 128;
