@@ -394,41 +394,34 @@ __global__ void __launch_bounds__(kPartThreads, 4) beam_part_kernel(const __grid
   }
 }
 
-// A candidate's place among all: better score first, then the lower beam, then
-// the larger key (a beam's own logits order its candidates).
-struct Cand {
-  Key score;  // the f64 score as an integer of the same order (never 0)
-  Key key;    // 0: no candidate
-  int beam;
-  __device__ __forceinline__ bool before(const Cand &o) const {
-    if (score != o.score) return score > o.score;
-    if (beam != o.beam) return beam < o.beam;
-    return key > o.key;
-  }
-};
-__device__ __forceinline__ Key ordered64(double x) {
-  const Key u = static_cast<Key>(__double_as_longlong(x + 0.0));  // -0 as +0
+__device__ __forceinline__ Key ordered64(double x) {  // never 0; -0 as +0
+  const Key u = static_cast<Key>(__double_as_longlong(x + 0.0));
   return u >> 63 ? ~u : u | Key{1} << 63;
 }
 __device__ __forceinline__ double unordered64(Key u) { return __longlong_as_double(static_cast<long long>(u >> 63 ? u & ~(Key{1} << 63) : ~u)); }
 
-// One utterance: of the W x S sorted lists of W keys each, those whose head is
-// among the W best heads hold all W best candidates; they are ranked by
-// counting.
+// One utterance: W x S sorted lists of W keys (beam, part of its row).  One
+// warp takes the best of their heads W times; a lane holds the best head of
+// every 32nd list.  Better scores go first, then lower beams, then larger keys
+// (a beam's own logits order its candidates).
 constexpr int kJoinThreads = 256;
+constexpr int kJoinKeys = 2048;  // candidates in shared memory; more are read and scored as they come up
 __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_constant__ BeamParams p) {
   __shared__ double lse[kBeamMax], base_score[kBeamMax];
-  __shared__ uint8_t done[kBeamMax];
-  __shared__ Cand head[kBeamMax * kBeamSplitsMax];
-  __shared__ Cand pick[kBeamMax * kBeamMax];
-  __shared__ int n_pick, w_head;
+  __shared__ uint8_t done[kBeamMax], taken[kBeamMax * kBeamSplitsMax];
+  __shared__ ulonglong2 near_keys[kJoinKeys], chosen[kBeamMax];  // score, key
+  __shared__ int chosen_list[kBeamMax];
   pdl_wait();
   pdl_trigger();
   const int W = p.beams, S = p.splits, b = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const Key *keys = p.part_keys + static_cast<int64_t>(b) * W * S * W;  // [beam][split][W]
   const int lists = W * S, all = lists * W;
-  const Key first = tid < all ? keys[tid] : 0;  // on its way while the sums are joined
-  if (tid == 0) n_pick = 0, w_head = -1;
+  const Key *far_keys = p.part_keys + static_cast<int64_t>(b) * all;  // [beam][split][W]
+  const bool small = all <= kJoinKeys;
+  constexpr int kAhead = 2;  // on their way while the sums are joined
+  Key ahead[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) ahead[i] = small && tid + i * kJoinThreads < all ? far_keys[tid + i * kJoinThreads] : 0;
+  for (int i = tid; i < lists; i += kJoinThreads) taken[i] = 0;
   // log sum exp of each beam's row, over its parts (a lane each)
   for (int k = warp; k < W; k += kJoinThreads / 32) {
     const int row = b * W + k;
@@ -453,87 +446,70 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
     }
   }
   __syncthreads();
-  auto candidate = [&](int k, Key key) {
-    Cand c;
-    c.beam = k;
-    c.key = key;
-    if (done[k]) {
-      c.score = ordered64(base_score[k]);
-    } else {
-      const float x = unordered(static_cast<uint32_t>(key >> 32));
-      // every logit -inf: there is no sum, and the candidates count as -inf
-      const double s = x > -INFINITY ? base_score[k] + (static_cast<double>(x) - lse[k]) : -INFINITY;
-      c.score = ordered64(isnan(s) ? -INFINITY : s);
+  // Entry r of list l, and its score.  A finished beam's only candidate stands
+  // first in its first list; its row was not read.
+  auto entry = [&](int l, int r, Key y) {
+    const int k = l / S;
+    if (done[k]) y = r == 0 && l == k * S ? static_cast<Key>(~static_cast<uint32_t>(p.eos)) | Key{1} << 63 : 0;
+    if (y == 0) return make_ulonglong2(0, 0);
+    const float x = unordered(static_cast<uint32_t>(y >> 32));
+    // every logit -inf: there is no sum, and the candidates count as -inf
+    const double s = done[k] ? base_score[k] : x > -INFINITY ? base_score[k] + (static_cast<double>(x) - lse[k]) : -INFINITY;
+    return make_ulonglong2(ordered64(isnan(s) ? -INFINITY : s), y);
+  };
+  if (small) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int e = tid + i * kJoinThreads;
+      if (e < all) near_keys[e] = entry(e / W, e % W, ahead[i]);
     }
-    return c;
+    for (int e = tid + kAhead * kJoinThreads; e < all; e += kJoinThreads) near_keys[e] = entry(e / W, e % W, far_keys[e]);
+  }
+  __syncthreads();
+  if (warp) return;
+  // The best head of the lane's lists: score (0: none), key, list.
+  Key score = 0, key = 0;
+  int list = 0;
+  auto look = [&]() {
+    score = 0;
+    for (int l = lane; l < lists; l += 32) {
+      const int r = taken[l];
+      if (r == W) continue;
+      const ulonglong2 y = small ? near_keys[l * W + r] : entry(l, r, far_keys[l * W + r]);
+      if (y.x > score || (y.x && y.x == score && l / S == list / S && y.y > key)) score = y.x, key = y.y, list = l;
+    }
   };
-  // Entry i of the lists: a finished beam's only candidate stands first in its
-  // first list; the parts of its row were not written.
-  auto entry = [&](int i, Key key) -> Key {
-    const int k = i / (S * W);
-    return done[k] ? (i % (S * W) == 0 ? static_cast<Key>(~static_cast<uint32_t>(p.eos)) | Key{1} << 63 : 0) : key;
-  };
-  auto put = [&](const Cand &c, int above) {
-    const int out = b * W + above;
-    const int t = done[c.beam] ? p.eos : static_cast<int>(~static_cast<uint32_t>(c.key));
-    p.out_scores[out] = static_cast<float>(unordered64(c.score));
-    p.out_parents[out] = b * W + c.beam;
+  look();
+  for (int r = 0; r < W; ++r) {
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(score >> 32));
+    bool mine = score && static_cast<uint32_t>(score >> 32) == hi;
+    const uint32_t lo = __reduce_max_sync(0xffffffffu, mine ? static_cast<uint32_t>(score) : 0u);
+    mine = mine && static_cast<uint32_t>(score) == lo;
+    unsigned who = __ballot_sync(0xffffffffu, mine);
+    if (who & (who - 1)) {  // equal scores
+      const uint32_t beam = __reduce_min_sync(0xffffffffu, mine ? static_cast<uint32_t>(list / S) : 64u);
+      mine = mine && static_cast<uint32_t>(list / S) == beam;
+      const uint32_t value = __reduce_max_sync(0xffffffffu, mine ? static_cast<uint32_t>(key >> 32) : 0u);
+      mine = mine && static_cast<uint32_t>(key >> 32) == value;
+      const uint32_t token = __reduce_max_sync(0xffffffffu, mine ? static_cast<uint32_t>(key) : 0u);
+      mine = mine && static_cast<uint32_t>(key) == token;
+      who = __ballot_sync(0xffffffffu, mine);
+    }
+    if (lane == __ffs(who) - 1) {
+      chosen[r] = make_ulonglong2(score, key);
+      chosen_list[r] = list;
+      ++taken[list];
+      look();
+    }
+  }
+  __syncwarp();
+  if (lane < W) {
+    const int out = b * W + lane, k = chosen_list[lane] / S;
+    const int t = done[k] ? p.eos : static_cast<int>(~static_cast<uint32_t>(chosen[lane].y));
+    p.out_scores[out] = static_cast<float>(unordered64(chosen[lane].x));
+    p.out_parents[out] = b * W + k;
     p.out_tokens[out] = t;
-    if (p.out_finished) p.out_finished[out] = done[c.beam] || t == p.eos;
-  };
-  if (all <= kJoinThreads) {  // few: each thread ranks its own among all
-    // score (0: none), then 31 - beam and the logit, then the inverted token
-    ulonglong2 *major = reinterpret_cast<ulonglong2 *>(pick);
-    uint32_t *minor = reinterpret_cast<uint32_t *>(head);
-    Cand mine{};
-    if (tid < all) {
-      const Key key = entry(tid, first);
-      if (key) mine = candidate(tid / (S * W), key);
-      major[tid] = make_ulonglong2(mine.score, static_cast<Key>(31 - mine.beam) << 32 | mine.key >> 32);
-      minor[tid] = static_cast<uint32_t>(mine.key);
-    }
-    __syncthreads();
-    if (mine.key) {
-      const Key m = static_cast<Key>(31 - mine.beam) << 32 | mine.key >> 32;
-      const uint32_t t = static_cast<uint32_t>(mine.key);
-      int above = 0;
-#pragma unroll 4
-      for (int z = 0; z < all; ++z) {
-        const ulonglong2 y = major[z];
-        above += (y.x > mine.score) | ((y.x == mine.score) & ((y.y > m) | ((y.y == m) & (minor[z] > t))));
-      }
-      if (above < W) put(mine, above);
-    }
-    return;
-  }
-  for (int i = tid; i < lists; i += kJoinThreads) head[i] = candidate(i / S, entry(i * W, keys[static_cast<int64_t>(i) * W]));
-  __syncthreads();
-  // The W-th best head; fewer heads than W: all lists.
-  for (int i = tid; i < lists; i += kJoinThreads) {
-    if (head[i].key == 0) continue;
-    int above = 0;
-    for (int z = 0; z < lists; ++z) above += head[z].key != 0 && head[z].before(head[i]);
-    if (above == W - 1) w_head = i;
-  }
-  __syncthreads();
-  const int last = w_head;
-  const Cand floor_c = last >= 0 ? head[last] : Cand{};
-  for (int i = tid; i < all; i += kJoinThreads) {
-    const int l = i / W;
-    if (head[l].key == 0 || (last >= 0 && floor_c.before(head[l]))) continue;
-    const Key key = entry(i, keys[i]);
-    if (key == 0) continue;
-    const Cand c = candidate(l / S, key);
-    if (last >= 0 && floor_c.before(c)) continue;
-    pick[atomicAdd(&n_pick, 1)] = c;
-  }
-  __syncthreads();
-  const int n = n_pick;
-  for (int i = tid; i < n; i += kJoinThreads) {
-    const Cand c = pick[i];
-    int above = 0;
-    for (int z = 0; z < n; ++z) above += pick[z].before(c);
-    if (above < W) put(c, above);
+    if (p.out_finished) p.out_finished[out] = done[k] || t == p.eos;
   }
 }
 
