@@ -232,34 +232,50 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (warp >= kWarpK) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
   if (warp == kWarpK || warp == kWarpV) {
-    if (lane == 0 && nt > 0) {
+    if ((PAGED || lane == 0) && nt > 0) {
       // ------------------------------------------------------------- loads
+      // Plain rows: one lane, a box a tile.  Pages: a lane for each box of a
+      // tile (at most 16), whose page is looked up a tile ahead.
       const bool is_v = warp == kWarpV;
       const CUtensorMap *map = is_v ? &tm_v : &tm_k;
       const int full0 = is_v ? L::kVFull : L::kKFull, empty0 = is_v ? L::kVEmpty : L::kKEmpty;
       const uint32_t slot0 = is_v ? L::kOffV : L::kOffK;
-      prefetch_tmap(map);
       bool q_issued = false;
-      if (!is_v) {
-        prefetch_tmap(&tm_q);
-        const int toks = 128 / G;
-        mbar_arrive_expect_tx(bar(L::kQFull), 2 * (DP / 64) * static_cast<uint32_t>(toks * G * 128));
+      if (lane == 0) {
+        prefetch_tmap(map);
+        if (!is_v) {
+          prefetch_tmap(&tm_q);
+          const int toks = 128 / G;
+          mbar_arrive_expect_tx(bar(L::kQFull), 2 * (DP / 64) * static_cast<uint32_t>(toks * G * 128));
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
+          for (int x = 0; x < 2; ++x)
 #pragma unroll
-          for (int c = 0; c < DP / 64; ++c)
-            tma_load_3d(sbase + L::kOffQ + x * L::kTile + c * L::kBox, &tm_q, bar(L::kQFull), 64 * c, h * G,
-                        sq.q0 + (row0 + x * rows) / G);
-        q_issued = true;
+            for (int c = 0; c < DP / 64; ++c)
+              tma_load_3d(sbase + L::kOffQ + x * L::kTile + c * L::kBox, &tm_q, bar(L::kQFull), 64 * c, h * G,
+                          sq.q0 + (row0 + x * rows) / G);
+          q_issued = true;
+        }
       }
+      const int box = PAGED ? min(kKT, 1 << p.page_shift) : kKT;  // rows of a box
+      const int *table = PAGED ? p.table + static_cast<int64_t>(b) * p.table_ld : nullptr;
+      auto page_of = [&](int t) {  // of this lane's box; -1: none, or no key of the list
+        const int key = t < nt ? tl.base(t) + lane * box : 0;
+        if (t >= nt || lane * box >= kKT || key > ks.hi || (tl.in_sinks(t) && key >= ks.s_end)) return -1;
+        const int pg = __ldg(table + (key >> p.page_shift));
+        return pg < p.pages ? pg : -1;
+      };
+      int pg = PAGED ? page_of(0) : 0;
       int n = 0;
       for (int t = 0; t < nt; ++t) {
         const int s = t % S, use = t / S;
-        if (use > 0 && !mbar_wait(bar(empty0 + s), (use - 1) & 1, lim, abort_flag)) {
-          if (!*abort_flag) report(p.ctl, abort_flag, kDevTimeoutProducer);
+        const int pg_next = PAGED ? page_of(t + 1) : 0;
+        bool ok = use == 0 || mbar_wait(bar(empty0 + s), (use - 1) & 1, lim, abort_flag);
+        if (PAGED) ok = __all_sync(0xffffffffu, ok);
+        if (!ok) {
+          if (lane == 0 && !*abort_flag) report(p.ctl, abort_flag, kDevTimeoutProducer);
           break;
         }
-        if (*abort_flag) break;
+        if (PAGED ? __any_sync(0xffffffffu, *abort_flag) : *abort_flag) break;
         const uint32_t full = bar(full0 + s), dst = sbase + slot0 + s * L::kTile;
         const int base = tl.base(t);
         if constexpr (!PAGED) {
@@ -267,60 +283,48 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
           for (int c = 0; c < DP / 64; ++c) tma_load_3d(dst + c * L::kBox, map, full, 64 * c, h, sq.k0 + base);
         } else {
-          const int box = min(kKT, 1 << p.page_shift);  // rows of a box
-          const int *table = p.table + static_cast<int64_t>(b) * p.table_ld;
           const int boxes = kKT / box;
-          uint32_t have = 0;  // boxes whose page exists and holds a key of the window
-          int pg[16];
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            pg[j] = -1;
-            const int key = base + j * box;
-            if (j < boxes && key <= ks.hi && (!tl.in_sinks(t) || key < ks.s_end)) pg[j] = __ldg(table + (key >> p.page_shift));
-            if (pg[j] >= 0 && pg[j] < p.pages) have |= 1u << j;
-          }
+          const unsigned have = __ballot_sync(0xffffffffu, pg >= 0);  // boxes whose page exists
           if (!is_v) {
             // the softmax's view of missing pages (keys past the end are masked anyway)
-            uint32_t m[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (j < boxes && !(have >> j & 1)) {
-#pragma unroll
-                for (int x = 0; x < 4; ++x) m[x] |= bit_range(j * box - 32 * x, (j + 1) * box - 1 - 32 * x);
-              }
-#pragma unroll
-            for (int x = 0; x < 4; ++x) holes[(t & 7) * 4 + x] = m[x];
-          } else {
-            // missing pages' values: zeros (their weights are zero)
-            bool any = false;
-            for (int j = 0; j < boxes; ++j)
-              if (!(have >> j & 1)) {
-                any = true;
-                for (int c = 0; c < DP / 64; ++c)
-                  for (int x = 0; x < box * 8; ++x)
-                    asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(dst + c * L::kBox + j * box * 128 + x * 16), "r"(0) : "memory");
-              }
-            if (any) fence_proxy_async_smem();
-          }
-          const uint32_t box_bytes = static_cast<uint32_t>(box) * 128u;
-          mbar_arrive_expect_tx(full, __popc(have) * box_bytes * (DP / 64));
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (have >> j & 1) {
-              const int row = ((pg[j] * p.kv_heads + h) << p.page_shift) + ((base + j * box) & ((1 << p.page_shift) - 1));
-#pragma unroll
-              for (int c = 0; c < DP / 64; ++c) tma_load_2d(dst + c * L::kBox + j * box_bytes, map, full, 64 * c, row);
+            if (lane < 4) {
+              uint32_t m = 0;
+              for (int j = 0; j < boxes; ++j)
+                if (!(have >> j & 1)) m |= bit_range(j * box - 32 * lane, (j + 1) * box - 1 - 32 * lane);
+              holes[(t & 7) * 4 + lane] = m;
             }
+          } else if (have != (boxes == 32 ? 0xffffffffu : (1u << boxes) - 1u)) {
+            // missing pages' values: zeros (their weights are zero)
+            for (int j = 0; j < boxes; ++j)
+              if (!(have >> j & 1))
+                for (int c = 0; c < DP / 64; ++c)
+                  for (int x = lane; x < box * 8; x += 32)
+                    asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(dst + c * L::kBox + j * box * 128 + x * 16), "r"(0) : "memory");
+            fence_proxy_async_smem();
+          }
+          __syncwarp();
+          const uint32_t box_bytes = static_cast<uint32_t>(box) * 128u;
+          if (lane == 0) mbar_arrive_expect_tx(full, __popc(have) * box_bytes * (DP / 64));
+          __syncwarp();
+          if (pg >= 0) {
+            const int row = ((pg * p.kv_heads + h) << p.page_shift) + ((base + lane * box) & ((1 << p.page_shift) - 1));
+#pragma unroll
+            for (int c = 0; c < DP / 64; ++c) tma_load_2d(dst + c * L::kBox + lane * box_bytes, map, full, 64 * c, row);
+          }
+          pg = pg_next;
         }
         ++n;
       }
-      // Every copy this lane issued into shared memory has landed.
+      // Every copy issued into shared memory has landed.
       volatile int no_abort = 0;
-      for (int s = 0; s < S; ++s) {
-        const int uses = n > s ? (n - 1 - s) / S + 1 : 0;
-        if (uses > 0 && !mbar_wait(bar(full0 + s), (uses - 1) & 1, lim, &no_abort)) atomicOr(p.ctl.status, kDevTimeoutDrain);
+      if (lane == 0) {
+        for (int s = 0; s < S; ++s) {
+          const int uses = n > s ? (n - 1 - s) / S + 1 : 0;
+          if (uses > 0 && !mbar_wait(bar(full0 + s), (uses - 1) & 1, lim, &no_abort)) atomicOr(p.ctl.status, kDevTimeoutDrain);
+        }
+        if (q_issued && !mbar_wait(bar(L::kQFull), 0, lim, &no_abort)) atomicOr(p.ctl.status, kDevTimeoutDrain);
       }
-      if (q_issued && !mbar_wait(bar(L::kQFull), 0, lim, &no_abort)) atomicOr(p.ctl.status, kDevTimeoutDrain);
+      __syncwarp(PAGED ? 0xffffffffu : 1u);
     }
   } else if (warp == kWarpMma && nt > 0) {
     // ----------------------------------------------------------------- MMA
