@@ -155,6 +155,7 @@ int run_attention(const char *who, nq::WinAttnParams &p, int dtype, int64_t key_
                                                p.kv_heads, p.group, p.dim, p.left, p.right, p.sinks);
   p.splits = workspace ? pl.splits : 1;
   p.split_keys = pl.split_keys;
+  p.pair = pl.pair;
   if (p.splits > 1) {
     if (static_cast<size_t>(workspace_bytes < 0 ? 0 : workspace_bytes) < pl.workspace)
       return bad(NQ_ERR_SHAPE, "%s: a workspace of %lld bytes, %zu are needed", who, (long long)workspace_bytes, pl.workspace);

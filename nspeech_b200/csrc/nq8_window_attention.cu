@@ -929,11 +929,15 @@ bool win_attn_tc_fits(int f32, int seqs, int q_rows, int group) {
 
 WinAttnPlan win_attn_plan(int sm_count, int f32, bool tensor, bool uniform, int seqs, int q_rows, int64_t key_bound, int kv_heads,
                           int group, int dim, int left, int right, int sinks) {
-  WinAttnPlan pl;
+  WinAttnPlan pl = {};
   const int64_t rows = static_cast<int64_t>(q_rows) * group;
   const int64_t mean = (rows + seqs - 1) / seqs;  // rows of a sequence and kv head
   if (tensor) {
-    pl.rows = 2 * (128 / group * group);
+    // Two tiles keep the tensor cores busy during one's exponentials; where even
+    // single ones leave SMs idle, they end sooner.
+    const int64_t one = 128 / group * group, items = (rows + one - 1) / one;
+    pl.pair = (items > seqs ? items : seqs) * kv_heads <= sm_count ? 1 : 2;
+    pl.rows = pl.pair * static_cast<int>(one);
   } else if (f32) {
     pl.rows = mean <= 1 ? 1 : mean <= 2 ? 2 : mean <= 4 ? 4 : mean <= 16 ? 16 : mean <= 32 ? 32 : 64;
   } else {

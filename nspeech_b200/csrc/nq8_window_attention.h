@@ -41,6 +41,7 @@ struct WinAttnParams {
   // Split of a row tile's keys over gridDim.z CTAs: unnormalised outputs,
   // row maxima (log2 units) and sums, joined by a second kernel.
   int splits, split_keys;  // CTAs of a tile's keys, and the keys that each takes at least
+  int pair;                // as in WinAttnPlan
   float *part_o;           // [splits][q_rows * query heads][dim padded to 64 or 128]
   float2 *part_ml;         // [splits][q_rows * query heads]
   DevCtl ctl;
@@ -50,6 +51,7 @@ struct WinAttnParams {
 struct WinAttnPlan {
   int rows;    // query rows (token, head of a group) of a CTA
   int splits, split_keys;
+  int pair;    // tensor-core form: 128-row tiles of a CTA, 1 or 2
   int tiles;   // CTAs along x: an upper bound of the row tiles of all sequences
   size_t workspace;
 };

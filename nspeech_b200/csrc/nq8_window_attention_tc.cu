@@ -1,7 +1,8 @@
 // nq8_window_attention_tc.cu -- window attention of many bf16 query rows on
 // the 5th-generation tensor cores (tcgen05 + TMEM).
 //
-// Work item: two tiles (A, B) of 128 query rows of one kv head; a row is a
+// Work item: two tiles (A, B) of 128 query rows of one kv head (one where that
+// many items leave SMs idle); a row is a
 // (token, head of the group) pair, token-major, which is the order in which
 // one TMA box {64 columns, group heads, tokens} arrives.  The item's keys (the
 // sinks, then the window of all its rows) are walked in tiles of 128; a tile
@@ -39,6 +40,8 @@
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "nq8_window_attention.cuh"
 
@@ -208,10 +211,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   Seq sq = {};
   Keys ks = {};
   Tiles tl = {};
-  if (find_tile(p, gridDim.x - 1 - blockIdx.x, 2 * rows, b, row0)) {
+  if (find_tile(p, gridDim.x - 1 - blockIdx.x, p.pair * rows, b, row0)) {
     sq = seq_of(p, b);
     n_rows = sq.nq * G;
-    ks = keys_of<kKT>(p, sq, row0 / G, (min(row0 + 2 * rows, n_rows) - 1) / G);
+    ks = keys_of<kKT>(p, sq, row0 / G, (min(row0 + p.pair * rows, n_rows) - 1) / G);
     tl.sink_tiles = ks.sink_tiles;
     tl.lo = ks.lo;
     if (PAGED) tl.lo &= ~(min(kKT, 1 << p.page_shift) - 1);  // the window's tiles begin with a box
@@ -246,9 +249,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (!is_v) {
           prefetch_tmap(&tm_q);
           const int toks = 128 / G;
-          mbar_arrive_expect_tx(bar(L::kQFull), 2 * (DP / 64) * static_cast<uint32_t>(toks * G * 128));
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
+          mbar_arrive_expect_tx(bar(L::kQFull), p.pair * (DP / 64) * static_cast<uint32_t>(toks * G * 128));
+          for (int x = 0; x < p.pair; ++x)
 #pragma unroll
             for (int c = 0; c < DP / 64; ++c)
               tma_load_3d(sbase + L::kOffQ + x * L::kTile + c * L::kBox, &tm_q, bar(L::kQFull), 64 * c, h * G,
@@ -344,7 +346,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     int final_t[2];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      const Part y = part_of(p, tl, sq, G, row0 + x * rows, rows, n_rows);
+      const Part y = part_of(p, tl, sq, G, row0 + x * rows, rows, x < p.pair ? n_rows : 0);
       part[x] = Part{uniform(y.head), uniform(y.first), uniform(y.last)};
       final_t[x] = max(part[x].head - 1, part[x].last);
     }
@@ -441,11 +443,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int x = warp >> 2;
     const int r = 32 * (warp & 3) + lane;        // TMEM lane, row of the tile
     const int row = row0 + x * rows + r;         // row of the sequence
-    const bool there = r < rows && row < n_rows;
+    const bool there = r < rows && row < n_rows && x < p.pair;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
     const uint32_t ts = lanes + x * 128, to = lanes + 256 + x * DP;
     const int pos = there ? sq.nk - sq.nq + row / G : 0;
-    const Part part = part_of(p, tl, sq, G, row0 + x * rows, rows, n_rows);
+    const Part part = part_of(p, tl, sq, G, row0 + x * rows, rows, x < p.pair ? n_rows : 0);
     // keys that every row of the tile sees: [all_lo, all_hi], sinks apart
     const int pos_lo = sq.nk - sq.nq + (row0 + x * rows) / G, pos_hi = sq.nk - sq.nq + (min(row0 + (x + 1) * rows, n_rows) - 1) / G;
     const int all_hi = p.right >= kWinUnlimited ? sq.nk - 1 : min(sq.nk - 1, pos_lo + p.right);
@@ -479,11 +481,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int c = 0; c < 4; ++c) hole[c] = *reinterpret_cast<volatile uint32_t *>(holes + (t & 7) * 4 + c);
       }
       const bool inside = base + kKT - 1 <= all_hi && (base >= all_lo || base + kKT <= p.sinks) && !(hole[0] | hole[1] | hole[2] | hole[3]);
+      unsigned live = 15;  // quarters of the tile that a row of the warp sees a key of
       if (!inside) {
+        live = 0;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           const int o = base + 32 * c;
           const uint32_t see = (bit_range(jmin_row - o, jmax_row - o) | bit_range(0, min(p.sinks - 1, jmax_row) - o)) & ~hole[c];
+          live |= __any_sync(0xffffffffu, see != 0u) ? 1u << c : 0u;
 #pragma unroll
           for (int e = 0; e < 32; ++e) sr[32 * c + e] = see >> e & 1u ? sr[32 * c + e] : __float_as_uint(-INFINITY);
         }
@@ -515,24 +520,39 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const float ref = m_use == -INFINITY ? 0.f : m_use;
       const uint64_t scale2 = f2(p.sl2, p.sl2), nref2 = f2(-ref, -ref);
       uint64_t sum2 = f2(0.f, 0.f);
-      // P in two halves, so that PV begins with the first
+      // P in two halves, so that PV begins with the first.  In a masked tile the
+      // quarters that nobody sees are zeros.
+      auto weights = [&](auto masked) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t pk[32];
+        for (int c = 0; c < 2; ++c) {
+          uint32_t pk[32];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          float pa, pb;
-          unpack2(fma2(f2(__uint_as_float(sr[64 * c + 2 * e]), __uint_as_float(sr[64 * c + 2 * e + 1])), scale2, nref2), pa, pb);
-          pa = ex2(pa);
-          pb = ex2(pb);
-          sum2 = add2(sum2, f2(pa, pb));
-          pk[e] = pack_bf16x2(pa, pb);
+          for (int q = 0; q < 2; ++q) {
+            if (!decltype(masked)::value || (live >> (2 * c + q) & 1u)) {
+#pragma unroll
+              for (int e = 16 * q; e < 16 * q + 16; ++e) {
+                float pa, pb;
+                unpack2(fma2(f2(__uint_as_float(sr[64 * c + 2 * e]), __uint_as_float(sr[64 * c + 2 * e + 1])), scale2, nref2), pa, pb);
+                pa = ex2(pa);
+                pb = ex2(pb);
+                sum2 = add2(sum2, f2(pa, pb));
+                pk[e] = pack_bf16x2(pa, pb);
+              }
+            } else {
+#pragma unroll
+              for (int e = 16 * q; e < 16 * q + 16; ++e) pk[e] = 0u;
+            }
+          }
+          tmem_st32(ts + 32 * c, pk);
+          tmem_st_wait();
+          tc_fence_before();
+          mbar_arrive(bar(L::kPReady + 2 * c + x));
         }
-        tmem_st32(ts + 32 * c, pk);
-        tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(bar(L::kPReady + 2 * c + x));
-      }
+      };
+      if (inside)
+        weights(std::false_type());
+      else
+        weights(std::true_type());
       float la, lb;
       unpack2(sum2, la, lb);
       l += la + lb;
