@@ -84,6 +84,23 @@ __device__ __forceinline__ bool sees(const WinAttnParams &p, const KeyList &k, i
   return u < k.n && (p.right >= kWinUnlimited || j <= at + p.right) && (p.left >= kWinUnlimited || j >= at - p.left || j < p.sinks);
 }
 
+// The same for the list's entries [u, u + 32) as bits.
+__device__ __forceinline__ uint32_t bits_between(int lo, int hi) {  // bits lo..hi, any integers
+  lo = max(lo, 0);
+  hi = min(hi, 31);
+  return hi < lo ? 0u : (0xffffffffu >> (31 - hi)) & (0xffffffffu << lo);
+}
+__device__ __forceinline__ uint32_t row_bits(const WinAttnParams &p, const KeyList &k, int u, int at) {
+  const int shift = k.s_end - k.lo - u;  // of a window key's bit
+  const int last = k.n - 1 - u;
+  const int hi = p.right >= kWinUnlimited ? last : min(last, at + p.right + shift);
+  const int lo = max(k.s_end - u, p.left >= kWinUnlimited ? k.s_end - u : at - p.left + shift);
+  // first keys: entries of their own, or the window's first where it begins at key 0
+  const int first = k.s_end ? k.s_end : k.lo ? 0 : p.sinks;
+  const int first_hi = min(p.right >= kWinUnlimited ? first - 1 : min(first - 1, at + p.right), k.n - 1) - u;
+  return bits_between(lo, hi) | bits_between(-u, first_hi);
+}
+
 // Element offset of the row of entry u for kv head h; -1 past the list's end
 // and where the key's page is missing (the row reads as zeros).
 template <bool PAGED>
@@ -297,19 +314,33 @@ __global__ void __launch_bounds__(kThreads) win_attn_mma(const __grid_constant__
     }
     const bool inside = all_see<KT>(p, s, k, base, pos_lo, pos_hi) && !(hole[0] | hole[1]);
     float top[2] = {-INFINITY, -INFINITY};
+    if (inside) {
 #pragma unroll
-    for (int n = 0; n < KW / 8; ++n)
+      for (int n = 0; n < KW / 8; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float x = sc[n][e] * p.sl2;
-        if (!inside) {
-          const int jl = wk * KW + 8 * n + 2 * (lane & 3) + (e & 1);
-          const bool see = sees(p, k, base + jl, pos[e >> 1]) && !((hole[jl >> 5] >> (jl & 31)) & 1u);
-          x = see ? x : -INFINITY;
+        for (int e = 0; e < 4; ++e) {
+          sc[n][e] *= p.sl2;
+          top[e >> 1] = fmaxf(top[e >> 1], sc[n][e]);
         }
-        sc[n][e] = x;
-        top[e >> 1] = fmaxf(top[e >> 1], x);
-      }
+    } else {
+      constexpr int kWords = (KW + 31) / 32;  // of this warp's keys
+      uint32_t see[2][kWords];
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int w = 0; w < kWords; ++w) {
+          const int u = wk * KW + 32 * w;
+          see[x][w] = row_bits(p, k, base + u, pos[x]) & ~(hole[u >> 5] >> (u & 31));
+        }
+#pragma unroll
+      for (int n = 0; n < KW / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool on = see[e >> 1][8 * n / 32] >> (8 * n % 32 + 2 * (lane & 3) + (e & 1)) & 1u;
+          sc[n][e] = on ? sc[n][e] * p.sl2 : -INFINITY;
+          top[e >> 1] = fmaxf(top[e >> 1], sc[n][e]);
+        }
+    }
     float ref[2];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
@@ -452,9 +483,13 @@ __global__ void __launch_bounds__(kThreads) win_attn_mma(const __grid_constant__
 // x - xh (exact, taken at 11 bits): 2^-20 of |x y| at most is lost, 2^-22 on
 // the mean.  The tensor cores add with truncation, so their sums are kept
 // short: the large and the small products apart, and an output's sum over the
-// 32 keys of a tile is added to the running one in f32.  (FMA form of the same
-// tile: bound by shared memory, 128-bit loads of operands that only 16
-// products each use; 32 segments of up to 1501 tokens 544 us, this 1XX us.)
+// 32 keys of a tile is added to the running one in f32.  Bound by issue slots:
+// the parts' splitting (three instructions an element, in every warp) and the
+// warp-level MMAs (0.27 PFLOP/s of tf32, a third of it for f32 products).  32
+// segments of up to 1501 tokens, 10 heads of 64, window 64 + 16: 307 us; the
+// same tiles by FMA 544 us, bound by shared memory (128-bit loads of operands
+// that 16 products each use); two row tiles a warp, which share the parts of
+// keys and values but leave two CTAs an SM, 400 us.
 template <int DP>
 struct F32Smem {
   static constexpr int kKT = 32, kP = DP + 4;  // pitch: rows 16 bytes apart in the banks
@@ -612,22 +647,21 @@ __global__ void __launch_bounds__(kThreads) win_attn_tf32(const __grid_constant_
         }
       }
     }
-    bool inside = all_see<KT>(p, s, k, base, pos_lo, pos_hi);
-    if constexpr (PAGED) inside = __all_sync(0xffffffffu, inside && row_off[(t % 3) * KT + lane] >= 0);
+    const bool inside = all_see<KT>(p, s, k, base, pos_lo, pos_hi);
+    uint32_t see[2] = {0xffffffffu, 0xffffffffu}, gone = 0;  // gone: entries whose page is missing
+    if constexpr (PAGED) gone = __ballot_sync(0xffffffffu, row_off[(t % 3) * KT + lane] < 0);
+    if (!inside || gone) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) see[x] = row_bits(p, k, base, pos[x]) & ~gone;
+    }
     float top[2] = {m[0], m[1]};
 #pragma unroll
     for (int n = 0; n < N; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float x = (hi[n][e] + lo[n][e]) * p.sl2;
-        if (!inside) {
-          const int jl = wk * KW + 8 * n + 2 * qc + (e & 1);
-          bool see = sees(p, k, base + jl, pos[e >> 1]);
-          if constexpr (PAGED) see = see && row_off[(t % 3) * KT + jl] >= 0;
-          x = see ? x : -INFINITY;
-        }
-        hi[n][e] = x;
-        top[e >> 1] = fmaxf(top[e >> 1], x);
+        const float x = (hi[n][e] + lo[n][e]) * p.sl2;
+        hi[n][e] = see[e >> 1] >> (wk * KW + 8 * n + 2 * qc + (e & 1)) & 1u ? x : -INFINITY;
+        top[e >> 1] = fmaxf(top[e >> 1], hi[n][e]);
       }
     float ref[2], f[2];
 #pragma unroll
