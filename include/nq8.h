@@ -451,8 +451,9 @@ int nq_beam_select(const void *logits, int dtype, int64_t ld, int items, int bea
 
 /* dst[i][r] = src[i][parents[r]] for up to 16 states of `rows` rows (up to
  * 12288): row_bytes[i] bytes, src_stride[i] and dst_stride[i] bytes apart.  A
- * parent out of range leaves its row.  dst[i] may be src[i] (with the same
- * stride), and otherwise overlaps no state.  One launch. */
+ * parent out of range stands for the row itself.  dst[i] may be src[i] (with
+ * the same stride); an output that otherwise overlaps a state or another
+ * output is refused.  One launch. */
 int nq_beam_reorder(const void *const *src, void *const *dst, const int64_t *row_bytes, const int64_t *src_stride,
                     const int64_t *dst_stride, int count, int rows, const int32_t *parents, void *stream);
 

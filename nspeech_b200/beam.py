@@ -35,7 +35,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: Optional[t
 def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, out: Optional[Sequence[torch.Tensor]] = None,
                  stream: Optional[torch.cuda.Stream] = None) -> List[torch.Tensor]:
     """out[i][r] = states[i][parents[r]] for every state (any dtype, [rows, ...] with contiguous rows), in one launch for
-    up to 16 states.  parents: int32, `rows` of them in any shape (``beam_select``'s).  out[i] may be states[i]."""
+    up to 16 states.  parents: int32, `rows` of them in any shape (``beam_select``'s); one out of range stands for the row
+    itself.  out[i] may be states[i], but overlaps no other state or output."""
     if stream is not None:
         with _on(stream, parents):
             return beam_reorder(states, parents, out)

@@ -10,6 +10,7 @@
 #include "../../include/nq8.h"
 #include "nq8_cache.h"
 #include "nq8_host.h"
+#include "nq8_overlap.h"
 #include "nq8_window_attention.h"
 
 namespace nq {
@@ -436,9 +437,7 @@ int nq_beam_reorder(const void *const *src, void *const *dst, const int64_t *row
   const char *who = "nq_beam_reorder";
   if (count < 0 || count > nq::kReorderMax) return bad(NQ_ERR_SHAPE, "%s: %d states, at most %d a call", who, count, nq::kReorderMax);
   if (rows < 0 || rows > nq::kReorderMaxRows) return bad(NQ_ERR_SHAPE, "%s: %d rows, at most %d", who, rows, nq::kReorderMaxRows);
-  int sm = 0;
-  const int rc = nq::device_info(&sm, nullptr);
-  if (rc || count == 0 || rows == 0) return rc;
+  if (count == 0 || rows == 0) return NQ_OK;
   if (!src || !dst || !row_bytes || !src_stride || !dst_stride || !parents) return bad(NQ_ERR_ARG, "%s: null argument", who);
   nq::ReorderParams p = {};
   int64_t strips = 0;
@@ -455,6 +454,11 @@ int nq_beam_reorder(const void *const *src, void *const *dst, const int64_t *row
     p.dst_ld[i] = dst_stride[i];
   }
   if (strips > (1LL << 30)) return bad(NQ_ERR_SHAPE, "%s: rows too long", who);
+  if (nq::reorder_overlaps(src, dst, row_bytes, src_stride, dst_stride, count, rows))
+    return bad(NQ_ERR_ARG, "%s: an output overlaps another state", who);
+  int sm = 0;
+  const int rc = nq::device_info(&sm, nullptr);
+  if (rc) return rc;
   p.count = count;
   p.rows = rows;
   p.parents = parents;

@@ -21,6 +21,7 @@
 #include <vector>
 
 #include "../../include/nq8.h"
+#include "nq8_overlap.h"
 
 namespace {
 
@@ -393,7 +394,10 @@ PyObject *beam_reorder(PyObject *const *a) {
     src_by.push_back(row_stride(t, rows, row));
     dst_by.push_back(row_stride(o, rows, row));
   }
-  constexpr size_t kMost = 16;  // states of one launch
+  constexpr size_t kMost = 16;  // states of one launch, which checks its own
+  if (src.size() > kMost &&
+      nq::reorder_overlaps(src.data(), dst.data(), bytes.data(), src_by.data(), dst_by.data(), static_cast<int>(src.size()), rows))
+    misfit("an output overlaps another state");
   for (size_t i = 0; i < src.size(); i += kMost)
     check(nq_beam_reorder(&src[i], &dst[i], &bytes[i], &src_by[i], &dst_by[i], static_cast<int>(std::min(kMost, src.size() - i)),
                           static_cast<int>(rows), static_cast<const int32_t *>(parents.data_ptr()), dev.stream()));

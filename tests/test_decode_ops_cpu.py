@@ -105,6 +105,25 @@ def test_beam_calls_refuse(lib):
     assert lib.nq_beam_reorder(one, one, size, size, size, 1, 12289, PTR, None) == L.NQ_ERR_SHAPE
 
 
+def test_beam_reorder_refuses_outputs_that_overlap(lib):
+    def reorder(src, dst, row=16, src_by=64, dst_by=64):
+        n = len(src)
+        ints = [(ctypes.c_int64 * n)(*([x] * n)) for x in (row, src_by, dst_by)]
+        return lib.nq_beam_reorder((ctypes.c_void_p * n)(*src), (ctypes.c_void_p * n)(*dst), *ints, n, 4, PTR, None)
+
+    for src, dst in (([PTR, PTR], [PTR, PTR]),                          # one state twice, in place
+                     ([PTR, PTR + 256], [PTR + 512, PTR + 512]),        # one output twice
+                     ([PTR, PTR + 256], [PTR + 256, PTR + 512]),        # an output that is another's state
+                     ([PTR], [PTR + 64]),                               # the state's second row on
+                     ([PTR, PTR + 16], [PTR + 512, PTR + 520])):        # rows that meet halfway
+        assert reorder(src, dst) == L.NQ_ERR_ARG, (src, dst)
+        assert "overlap" in L.last_error()
+    assert reorder([PTR], [PTR], dst_by=32) == L.NQ_ERR_ARG             # in place, other strides
+    if not torch.cuda.is_available():  # columns of one tensor, in place: the call gets as far as the device
+        columns = [PTR, PTR + 16, PTR + 48]
+        assert reorder(columns, columns) == L.NQ_ERR_NOT_INIT
+
+
 def test_python_refuses_host_tensors_and_misfits():
     from nspeech_b200.attention import window_attention
     from nspeech_b200.beam import beam_select

@@ -608,6 +608,26 @@ def test_beam_reorder(rows):
     assert torch.equal(beam_reorder([state], parents * 0 - 1)[0], state)  # out of range: the row stays
 
 
+def test_beam_reorder_of_columns_and_of_the_same_state_twice():
+    from nspeech_b200.beam import beam_reorder
+    from nspeech_b200.fast_matmul import MatMulError
+    from nspeech_b200.lib import NqError
+    parents = torch.tensor([2, 0, 0, 1], dtype=torch.int32, device="cuda")
+    whole = torch.arange(4 * 96, device="cuda").view(4, 96)
+    want = whole[parents.long()]
+    twice = beam_reorder([whole, whole], parents)  # read twice, written once each
+    assert torch.equal(twice[0], want) and torch.equal(twice[1], want)
+    columns = [whole[:, :32], whole[:, 32:40], whole[:, 40:]]
+    beam_reorder(columns, parents, out=columns)
+    assert torch.equal(whole, want)
+    with pytest.raises(NqError, match="overlap"):
+        beam_reorder([whole, whole], parents, out=[whole, whole])
+    many = [whole.clone() for _ in range(17)] + [whole]
+    with pytest.raises(MatMulError, match="overlap"):
+        beam_reorder(many, parents, out=many[:17] + [many[0]])
+    assert torch.equal(whole, want)
+
+
 # ------------------------------------------------------------------------------------------------ a decoder, end to end
 class Decoder:
     """One attention layer, an output projection and a lm_head on Q8_0-path weights (kept at bf16 precision, f32
