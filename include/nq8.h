@@ -379,7 +379,7 @@ typedef struct nq_cache {
   int32_t *state;   /* [nq_cache_state_ints(slots, pages)] status and scratch */
   int dtype;        /* NQ_F32 | NQ_BF16 */
   int layers, pages, page_tokens; /* page_tokens: a power of two, 8 to 1024; pages up to 2^20 */
-  int kv_heads, head_dim;         /* head_dim 1 to 128 */
+  int kv_heads, head_dim;         /* head_dim 1 to 128; page_tokens * kv_heads * head_dim up to 2^28 */
   int slots, max_pages;           /* max_pages * page_tokens up to 2^30 */
 } nq_cache;
 #define NQ_CACHE_OUT_OF_PAGES 0x1

@@ -24,6 +24,7 @@ struct CacheView {
 constexpr int kCacheOutOfPages = 1, kCacheSlotFull = 2, kCacheBadIndex = 4, kCacheSharedPage = 8;
 constexpr int kCacheMaxCall = 4096;       // slots of one call
 constexpr int kCacheMaxPages = 1 << 20;
+constexpr int kCacheMaxPageElems = 1 << 28;  // of a page in one layer: a copy's units are counted in 32 bits
 // state[0] status bits, [1] live pages after a compaction, [2] entries of the
 // copy list; then the copy list (page from, page to, rows) per slot, and three
 // lists of `pages` entries.

@@ -68,6 +68,8 @@ int check_cache(const char *who, const nq_cache *c) {
   if (c->pages < 1 || c->pages > nq::kCacheMaxPages || c->slots < 1 || c->slots > (1 << 24) || c->max_pages < 1 ||
       static_cast<int64_t>(c->max_pages) * c->page_tokens > (1 << 30))
     return bad(NQ_ERR_SHAPE, "%s: %d pages, %d slots of up to %d pages", who, c->pages, c->slots, c->max_pages);
+  if (static_cast<int64_t>(c->page_tokens) * c->kv_heads * c->head_dim > nq::kCacheMaxPageElems)
+    return bad(NQ_ERR_SHAPE, "%s: pages of %d tokens, %d kv heads of %d", who, c->page_tokens, c->kv_heads, c->head_dim);
   if (!aligned(c->k, 16) || !aligned(c->v, 16)) return bad(NQ_ERR_ALIGN, "%s: the pages must be 16-byte aligned", who);
   return NQ_OK;
 }

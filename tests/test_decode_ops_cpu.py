@@ -59,6 +59,7 @@ BAD_CACHES = [(dict(k=None), L.NQ_ERR_ARG), (dict(state=None), L.NQ_ERR_ARG), (d
               (dict(page_tokens=12), L.NQ_ERR_SHAPE), (dict(page_tokens=4), L.NQ_ERR_SHAPE), (dict(page_tokens=2048), L.NQ_ERR_SHAPE),
               (dict(layers=0), L.NQ_ERR_SHAPE), (dict(head_dim=130), L.NQ_ERR_SHAPE), (dict(pages=0), L.NQ_ERR_SHAPE),
               (dict(pages=(1 << 20) + 1), L.NQ_ERR_SHAPE), (dict(slots=0), L.NQ_ERR_SHAPE), (dict(max_pages=1 << 27), L.NQ_ERR_SHAPE),
+              (dict(page_tokens=1024, kv_heads=4096, head_dim=128, dtype=L.NQ_F32), L.NQ_ERR_SHAPE),
               (dict(v=PTR + 8), L.NQ_ERR_ALIGN)]
 
 
