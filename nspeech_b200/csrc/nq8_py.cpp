@@ -96,7 +96,13 @@ class Device {
     was = c10::cuda::current_device();
     if (was != index) c10::cuda::set_device(static_cast<c10::DeviceIndex>(index));
     if (index < 64 && !(g_ready >> index & 1)) {
-      check(nq_init(index));
+      // nq_init allocates: allowed while this thread captures another stream
+      cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+      cudaThreadExchangeStreamCaptureMode(&mode);
+      const int rc = nq_init(index);
+      cudaThreadExchangeStreamCaptureMode(&mode);
+      if (rc < 0 && was != index) c10::cuda::set_device(static_cast<c10::DeviceIndex>(was));  // no object, no destructor
+      check(rc);
       g_ready |= uint64_t{1} << index;
     }
   }

@@ -4,6 +4,10 @@ Tolerances come from the arithmetic.  A score is a sum of head_dim products in f
 sum of absolute products; exp2 adds 2^-21 at most; the softmax sums up to n terms in f32.  A relative change of e of
 every weight moves the output by at most 2 e sum p |v|.  bf16 rounds each weight (2^-8 of it) and the output (2^-8).
 """
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
@@ -735,6 +739,29 @@ def test_beam_search_over_the_cache_and_its_graph():
         assert torch.equal(g["scores"], trail[t][0]) and torch.equal(g["history"], trail[t][1])
     graph_cache.check()
     assert torch.equal(cache.table, graph_cache.table) and torch.equal(cache.refs, graph_cache.refs)
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    program = """
+import torch
+from nspeech_b200.attention import window_attention
+from nspeech_b200.beam import beam_select
+torch.manual_seed(0)
+q, x = torch.randn(300, 4, 64, device="cuda").bfloat16(), torch.randn(2, 3, 1000, device="cuda")
+scores = torch.zeros(2, 3, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    a, b = window_attention(q, q, q, 20, 0), beam_select(x, scores)
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(a, window_attention(q, q, q, 20, 0))
+assert all(torch.equal(s, t) for s, t in zip(b, beam_select(x, scores)))
+print("captured")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", program], cwd=root, capture_output=True, text=True, timeout=300)
+    assert "captured" in r.stdout, r.stderr[-2000:]
 
 
 def test_calls_on_another_stream():
