@@ -325,7 +325,9 @@ int nq_conv_transpose1d(const nq_weight *w, const void *x, int x_dtype, int64_t 
  *     different ones.
  *   - dtype is NQ_F32 or NQ_BF16, the same for all rows of a call.  Scores,
  *     softmax maxima and sums and output sums are f32; with bf16 rows the
- *     softmax weights are rounded to bf16 for the tensor cores.
+ *     softmax weights are rounded to bf16 for the tensor cores, with f32 rows
+ *     (more than four that share keys) a product is three tf32 products, which
+ *     lose 2^-20 of it at most.
  *   - Sequences are ragged: `offsets` (device int32 [n + 1], ascending) gives
  *     the rows of each; NULL: the same number of rows each.  Rows that belong
  *     to no sequence are neither read nor written.  Offsets and lengths are
@@ -350,7 +352,8 @@ typedef struct nq_rows {
  * [seqs] or NULL): only the first rows of each sequence's span count (padded
  * batches); k_offsets / q_offsets NULL: k_rows / seqs (q_rows / seqs) rows
  * each.  K and V rows that no query of the call sees may hold anything; those
- * that one sees should be finite (a weight of 0 times an infinity is NaN).
+ * that one sees should be finite (a weight of 0 times an infinity is NaN; f32
+ * below 2^127 in magnitude).
  * out must not overlap the inputs.  workspace (16-byte aligned, at least
  * nq_window_attention_workspace bytes; NULL: none) lets few query rows over
  * many keys be split over more of the GPU; results then differ by f32
@@ -368,9 +371,10 @@ int nq_window_attention(const nq_rows *q, const nq_rows *k, const nq_rows *v, co
  * refs = state = 0.  Calls on one cache follow one another on the GPU (one
  * stream, or events between); attention calls may run side by side.
  * A call that cannot be done (no free pages, a slot at max_pages, an index out
- * of range) changes nothing and sets a status bit; the cache's calls then do
- * nothing until nq_cache_status has reported it.  nq_cache_write may have
- * written some of its rows by then. */
+ * of range) changes nothing and sets a status bit; the calls that change the
+ * cache then do nothing until nq_cache_status has reported it, and attention
+ * goes on over what is there.  nq_cache_write may have written some of its rows
+ * by then. */
 typedef struct nq_cache {
   void *k, *v;      /* [layers][pages][kv_heads][page_tokens][head_dim], 16-byte aligned */
   int32_t *table;   /* [slots][max_pages] page of each page_tokens tokens, -1: none */

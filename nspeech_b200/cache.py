@@ -7,7 +7,8 @@ synchronisation, and can be captured into a CUDA graph.  It takes the place of t
 of its decoder's contiguous caches (src/moonshine/gpu_decoder.rs:21-88) for batches and beams.
 
 A decoding step: ``reserve`` once, then per layer ``write`` and ``attention``.  A call that cannot be done (no free
-pages, a full slot, a bad index) changes nothing, and the calls after it do nothing, until ``check`` has raised it.
+pages, a full slot, a bad index) changes nothing, and the calls that change the cache do nothing after it, until
+``check`` has raised it; attention goes on over what is there.
 """
 from __future__ import annotations
 

@@ -7,8 +7,10 @@
 // over the logits makes, per part of a row, its maximum, its sum of
 // exponentials and its `beams` best values (beam_part_kernel); a second, small
 // launch joins the parts and compares across beams in f64 (beam_join_kernel):
-// the terms of a sum are f32, everything added up is f64, so that candidates
-// of two beams compare as their exact scores do up to about 1e-8.
+// the terms of a sum are f32 and added up in f64 from one thread's round on, so
+// that candidates of two beams compare as their exact scores do up to about
+// 2e-7 (the exponential's 2^-22; up to 1.5e-6 where the row's maximum lies up to
+// 40 above its first round's, to which the terms then refer).
 //
 // Selection of the W best of a round of logits without sorting it: the W-th
 // largest of the maxima of 32 thread groups is no larger than the W-th largest

@@ -2,6 +2,7 @@
 // include/nq8.h): window attention, the paged cache, beam search.
 #include <cuda_runtime.h>
 
+#include <cfloat>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -122,12 +123,13 @@ struct MapRows {
 };
 
 // The tensor maps of the tensor-core form; *fits: whether the call is one that
-// it takes (its sizes, 16-byte alignment, a positive scale).
+// it takes (its sizes, 16-byte alignment, a positive scale: masked scores are
+// -inf before the scaling, which must neither turn nor lose them).
 int tensor_maps(const nq::WinAttnParams &p, int dtype, CUtensorMap *tq, CUtensorMap *tk, CUtensorMap *tv, bool *fits) {
   *fits = false;
   const int heads = p.kv_heads * p.group;
   const MapRows q{p.q, p.q_ts, p.q_hs, p.q_rows, heads}, out{p.out, p.o_ts, p.o_hs, p.q_rows, heads};
-  if (p.dim % 8 || !(p.sl2 > 0.f) || !nq::win_attn_tc_fits(dtype == NQ_F32, p.seqs, p.q_rows, p.group) || !q.fits() || !out.fits())
+  if (p.dim % 8 || !(p.sl2 >= FLT_MIN) || !nq::win_attn_tc_fits(dtype == NQ_F32, p.seqs, p.q_rows, p.group) || !q.fits() || !out.fits())
     return NQ_OK;
   int rc;
   if (p.table) {

@@ -93,8 +93,8 @@ __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {  // bits lo..
 __device__ __forceinline__ uint32_t row_bits(const WinAttnParams &p, const KeyList &k, int u, int at) {
   const int shift = k.s_end - k.lo - u;  // of a window key's bit
   const int last = k.n - 1 - u;
-  const int hi = p.right >= kWinUnlimited ? last : min(last, at + p.right + shift);
-  const int lo = max(k.s_end - u, p.left >= kWinUnlimited ? k.s_end - u : at - p.left + shift);
+  const int hi = p.right >= kWinUnlimited ? last : min(last, max(at + p.right, -1) + shift);
+  const int lo = p.left >= kWinUnlimited ? k.s_end - u : max(at - p.left, k.lo) + shift;
   // first keys: entries of their own, or the window's first where it begins at key 0
   const int first = k.s_end ? k.s_end : k.lo ? 0 : p.sinks;
   const int first_hi = min(p.right >= kWinUnlimited ? first - 1 : min(first - 1, at + p.right), k.n - 1) - u;

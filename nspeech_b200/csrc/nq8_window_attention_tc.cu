@@ -8,7 +8,7 @@
 // sinks, then the window of all its rows) are walked in tiles of 128; a tile
 // that none of A's (B's) rows sees is skipped for A (B).
 //
-// Roles (352 threads, one CTA an SM):
+// Roles (384 threads, one CTA an SM; a twelfth warp idles):
 //   warps 0-3   softmax of tile A: thread = query row = TMEM lane
 //   warps 4-7   softmax of tile B
 //   warp 8      K loads (one lane); owns the TMEM
@@ -22,8 +22,14 @@
 // A's threads are in their exponentials, the tensor cores work for B.
 //
 // Bound: per pair of tiles and 128 keys the MMAs take 2 x 2 x 128 x 128 x DP x 2
-// flops (2048 clocks at DP = 128) and the exponentials 2 x 128 x 128 at 16 a
-// clock (2048 clocks).
+// flops (2048 clocks at DP = 128), the exponentials 2 x 128 x 128 at 16 a clock
+// (2048 clocks), and shared memory moves about as long (operands of QK^T 1024,
+// of PV 512, TMA 512).  Such a step takes about 3300 clocks.  16384 tokens, 16
+// query heads over 4 kv heads of 128, window 4096 and 4 sinks: 429 us, 0.67 of
+// the time of its flops at the measured 1666 TFLOP/s; the warp-level form takes
+// 2460 us.  On the way: registers limited for all code by a setmaxnreg ahead of
+// the branches 661 us, MMAs issued by one lane of a divergent warp 471 us, a
+// quarter to three quarters of the exponentials on the FMA pipe 501 to 514 us.
 //
 // O is rescaled only when a row's maximum grows by more than 2^8 (exponentials
 // stay <= 256; the final O / l does not depend on the reference maximum).
@@ -233,210 +239,210 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   // Registers: 384 threads launch with 168 each; 256 x 208 + 128 x 80 is less.
   // One branch for each of the two shares, or the lower limit would hold for all code.
   if (warp >= kWarpK) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-  if (warp == kWarpK || warp == kWarpV) {
-    if ((PAGED || lane == 0) && nt > 0) {
-      // ------------------------------------------------------------- loads
-      // Plain rows: one lane, a box a tile.  Pages: a lane for each box of a
-      // tile (at most 16), whose page is looked up a tile ahead.
-      const bool is_v = warp == kWarpV;
-      const CUtensorMap *map = is_v ? &tm_v : &tm_k;
-      const int full0 = is_v ? L::kVFull : L::kKFull, empty0 = is_v ? L::kVEmpty : L::kKEmpty;
-      const uint32_t slot0 = is_v ? L::kOffV : L::kOffK;
-      bool q_issued = false;
-      if (lane == 0) {
-        prefetch_tmap(map);
-        if (!is_v) {
-          prefetch_tmap(&tm_q);
-          const int toks = 128 / G;
-          mbar_arrive_expect_tx(bar(L::kQFull), p.pair * (DP / 64) * static_cast<uint32_t>(toks * G * 128));
-          for (int x = 0; x < p.pair; ++x)
-#pragma unroll
-            for (int c = 0; c < DP / 64; ++c)
-              tma_load_3d(sbase + L::kOffQ + x * L::kTile + c * L::kBox, &tm_q, bar(L::kQFull), 64 * c, h * G,
-                          sq.q0 + (row0 + x * rows) / G);
-          q_issued = true;
-        }
-      }
-      const int box = PAGED ? min(kKT, 1 << p.page_shift) : kKT;  // rows of a box
-      const int *table = PAGED ? p.table + static_cast<int64_t>(b) * p.table_ld : nullptr;
-      auto page_of = [&](int t) {  // of this lane's box; -1: none, or no key of the list
-        const int key = t < nt ? tl.base(t) + lane * box : 0;
-        if (t >= nt || lane * box >= kKT || key > ks.hi || (tl.in_sinks(t) && key >= ks.s_end)) return -1;
-        const int pg = __ldg(table + (key >> p.page_shift));
-        return pg < p.pages ? pg : -1;
-      };
-      int pg = PAGED ? page_of(0) : 0;
-      int n = 0;
-      for (int t = 0; t < nt; ++t) {
-        const int s = t % S, use = t / S;
-        const int pg_next = PAGED ? page_of(t + 1) : 0;
-        bool ok = use == 0 || mbar_wait(bar(empty0 + s), (use - 1) & 1, lim, abort_flag);
-        if (PAGED) ok = __all_sync(0xffffffffu, ok);
-        if (!ok) {
-          if (lane == 0 && !*abort_flag) report(p.ctl, abort_flag, kDevTimeoutProducer);
-          break;
-        }
-        if (PAGED ? __any_sync(0xffffffffu, *abort_flag) : *abort_flag) break;
-        const uint32_t full = bar(full0 + s), dst = sbase + slot0 + s * L::kTile;
-        const int base = tl.base(t);
-        if constexpr (!PAGED) {
-          mbar_arrive_expect_tx(full, L::kTile);
-#pragma unroll
-          for (int c = 0; c < DP / 64; ++c) tma_load_3d(dst + c * L::kBox, map, full, 64 * c, h, sq.k0 + base);
-        } else {
-          const int boxes = kKT / box;
-          const unsigned have = __ballot_sync(0xffffffffu, pg >= 0);  // boxes whose page exists
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if (warp == kWarpK || warp == kWarpV) {
+      if ((PAGED || lane == 0) && nt > 0) {
+        // ------------------------------------------------------------- loads
+        // Plain rows: one lane, a box a tile.  Pages: a lane for each box of a
+        // tile (at most 16), whose page is looked up a tile ahead.
+        const bool is_v = warp == kWarpV;
+        const CUtensorMap *map = is_v ? &tm_v : &tm_k;
+        const int full0 = is_v ? L::kVFull : L::kKFull, empty0 = is_v ? L::kVEmpty : L::kKEmpty;
+        const uint32_t slot0 = is_v ? L::kOffV : L::kOffK;
+        bool q_issued = false;
+        if (lane == 0) {
+          prefetch_tmap(map);
           if (!is_v) {
-            // the softmax's view of missing pages (keys past the end are masked anyway)
-            if (lane < 4) {
-              uint32_t m = 0;
+            prefetch_tmap(&tm_q);
+            const int toks = 128 / G;
+            mbar_arrive_expect_tx(bar(L::kQFull), p.pair * (DP / 64) * static_cast<uint32_t>(toks * G * 128));
+            for (int x = 0; x < p.pair; ++x)
+  #pragma unroll
+              for (int c = 0; c < DP / 64; ++c)
+                tma_load_3d(sbase + L::kOffQ + x * L::kTile + c * L::kBox, &tm_q, bar(L::kQFull), 64 * c, h * G,
+                            sq.q0 + (row0 + x * rows) / G);
+            q_issued = true;
+          }
+        }
+        const int box = PAGED ? min(kKT, 1 << p.page_shift) : kKT;  // rows of a box
+        const int *table = PAGED ? p.table + static_cast<int64_t>(b) * p.table_ld : nullptr;
+        auto page_of = [&](int t) {  // of this lane's box; -1: none, or no key of the list
+          const int key = t < nt ? tl.base(t) + lane * box : 0;
+          if (t >= nt || lane * box >= kKT || key > ks.hi || (tl.in_sinks(t) && key >= ks.s_end)) return -1;
+          const int pg = __ldg(table + (key >> p.page_shift));
+          return pg < p.pages ? pg : -1;
+        };
+        int pg = PAGED ? page_of(0) : 0;
+        int n = 0;
+        for (int t = 0; t < nt; ++t) {
+          const int s = t % S, use = t / S;
+          const int pg_next = PAGED ? page_of(t + 1) : 0;
+          bool ok = use == 0 || mbar_wait(bar(empty0 + s), (use - 1) & 1, lim, abort_flag);
+          if (PAGED) ok = __all_sync(0xffffffffu, ok);
+          if (!ok) {
+            if (lane == 0 && !*abort_flag) report(p.ctl, abort_flag, kDevTimeoutProducer);
+            break;
+          }
+          if (PAGED ? __any_sync(0xffffffffu, *abort_flag) : *abort_flag) break;
+          const uint32_t full = bar(full0 + s), dst = sbase + slot0 + s * L::kTile;
+          const int base = tl.base(t);
+          if constexpr (!PAGED) {
+            mbar_arrive_expect_tx(full, L::kTile);
+  #pragma unroll
+            for (int c = 0; c < DP / 64; ++c) tma_load_3d(dst + c * L::kBox, map, full, 64 * c, h, sq.k0 + base);
+          } else {
+            const int boxes = kKT / box;
+            const unsigned have = __ballot_sync(0xffffffffu, pg >= 0);  // boxes whose page exists
+            if (!is_v) {
+              // the softmax's view of missing pages (keys past the end are masked anyway)
+              if (lane < 4) {
+                uint32_t m = 0;
+                for (int j = 0; j < boxes; ++j)
+                  if (!(have >> j & 1)) m |= bit_range(j * box - 32 * lane, (j + 1) * box - 1 - 32 * lane);
+                holes[(t & 7) * 4 + lane] = m;
+              }
+            } else if (have != (boxes == 32 ? 0xffffffffu : (1u << boxes) - 1u)) {
+              // missing pages' values: zeros (their weights are zero)
               for (int j = 0; j < boxes; ++j)
-                if (!(have >> j & 1)) m |= bit_range(j * box - 32 * lane, (j + 1) * box - 1 - 32 * lane);
-              holes[(t & 7) * 4 + lane] = m;
-            }
-          } else if (have != (boxes == 32 ? 0xffffffffu : (1u << boxes) - 1u)) {
-            // missing pages' values: zeros (their weights are zero)
-            for (int j = 0; j < boxes; ++j)
-              if (!(have >> j & 1))
-                for (int c = 0; c < DP / 64; ++c)
-                  for (int x = lane; x < box * 8; x += 32)
-                    asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(dst + c * L::kBox + j * box * 128 + x * 16), "r"(0) : "memory");
-            fence_proxy_async_smem();
-          }
-          __syncwarp();
-          const uint32_t box_bytes = static_cast<uint32_t>(box) * 128u;
-          if (lane == 0) mbar_arrive_expect_tx(full, __popc(have) * box_bytes * (DP / 64));
-          __syncwarp();
-          if (pg >= 0) {
-            const int row = ((pg * p.kv_heads + h) << p.page_shift) + ((base + lane * box) & ((1 << p.page_shift) - 1));
-#pragma unroll
-            for (int c = 0; c < DP / 64; ++c) tma_load_2d(dst + c * L::kBox + lane * box_bytes, map, full, 64 * c, row);
-          }
-          pg = pg_next;
-        }
-        ++n;
-      }
-      // Every copy issued into shared memory has landed.
-      volatile int no_abort = 0;
-      if (lane == 0) {
-        for (int s = 0; s < S; ++s) {
-          const int uses = n > s ? (n - 1 - s) / S + 1 : 0;
-          if (uses > 0 && !mbar_wait(bar(full0 + s), (uses - 1) & 1, lim, &no_abort)) atomicOr(p.ctl.status, kDevTimeoutDrain);
-        }
-        if (q_issued && !mbar_wait(bar(L::kQFull), 0, lim, &no_abort)) atomicOr(p.ctl.status, kDevTimeoutDrain);
-      }
-      __syncwarp(PAGED ? 0xffffffffu : 1u);
-    }
-  } else if (warp == kWarpMma && nt > 0) {
-    // ----------------------------------------------------------------- MMA
-    // The whole warp walks the loop, so that addresses and descriptors live in
-    // uniform registers; one elected lane issues.
-    constexpr uint32_t kIdescS = idesc_bf16_f32(128, kKT);
-    constexpr uint32_t kIdescPV = idesc_bf16_f32(128, DP) | (1u << 16);  // B (V) MN-major
-    const bool leader = elect_one();
-    auto uniform = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
-    auto wait = [&](int i, int parity) -> bool {
-      if (__all_sync(0xffffffffu, mbar_try_wait(bar(i), parity))) return true;
-      const bool ok = __all_sync(0xffffffffu, mbar_wait(bar(i), parity, lim, abort_flag));
-      if (!ok && lane == 0 && !*abort_flag) report(p.ctl, abort_flag, kDevTimeoutMma);
-      return ok;
-    };
-    Part part[2];
-    int final_t[2];
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const Part y = part_of(p, tl, sq, G, row0 + x * rows, rows, x < p.pair ? n_rows : 0);
-      part[x] = Part{uniform(y.head), uniform(y.first), uniform(y.last)};
-      final_t[x] = max(part[x].head - 1, part[x].last);
-    }
-    const int n_tiles = uniform(nt);
-    const uint32_t tm = uniform(tmem);
-    int done_p[2] = {0, 0};  // P tiles consumed
-    bool ok = wait(L::kQFull, 0);
-    int slot = 0, phase = 0, v_slot = 0, v_phase = 0;  // of K tile t, of V tile t - 1
-    for (int t = 0; t <= n_tiles && ok; ++t) {
-      if (t < n_tiles && !(ok = wait(L::kKFull + slot, phase))) break;
-      const uint32_t va = sbase + L::kOffV + v_slot * L::kTile;
-      // Descriptors differ in the address field alone.
-      const uint64_t vd = mn_desc(va, L::kBox), kd = sw128_kmajor_desc(sbase + L::kOffK + slot * L::kTile);
-      bool v_ready = false;
-      int k0 = 0, k1 = kKT / 16;
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        if (!ok) break;
-        if (t > 0 && part[x].sees(t - 1)) {
-          if (!v_ready) {
-            if (!(ok = wait(L::kVFull + v_slot, v_phase))) break;
-            v_ready = true;
-            int v0, v1;
-            seen_rows(t - 1, v0, v1);
-            if (v0 > 0 || v1 < kKT) {
-              k0 = uniform(v0 / 16);
-              k1 = uniform((v1 + 15) / 16);
-              for (int r = 16 * k0 + lane / 8; r < 16 * k1; r += 4)
-                if (r < v0 || r >= v1)
+                if (!(have >> j & 1))
                   for (int c = 0; c < DP / 64; ++c)
-                    asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(va + c * L::kBox + r * 128 + (lane & 7) * 16), "r"(0) : "memory");
+                    for (int x = lane; x < box * 8; x += 32)
+                      asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(dst + c * L::kBox + j * box * 128 + x * 16), "r"(0) : "memory");
               fence_proxy_async_smem();
-              __syncwarp();
+            }
+            __syncwarp();
+            const uint32_t box_bytes = static_cast<uint32_t>(box) * 128u;
+            if (lane == 0) mbar_arrive_expect_tx(full, __popc(have) * box_bytes * (DP / 64));
+            __syncwarp();
+            if (pg >= 0) {
+              const int row = ((pg * p.kv_heads + h) << p.page_shift) + ((base + lane * box) & ((1 << p.page_shift) - 1));
+  #pragma unroll
+              for (int c = 0; c < DP / 64; ++c) tma_load_2d(dst + c * L::kBox + lane * box_bytes, map, full, 64 * c, row);
+            }
+            pg = pg_next;
+          }
+          ++n;
+        }
+        // Every copy issued into shared memory has landed.
+        volatile int no_abort = 0;
+        if (lane == 0) {
+          for (int s = 0; s < S; ++s) {
+            const int uses = n > s ? (n - 1 - s) / S + 1 : 0;
+            if (uses > 0 && !mbar_wait(bar(full0 + s), (uses - 1) & 1, lim, &no_abort)) atomicOr(p.ctl.status, kDevTimeoutDrain);
+          }
+          if (q_issued && !mbar_wait(bar(L::kQFull), 0, lim, &no_abort)) atomicOr(p.ctl.status, kDevTimeoutDrain);
+        }
+        __syncwarp(PAGED ? 0xffffffffu : 1u);
+      }
+    } else if (warp == kWarpMma && nt > 0) {
+      // ----------------------------------------------------------------- MMA
+      // The whole warp walks the loop, so that addresses and descriptors live in
+      // uniform registers; one elected lane issues.
+      constexpr uint32_t kIdescS = idesc_bf16_f32(128, kKT);
+      constexpr uint32_t kIdescPV = idesc_bf16_f32(128, DP) | (1u << 16);  // B (V) MN-major
+      const bool leader = elect_one();
+      auto uniform = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+      auto wait = [&](int i, int parity) -> bool {
+        if (__all_sync(0xffffffffu, mbar_try_wait(bar(i), parity))) return true;
+        const bool ok = __all_sync(0xffffffffu, mbar_wait(bar(i), parity, lim, abort_flag));
+        if (!ok && lane == 0 && !*abort_flag) report(p.ctl, abort_flag, kDevTimeoutMma);
+        return ok;
+      };
+      Part part[2];
+      int final_t[2];
+  #pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const Part y = part_of(p, tl, sq, G, row0 + x * rows, rows, x < p.pair ? n_rows : 0);
+        part[x] = Part{uniform(y.head), uniform(y.first), uniform(y.last)};
+        final_t[x] = max(part[x].head - 1, part[x].last);
+      }
+      const int n_tiles = uniform(nt);
+      const uint32_t tm = uniform(tmem);
+      int done_p[2] = {0, 0};  // P tiles consumed
+      bool ok = wait(L::kQFull, 0);
+      int slot = 0, phase = 0, v_slot = 0, v_phase = 0;  // of K tile t, of V tile t - 1
+      for (int t = 0; t <= n_tiles && ok; ++t) {
+        if (t < n_tiles && !(ok = wait(L::kKFull + slot, phase))) break;
+        const uint32_t va = sbase + L::kOffV + v_slot * L::kTile;
+        // Descriptors differ in the address field alone.
+        const uint64_t vd = mn_desc(va, L::kBox), kd = sw128_kmajor_desc(sbase + L::kOffK + slot * L::kTile);
+        bool v_ready = false;
+        int k0 = 0, k1 = kKT / 16;
+  #pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if (!ok) break;
+          if (t > 0 && part[x].sees(t - 1)) {
+            if (!v_ready) {
+              if (!(ok = wait(L::kVFull + v_slot, v_phase))) break;
+              v_ready = true;
+              int v0, v1;
+              seen_rows(t - 1, v0, v1);
+              if (v0 > 0 || v1 < kKT) {
+                k0 = uniform(v0 / 16);
+                k1 = uniform((v1 + 15) / 16);
+                for (int r = 16 * k0 + lane / 8; r < 16 * k1; r += 4)
+                  if (r < v0 || r >= v1)
+                    for (int c = 0; c < DP / 64; ++c)
+                      asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(va + c * L::kBox + r * 128 + (lane & 7) * 16), "r"(0) : "memory");
+                fence_proxy_async_smem();
+                __syncwarp();
+              }
+            }
+            const uint32_t first = done_p[x] == 0;
+            if (!(ok = wait(L::kPReady + x, done_p[x] & 1))) break;
+            tc_fence_after();
+            const uint32_t d = tm + 256 + x * DP, a = tm + x * 128;
+            const bool whole = k0 == 0 && k1 == kKT / 16;
+            if (whole && leader) {
+  #pragma unroll
+              for (int kk = 0; kk < kKT / 32; ++kk) umma_ts(d, a + kk * 8, vd + kk * (2048 >> 4), kIdescPV, kk > 0 ? 1u : 1u - first);
+            }
+            if (!(ok = wait(L::kPReady + 2 + x, done_p[x] & 1))) break;
+            ++done_p[x];
+            tc_fence_after();
+            if (leader) {
+              if (whole) {
+  #pragma unroll
+                for (int kk = kKT / 32; kk < kKT / 16; ++kk) umma_ts(d, a + kk * 8, vd + kk * (2048 >> 4), kIdescPV, 1u);
+              } else {
+                for (int kk = k0; kk < k1; ++kk) umma_ts(d, a + kk * 8, vd + kk * (2048 >> 4), kIdescPV, kk > k0 ? 1u : 1u - first);
+              }
+              if (t - 1 == final_t[x]) umma_commit(bar(L::kOFull + x));
             }
           }
-          const uint32_t first = done_p[x] == 0;
-          if (!(ok = wait(L::kPReady + x, done_p[x] & 1))) break;
-          tc_fence_after();
-          const uint32_t d = tm + 256 + x * DP, a = tm + x * 128;
-          const bool whole = k0 == 0 && k1 == kKT / 16;
-          if (whole && leader) {
-#pragma unroll
-            for (int kk = 0; kk < kKT / 32; ++kk) umma_ts(d, a + kk * 8, vd + kk * (2048 >> 4), kIdescPV, kk > 0 ? 1u : 1u - first);
-          }
-          if (!(ok = wait(L::kPReady + 2 + x, done_p[x] & 1))) break;
-          ++done_p[x];
-          tc_fence_after();
-          if (leader) {
-            if (whole) {
-#pragma unroll
-              for (int kk = kKT / 32; kk < kKT / 16; ++kk) umma_ts(d, a + kk * 8, vd + kk * (2048 >> 4), kIdescPV, 1u);
-            } else {
-              for (int kk = k0; kk < k1; ++kk) umma_ts(d, a + kk * 8, vd + kk * (2048 >> 4), kIdescPV, kk > k0 ? 1u : 1u - first);
+          if (t < n_tiles && part[x].sees(t)) {
+            tc_fence_after();
+            const uint64_t qd = sw128_kmajor_desc(sbase + L::kOffQ + x * L::kTile);
+            if (leader) {
+  #pragma unroll
+              for (int kk = 0; kk < DP / 16; ++kk) {
+                const uint32_t o = ((kk >> 2) * L::kBox + (kk & 3) * 32) >> 4;
+                umma_bf16(tm + x * 128, qd + o, kd + o, kIdescS, kk > 0 ? 1u : 0u);
+              }
+              umma_commit(bar(L::kSFull + x));
             }
-            if (t - 1 == final_t[x]) umma_commit(bar(L::kOFull + x));
           }
         }
-        if (t < n_tiles && part[x].sees(t)) {
-          tc_fence_after();
-          const uint64_t qd = sw128_kmajor_desc(sbase + L::kOffQ + x * L::kTile);
-          if (leader) {
-#pragma unroll
-            for (int kk = 0; kk < DP / 16; ++kk) {
-              const uint32_t o = ((kk >> 2) * L::kBox + (kk & 3) * 32) >> 4;
-              umma_bf16(tm + x * 128, qd + o, kd + o, kIdescS, kk > 0 ? 1u : 0u);
-            }
-            umma_commit(bar(L::kSFull + x));
-          }
+        if (!ok) break;
+        if (t > 0) {
+          // a tile's values are waited for even where no row sees them, so that the ring goes on
+          if (!v_ready && !(ok = wait(L::kVFull + v_slot, v_phase))) break;
+          if (leader) umma_commit(bar(L::kVEmpty + v_slot));
+          if (++v_slot == S) v_slot = 0, v_phase ^= 1;
+        }
+        if (t < n_tiles) {
+          if (leader) umma_commit(bar(L::kKEmpty + slot));
+          if (++slot == S) slot = 0, phase ^= 1;
         }
       }
-      if (!ok) break;
-      if (t > 0) {
-        // a tile's values are waited for even where no row sees them, so that the ring goes on
-        if (!v_ready && !(ok = wait(L::kVFull + v_slot, v_phase))) break;
-        if (leader) umma_commit(bar(L::kVEmpty + v_slot));
-        if (++v_slot == S) v_slot = 0, v_phase ^= 1;
+      // Every MMA issued completes before TMEM is freed.
+      volatile int no_abort = 0;
+      if (leader) {
+        umma_commit(bar(L::kDone));
+        if (!mbar_wait(bar(L::kDone), 0, lim, &no_abort)) atomicOr(p.ctl.status, kDevTimeoutDrain);
       }
-      if (t < n_tiles) {
-        if (leader) umma_commit(bar(L::kKEmpty + slot));
-        if (++slot == S) slot = 0, phase ^= 1;
-      }
+      __syncwarp();
     }
-    // Every MMA issued completes before TMEM is freed.
-    volatile int no_abort = 0;
-    if (leader) {
-      umma_commit(bar(L::kDone));
-      if (!mbar_wait(bar(L::kDone), 0, lim, &no_abort)) atomicOr(p.ctl.status, kDevTimeoutDrain);
-    }
-    __syncwarp();
-  }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ------------------------------------------------------------- softmax
@@ -462,7 +468,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       return ok;
     };
     const int jmax_row = p.right >= kWinUnlimited ? sq.nk - 1 : min(sq.nk - 1, pos + p.right);
-    const int jmin_row = p.left >= kWinUnlimited ? 0 : pos - p.left;
+    const int jmin_row = p.left >= kWinUnlimited ? 0 : max(0, pos - p.left);
     for (int t = 0; t < nt; ++t) {
       if (!part.sees(t)) continue;
       if (!wait_all(L::kSFull + x, n & 1, kDevTimeoutConsumer)) {

@@ -741,6 +741,15 @@ def test_beam_search_over_the_cache_and_its_graph():
     assert torch.equal(cache.table, graph_cache.table) and torch.equal(cache.refs, graph_cache.refs)
 
 
+def test_scales_below_the_normal_numbers():
+    from nspeech_b200.attention import window_attention
+    g = torch.Generator().manual_seed(8)
+    for dt in ("f32", "bf16"):
+        q, k, v = (torch.randn((150, 2, 64), generator=g).to(DT[dt]) for _ in range(3))
+        got = window_attention(q.cuda(), k.cuda(), v.cuda(), 40, 0, 2, scale=1e-40)
+        check_rows(got, *attention64(q, k, v, 40, 0, 2, 1e-40))
+
+
 def test_the_first_call_of_a_process_may_be_captured():
     program = """
 import torch
