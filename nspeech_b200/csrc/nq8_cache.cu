@@ -73,7 +73,10 @@ __device__ __forceinline__ void held_bits(const CacheView &c, uint32_t *bits) {
 
 // Room for the new tokens of slots [first, first + n): one CTA.
 // Shared: held bits of all pages, and per slot its shared last page (-1: none,
-// or it may keep it) and the rank of its first new page.
+// or it may keep it) and the rank of its first new page.  One CTA, because
+// "lowest free page first, in slot order" is one scan over all of them; bound by
+// latency (counts, lengths and tables, three scans, the rows' new entries): 64
+// slots 8.6 us by itself, of which its neighbours in the stream cover some.
 __global__ void __launch_bounds__(kBlock) cache_reserve_kernel(const CacheView c, const int *__restrict__ offsets, int uniform,
                                                                int first, int n) {
   extern __shared__ uint32_t sh[];
@@ -183,7 +186,8 @@ __global__ void __launch_bounds__(kBlock) cache_reserve_kernel(const CacheView c
 }
 
 // The copied last pages: entry blockIdx.x of the list, layer and side of
-// blockIdx.y, the first rows of each head's part of the page.
+// blockIdx.y, the first rows of each head's part of the page.  Bound by latency
+// where few are copied (a step of 8 x 8 beams, 14 layers: 7.5 us by itself).
 template <typename T>
 __global__ void __launch_bounds__(128) cache_copy_kernel(const CacheView c) {
   pdl_wait();
@@ -224,7 +228,9 @@ __device__ __forceinline__ int slot_of(const int *offsets, int n, int r) {
 
 // New tokens into their places: ROWS rows of one layer a CTA.  Within a head a
 // page's rows are adjacent, so the threads go along rows first; their first
-// loads are under way while the rows' places are looked up.
+// loads are under way while the rows' places are looked up.  Bound by memory:
+// 32 prompts of up to 1001 tokens, 14 layers, 10 heads of 64: 231 us, 0.99 of
+// the measured rate; a step's single tokens of 64 slots 5.4 us, by latency.
 template <typename T, int ROWS>
 __global__ void __launch_bounds__(256) cache_write_kernel(const CacheView c, const char *__restrict__ k, const char *__restrict__ v,
                                                           int64_t k_ts, int64_t k_hs, int64_t k_ls, int64_t v_ts, int64_t v_hs,
@@ -307,7 +313,8 @@ __global__ void __launch_bounds__(256) cache_write_kernel(const CacheView c, con
 
 // Slots [first, first + n) become what the slots src[i] were.  A CTA owns a
 // few columns of the table for all n rows and reads them before it writes
-// any, so sources may be among the rows written and repeat.
+// any, so sources may be among the rows written and repeat.  Bound by latency
+// (status, source, entry, count): 64 slots of up to 16 pages 5.4 us.
 __global__ void __launch_bounds__(256) cache_fork_kernel(const CacheView c, const int *__restrict__ src, int first, int n, int cols) {
   extern __shared__ int fork_sh[];  // sources [n], new entries [n][cols]
   int *from = fork_sh, *entry = fork_sh + n;
@@ -355,7 +362,7 @@ __global__ void __launch_bounds__(256) cache_fork_kernel(const CacheView c, cons
 }
 
 // Pages that hold neither one of the first `sinks` tokens nor one of the last
-// `window` of their slot are given back.
+// `window` of their slot are given back.  A CTA a slot; latency.
 __global__ void __launch_bounds__(128) cache_trim_kernel(const CacheView c, int first, int sinks, int window) {
   pdl_wait();
   pdl_trigger();
@@ -374,7 +381,7 @@ __global__ void __launch_bounds__(128) cache_trim_kernel(const CacheView c, int 
 
 // Which pages move: the live ones at or above their count, in order, into the
 // free ones below it.  list 0: moved pages, list 1: their places, list 2: the
-// place of each moved page.
+// place of each moved page.  One CTA, like a reservation; latency: 3001 pages 7 us.
 __global__ void __launch_bounds__(kBlock) cache_plan_kernel(const CacheView c) {
   extern __shared__ uint32_t bits[];
   __shared__ int sums[32];
@@ -425,7 +432,9 @@ __global__ void __launch_bounds__(kBlock) cache_plan_kernel(const CacheView c) {
   }
 }
 
-// The moves' data and the table's new page numbers.
+// The moves' data and the table's new page numbers.  Bound by memory: equal pieces
+// of at most 24 KB, read whole into registers before they are written, eight CTAs
+// an SM.  750 pages of 20 KB in 14 layers, keys and values: 140 us, 6.2 TB/s.
 constexpr int kMoveBytes = 24576;  // at most, of a CTA's turn
 __global__ void __launch_bounds__(256) cache_move_kernel(const CacheView c) {
   pdl_wait();

@@ -780,8 +780,11 @@ __global__ void __launch_bounds__(kThreads) win_attn_tf32(const __grid_constant_
 
 // Row form, for a decoder's single tokens: at most R (1, 2, 4) rows share a
 // key, and a warp takes 8 loads of 32 / (DP / 4) keys at a time straight from
-// memory (lane: four columns), K and V together, so that 16 KB of a CTA are in
-// flight; the four warps and the keys' lane groups join at the end.
+// memory (lane: four columns), K and V together, so that 32 KB of a CTA are in
+// flight; the four warps and the keys' lane groups join at the end.  Bound by
+// latency: a few rounds of dependent loads (length, page, key) a piece, then the
+// join.  16 sequences of up to 5000 tokens, 10 heads of 64, window 1023: 27 us,
+// 3.1 TB/s of the keys and values read.
 template <int DP, int R, bool PAGED, bool VEC>
 __global__ void __launch_bounds__(kThreads) win_attn_f32_rows(const __grid_constant__ WinAttnParams p) {
   constexpr int LPK = DP / 4, KPL = 32 / LPK, U = 8, KT = U * KPL;
@@ -987,13 +990,16 @@ WinAttnPlan win_attn_plan(int sm_count, int f32, bool tensor, bool uniform, int 
   const int64_t each = (rows + pl.rows - 1) / pl.rows;
   const int64_t have = (each > seqs ? each : seqs) * kv_heads;
   // CTAs an SM that a split aims at, and the keys that each takes at least: the
-  // f32 row form (little shared memory, loads straight to registers) six of
-  // 128, the other warp-level forms two of 256, the tensor-core form one of
-  // 1024 (it fills and drains in the time of 256).
+  // f32 row form (little shared memory, loads straight to registers, four CTAs
+  // an SM at 110 registers) four of 64, the other warp-level forms two of 256,
+  // the tensor-core form one of 1024 (it fills and drains in the time of 256).
+  // Measured for the row form, 16 sequences, 10 heads of 64, window 1023: four
+  // an SM 26.9 us, six 32.3 (a second wave); one sequence of 700 keys: 64 keys
+  // 8.4 us, 128 9.6, 256 12.4.
   const bool rows_form = f32 && pl.rows <= 4;
-  const int64_t want = static_cast<int64_t>(tensor ? 1 : rows_form ? 6 : 2) * sm_count;
+  const int64_t want = static_cast<int64_t>(tensor ? 1 : rows_form ? 4 : 2) * sm_count;
   int64_t z = have > 0 ? want / have : 1;
-  pl.split_keys = tensor ? 1024 : rows_form ? 128 : 256;
+  pl.split_keys = tensor ? 1024 : rows_form ? 64 : 256;
   const int64_t most = keys / pl.split_keys;
   z = z < most ? z : most;
   // Few rows over long contexts: pieces of 1024 keys (f32: 384), so that
