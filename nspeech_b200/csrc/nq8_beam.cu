@@ -15,7 +15,7 @@
 // Selection of the W best of a round of logits without sorting it: the W-th
 // largest of the maxima of 32 thread groups is no larger than the W-th largest
 // value, so only values from it on are looked at (about W ln of them for
-// unordered logits), and they are ranked by counting.  Where more than a list
+// unordered logits), and they are ranked by sorting networks.  Where more than a list
 // holds lie above it (many equal values), the same is done with keys (value
 // and inverted index, all different) and a second bound from the thread maxima
 // leaves W threads' values at most.
@@ -81,17 +81,27 @@ __device__ __forceinline__ uint64_t ex2_2(uint64_t v) {
   return f2(ex2(a), ex2(b));
 }
 
-// Keys of this round and the earlier best, ranked by counting; the W best to
-// best[cur ^ 1].
-__device__ __forceinline__ void merge_best(const Key *list, int n, const Key *old, Key *best, int W, int tid) {
-  for (int a = tid; a < n + W; a += kPartThreads) {
-    const Key k = a < n ? list[a] : old[a - n];
-    if (k == 0) continue;
-    int above = 0;
-    for (int z = 0; z < n; ++z) above += list[z] > k;
-    for (int z = 0; z < W; ++z) above += old[z] > k;
-    if (above < W) best[above] = k;
+// Sorting networks of a warp, a key a lane, largest in lane 0.
+__device__ __forceinline__ Key sort32(Key v, int lane) {
+#pragma unroll
+  for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+    for (int o = size / 2; o > 0; o >>= 1) {
+      const Key y = shfl_xor_key(v, o);
+      v = ((lane & o) == 0) == ((lane & size) == 0) ? (y > v ? y : v) : (y < v ? y : v);
+    }
+  return v;
+}
+// The 32 largest of two sorted runs, sorted.
+__device__ __forceinline__ Key merge32(Key a, Key b, int lane) {
+  const Key r = __shfl_sync(0xffffffffu, b, 31 - lane);
+  Key v = r > a ? r : a;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const Key y = shfl_xor_key(v, o);
+    v = (lane & o) == 0 ? (y > v ? y : v) : (y < v ? y : v);
   }
+  return v;
 }
 
 // One part of one row: CTA (blockIdx.x of `splits`, row blockIdx.y).  Values
@@ -106,7 +116,8 @@ __global__ void __launch_bounds__(kPartThreads, 4) beam_part_kernel(const __grid
   __shared__ float group_max[2][32];
   __shared__ Key key_max[32];
   __shared__ Key list[kList];
-  __shared__ Key best[2][kBeamMax];
+  __shared__ Key best[kBeamMax];  // of the rounds ranked so far, best first, 0: none
+  __shared__ Key runs[kPartThreads / 32][32];
   __shared__ int added[2];  // entries listed in rounds of either parity, ever
   __shared__ int listed, ties;
   __shared__ double sums[kPartThreads / 32];
@@ -186,28 +197,33 @@ __global__ void __launch_bounds__(kPartThreads, 4) beam_part_kernel(const __grid
       *place(q) = make_float4(clean(v.x), clean(v.y), clean(v.z), clean(v.w));
     }
   };
-  if (tid < kBeamMax) best[0][tid] = best[1][tid] = 0;
+  if (tid < kBeamMax) best[tid] = 0;
   if (tid == 0) added[0] = added[1] = 0;
-  int cur = 0;
   float ref = -INFINITY;  // the sum's reference: the first rounds' maximum
   double sum = 0.0;       // this thread's part of the sum of exp(x - ref)
   // At least W values of earlier rounds are `floor` or more; -inf counts with floored.
   float floor = -INFINITY;
   bool floored = false;
 
-  // The list's n entries and the earlier best are ranked together (all threads).
+  // The list's n entries and the earlier best are ranked together (all threads):
+  // every warp sorts 32 at a time and keeps its 32 best, one warp joins them.
   auto rank_list = [&](int n) {
-    merge_best(list, n, best[cur], best[cur ^ 1], W, tid);
+    const int warp = tid >> 5;
+    Key v = warp == 0 ? best[lane] : 0;
+    for (int at = 32 * warp; at < n; at += kPartThreads) v = merge32(v, sort32(at + lane < n ? list[at + lane] : 0, lane), lane);
+    runs[warp][lane] = v;
     __syncthreads();
-    if (tid < kBeamMax) best[cur][tid] = 0;  // the next merge's place
-    cur ^= 1;
+    if (warp == 0) {
+      for (int w = 1; w < min((n + 31) / 32, kPartThreads / 32); ++w) v = merge32(v, runs[w][lane], lane);
+      best[lane] = v;
+    }
     __syncthreads();
   };
   // Round c had more values at its bound than the list holds (many equal ones):
   // the same with keys, which are all different.  `before`: entries of earlier rounds.
   auto exact_round = [&](int c, int before) {
     rank_list(before);
-    const Key worst = best[cur][W - 1];
+    const Key worst = best[W - 1];
     const int base = c * kPartElems;
     fetch(c);
     keep([](const float4 &) {});
@@ -372,7 +388,7 @@ __global__ void __launch_bounds__(kPartThreads, 4) beam_part_kernel(const __grid
     // The threads that hold one, one after the other: a lane for each of the
     // thread's elements.
     const float *xf = reinterpret_cast<const float *>(xs);
-    for (unsigned who = __ballot_sync(0xffffffffu, mine >= bound && (!floored || mine > floor)); who; who &= who - 1) {
+    for (unsigned who = __ballot_sync(0xffffffffu, mine >= bound && (!floored || mine > floor) && index(base, 0) < p.vocab); who; who &= who - 1) {
       const int t = (tid & ~31) + __ffs(who) - 1;
       const int i = base + (lane / kVec * kPartThreads + t) * kVec + lane % kVec;
       const float v = clean(xf[(lane / 4 * kPartThreads + t) * 4 + lane % 4]);
@@ -390,7 +406,7 @@ __global__ void __launch_bounds__(kPartThreads, 4) beam_part_kernel(const __grid
   if (lane == 0) sums[tid >> 5] = sum;
   __syncthreads();
   const int64_t at = static_cast<int64_t>(row) * p.splits + blockIdx.x;
-  if (tid < W) p.part_keys[at * W + tid] = best[cur][tid];
+  if (tid < W) p.part_keys[at * W + tid] = best[tid];
   if (tid == 0) {
     double s = 0.0;
 #pragma unroll
@@ -406,40 +422,48 @@ __device__ __forceinline__ Key ordered64(double x) {  // never 0; -0 as +0
 }
 __device__ __forceinline__ double unordered64(Key u) { return __longlong_as_double(static_cast<long long>(u >> 63 ? u & ~(Key{1} << 63) : ~u)); }
 
-// One utterance: W x S sorted lists of W keys (beam, part of its row).  One
-// warp takes the best of their heads W times; a lane holds the best head of
-// every 32nd list.  Better scores go first, then lower beams, then larger keys
-// (a beam's own logits order its candidates).  Latency: 4 beams of four parts
-// 5.6 us, 8 beams 6.8, 32 beams 18 (126 when all candidates were ranked by
-// counting).
-constexpr int kJoinThreads = 256;
-constexpr int kJoinKeys = 2048;  // candidates in shared memory; more are read and scored as they come up
-__global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_constant__ BeamParams p) {
-  __shared__ double lse[kBeamMax], base_score[kBeamMax];
-  __shared__ uint8_t done[kBeamMax], taken[kBeamMax * kBeamSplitsMax];
-  __shared__ ulonglong2 near_keys[kJoinKeys], chosen[kBeamMax];  // score, key
-  __shared__ int chosen_list[kBeamMax];
+// One utterance, a warp a beam: the beam's log sum exp and its W best from its
+// parts' sorted lists, merged.  Then one warp takes the best head of the beams'
+// lists (a lane each) W times.  Better scores go first, then lower beams; within
+// a beam the keys' order is that of the scores.  Latency: one utterance of 4
+// beams 4.8 us, 64 of 8 beams 5.8, 8 of 32 beams 8.9; with one warp over all parts'
+// lists 32 beams over 200000 tokens took 250 us a step, so 37.
+__global__ void __launch_bounds__(32 * kBeamMax) beam_join_kernel(const __grid_constant__ BeamParams p) {
+  __shared__ ulonglong2 lists[kBeamMax][kBeamMax];  // [beam][rank]: score (0: none), key
+  __shared__ bool over[kBeamMax];  // out_finished may be finished: it is read before any is written
   pdl_wait();
   pdl_trigger();
-  const int W = p.beams, S = p.splits, b = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int lists = W * S, all = lists * W;
-  const Key *far_keys = p.part_keys + static_cast<int64_t>(b) * all;  // [beam][split][W]
-  const bool small = all <= kJoinKeys;
-  constexpr int kAhead = 2;  // on their way while the sums are joined
-  Key ahead[kAhead];
-#pragma unroll
-  for (int i = 0; i < kAhead; ++i) ahead[i] = small && tid + i * kJoinThreads < all ? far_keys[tid + i * kJoinThreads] : 0;
-  for (int i = tid; i < lists; i += kJoinThreads) taken[i] = 0;
-  // log sum exp of each beam's row, over its parts (a lane each)
-  for (int k = warp; k < W; k += kJoinThreads / 32) {
-    const int row = b * W + k;
-    const bool fin = p.finished && p.finished[row];
-    const float base = p.scores[row];
+  const int W = p.beams, S = p.splits, b = blockIdx.x, k = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row = b * W + k;
+  const bool fin = p.finished && p.finished[row];
+  const float given = p.scores[row];
+  const double base = isnan(given) ? -INFINITY : static_cast<double>(given);
+  Key key = 0;
+  double lse = 0.0;
+  if (fin) {  // its row was not read
+    if (lane == 0) key = static_cast<Key>(~static_cast<uint32_t>(p.eos)) | Key{1} << 63;
+  } else {
+    const Key *keys = p.part_keys + static_cast<int64_t>(row) * S * W;
     double sum = 0.0;
     float m = -INFINITY;
     if (lane < S) {
       m = p.part_max[static_cast<int64_t>(row) * S + lane];
       sum = p.part_sum[static_cast<int64_t>(row) * S + lane];
+    }
+    // Short lists are taken together, 32 keys at a time (a sort and a join for
+    // them all), long ones one by one (a join each).
+    const int step = W <= 8 ? 32 : W, runs = W <= 8 ? (S * W + 31) / 32 : S;
+    constexpr int kAhead = 4;
+    for (int run = 0; run < runs; run += kAhead) {
+      Key y[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) y[i] = lane < step && (run + i) * step + lane < S * W ? keys[(run + i) * step + lane] : 0;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (run + i < runs) {
+          const Key z = W <= 8 ? sort32(y[i], lane) : y[i];
+          key = run + i ? merge32(key, z, lane) : z;
+        }
     }
     float top = m;
 #pragma unroll
@@ -447,77 +471,34 @@ __global__ void __launch_bounds__(kJoinThreads) beam_join_kernel(const __grid_co
     sum = m > -INFINITY ? (m == top ? sum : sum * exp(static_cast<double>(m) - top)) : 0.0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) {
-      lse[k] = static_cast<double>(top) + log(sum);
-      base_score[k] = isnan(base) ? -INFINITY : static_cast<double>(base);
-      done[k] = fin;
-    }
+    lse = static_cast<double>(top) + log(sum);
   }
+  const float x = unordered(static_cast<uint32_t>(key >> 32));
+  // every logit -inf: there is no sum, and the candidates count as -inf
+  const double s = fin ? base : x > -INFINITY ? base + (static_cast<double>(x) - lse) : -INFINITY;
+  if (lane == 0) over[k] = fin;
+  lists[k][lane] = make_ulonglong2(key ? ordered64(isnan(s) ? -INFINITY : s) : 0, key);
   __syncthreads();
-  // Entry r of list l, and its score.  A finished beam's only candidate stands
-  // first in its first list; its row was not read.
-  auto entry = [&](int l, int r, Key y) {
-    const int k = l / S;
-    if (done[k]) y = r == 0 && l == k * S ? static_cast<Key>(~static_cast<uint32_t>(p.eos)) | Key{1} << 63 : 0;
-    if (y == 0) return make_ulonglong2(0, 0);
-    const float x = unordered(static_cast<uint32_t>(y >> 32));
-    // every logit -inf: there is no sum, and the candidates count as -inf
-    const double s = done[k] ? base_score[k] : x > -INFINITY ? base_score[k] + (static_cast<double>(x) - lse[k]) : -INFINITY;
-    return make_ulonglong2(ordered64(isnan(s) ? -INFINITY : s), y);
-  };
-  if (small) {
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int e = tid + i * kJoinThreads;
-      if (e < all) near_keys[e] = entry(e / W, e % W, ahead[i]);
-    }
-    for (int e = tid + kAhead * kJoinThreads; e < all; e += kJoinThreads) near_keys[e] = entry(e / W, e % W, far_keys[e]);
-  }
-  __syncthreads();
-  if (warp) return;
-  // The best head of the lane's lists: score (0: none), key, list.
-  Key score = 0, key = 0;
-  int list = 0;
-  auto look = [&]() {
-    score = 0;
-    for (int l = lane; l < lists; l += 32) {
-      const int r = taken[l];
-      if (r == W) continue;
-      const ulonglong2 y = small ? near_keys[l * W + r] : entry(l, r, far_keys[l * W + r]);
-      if (y.x > score || (y.x && y.x == score && l / S == list / S && y.y > key)) score = y.x, key = y.y, list = l;
-    }
-  };
-  look();
+  if (k) return;
+  // The lane's beam: its best candidate that is left, and that one's rank.
+  ulonglong2 head = lane < W ? lists[lane][0] : make_ulonglong2(0, 0);
+  int rank = 0, parent = 0;
+  ulonglong2 mine = make_ulonglong2(0, 0);  // the lane-th of the chosen
   for (int r = 0; r < W; ++r) {
-    const uint32_t hi = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(score >> 32));
-    bool mine = score && static_cast<uint32_t>(score >> 32) == hi;
-    const uint32_t lo = __reduce_max_sync(0xffffffffu, mine ? static_cast<uint32_t>(score) : 0u);
-    mine = mine && static_cast<uint32_t>(score) == lo;
-    unsigned who = __ballot_sync(0xffffffffu, mine);
-    if (who & (who - 1)) {  // equal scores
-      const uint32_t beam = __reduce_min_sync(0xffffffffu, mine ? static_cast<uint32_t>(list / S) : 64u);
-      mine = mine && static_cast<uint32_t>(list / S) == beam;
-      const uint32_t value = __reduce_max_sync(0xffffffffu, mine ? static_cast<uint32_t>(key >> 32) : 0u);
-      mine = mine && static_cast<uint32_t>(key >> 32) == value;
-      const uint32_t token = __reduce_max_sync(0xffffffffu, mine ? static_cast<uint32_t>(key) : 0u);
-      mine = mine && static_cast<uint32_t>(key) == token;
-      who = __ballot_sync(0xffffffffu, mine);
-    }
-    if (lane == __ffs(who) - 1) {
-      chosen[r] = make_ulonglong2(score, key);
-      chosen_list[r] = list;
-      ++taken[list];
-      look();
-    }
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(head.x >> 32));
+    const bool most = static_cast<uint32_t>(head.x >> 32) == hi;
+    const uint32_t lo = __reduce_max_sync(0xffffffffu, most ? static_cast<uint32_t>(head.x) : 0u);
+    const int who = __ffs(__ballot_sync(0xffffffffu, most && static_cast<uint32_t>(head.x) == lo)) - 1;
+    const Key chosen = __shfl_sync(0xffffffffu, head.y, who);
+    if (lane == r) parent = who, mine = make_ulonglong2(static_cast<Key>(hi) << 32 | lo, chosen);
+    if (lane == who) head = ++rank < W ? lists[lane][rank] : make_ulonglong2(0, 0);
   }
-  __syncwarp();
   if (lane < W) {
-    const int out = b * W + lane, k = chosen_list[lane] / S;
-    const int t = done[k] ? p.eos : static_cast<int>(~static_cast<uint32_t>(chosen[lane].y));
-    p.out_scores[out] = static_cast<float>(unordered64(chosen[lane].x));
-    p.out_parents[out] = b * W + k;
+    const int out = b * W + lane, t = static_cast<int>(~static_cast<uint32_t>(mine.y));
+    p.out_scores[out] = static_cast<float>(unordered64(mine.x));
+    p.out_parents[out] = b * W + parent;
     p.out_tokens[out] = t;
-    if (p.out_finished) p.out_finished[out] = done[k] || t == p.eos;
+    if (p.out_finished) p.out_finished[out] = over[parent] || t == p.eos;
   }
 }
 
@@ -609,7 +590,7 @@ cudaError_t launch_beam_select(const BeamParams &p, cudaStream_t s) {
                   : vec ? launch_pdl(beam_part_kernel<false, true>, grid, dim3(kPartThreads), smem, s, 1, p)
                         : launch_pdl(beam_part_kernel<false, false>, grid, dim3(kPartThreads), smem, s, 1, p);
   if (e != cudaSuccess) return e;
-  return launch_pdl(beam_join_kernel, dim3(p.items), dim3(kJoinThreads), 0, s, 1, p);
+  return launch_pdl(beam_join_kernel, dim3(p.items), dim3(32 * p.beams), 0, s, 1, p);
 }
 
 cudaError_t launch_beam_reorder(ReorderParams &p, cudaStream_t s) {
