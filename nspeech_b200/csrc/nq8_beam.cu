@@ -427,7 +427,7 @@ __device__ __forceinline__ double unordered64(Key u) { return __longlong_as_doub
 // lists (a lane each) W times.  Better scores go first, then lower beams; within
 // a beam the keys' order is that of the scores.  Latency: one utterance of 4
 // beams 4.8 us, 64 of 8 beams 5.8, 8 of 32 beams 8.9; with one warp over all parts'
-// lists 32 beams over 200000 tokens took 250 us a step, so 37.
+// lists 32 beams over 200000 tokens took 250 us a step, this way 37.
 __global__ void __launch_bounds__(32 * kBeamMax) beam_join_kernel(const __grid_constant__ BeamParams p) {
   __shared__ ulonglong2 lists[kBeamMax][kBeamMax];  // [beam][rank]: score (0: none), key
   __shared__ bool over[kBeamMax];  // out_finished may be finished: it is read before any is written

@@ -489,7 +489,9 @@ __global__ void __launch_bounds__(kThreads) win_attn_mma(const __grid_constant__
 // segments of up to 1501 tokens, 10 heads of 64, window 64 + 16: 307 us; the
 // same tiles by FMA 544 us, bound by shared memory (128-bit loads of operands
 // that 16 products each use); two row tiles a warp, which share the parts of
-// keys and values but leave two CTAs an SM, 400 us.
+// keys and values but leave two CTAs an SM, 400 us.  NARROW: heads of at most
+// DP - 8 skip the columns of zeros (4 x 1000 tokens, 10 heads of 40, causal: 158 -> 116
+// us); the test costs full ones 3 to 8 %, so they go without it.
 template <int DP>
 struct F32Smem {
   static constexpr int kKT = 32, kP = DP + 4;  // pitch: rows 16 bytes apart in the banks
@@ -527,7 +529,7 @@ __device__ __forceinline__ void split_tf32(uint32_t x, uint32_t &hi, uint32_t &l
   lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi));
 }
 
-template <int DP, int WR, bool PAGED, bool VEC>
+template <int DP, int WR, bool PAGED, bool VEC, bool NARROW>
 __global__ void __launch_bounds__(kThreads) win_attn_tf32(const __grid_constant__ WinAttnParams p) {
   using L = F32Smem<DP>;
   constexpr int KT = L::kKT, WK = 4 / WR, KW = KT / WK, R = 16 * WR, P = L::kP, CH = DP / 4;
@@ -619,6 +621,7 @@ __global__ void __launch_bounds__(kThreads) win_attn_tf32(const __grid_constant_
       const uint32_t k_at = ks + ((wk * KW + (lane & 7) + ((lane >> 4) << 3)) * P + ((lane >> 3) & 1) * 4) * 4;
 #pragma unroll
       for (int kk = 0; kk < DP / 8; ++kk) {
+        if (NARROW && 8 * kk >= p.dim) break;
         uint32_t a[4], ah[4], al[4];
         ldsm4(a, q_at + kk * 32);
 #pragma unroll
@@ -635,6 +638,7 @@ __global__ void __launch_bounds__(kThreads) win_attn_tf32(const __grid_constant_
       const uint32_t k_at = ks + ((wk * KW + (lane & 7)) * P + (lane >> 3) * 4) * 4;
 #pragma unroll
       for (int kk = 0; kk < DP / 8; kk += 2) {
+        if (NARROW && 8 * kk >= p.dim) break;
         uint32_t f[4];
         ldsm4(f, k_at + kk * 32);
 #pragma unroll
@@ -687,6 +691,7 @@ __global__ void __launch_bounds__(kThreads) win_attn_tf32(const __grid_constant_
       }
 #pragma unroll
     for (int d = 0; d < DP / 8; ++d) {
+      if (NARROW && 8 * d >= p.dim) break;
       float big[4] = {0.f, 0.f, 0.f, 0.f}, small[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int n = 0; n < N; ++n) {
@@ -933,6 +938,12 @@ cudaError_t launch_smem(dim3 grid, size_t smem, cudaStream_t stream, const WinAt
   return launch_pdl(KERN, grid, dim3(kThreads), smem, stream, 1, p);
 }
 
+template <int DP, int WR, bool PAGED, bool VEC>
+cudaError_t launch_tf32(dim3 grid, cudaStream_t stream, const WinAttnParams &p) {
+  return p.dim <= DP - 8 ? launch_smem<win_attn_tf32<DP, WR, PAGED, VEC, true>>(grid, F32Smem<DP>::kBytes, stream, p)
+                         : launch_smem<win_attn_tf32<DP, WR, PAGED, VEC, false>>(grid, F32Smem<DP>::kBytes, stream, p);
+}
+
 template <int DP, bool PAGED, bool VEC>
 cudaError_t launch_form(const WinAttnParams &p, int f32, const WinAttnPlan &pl, cudaStream_t stream) {
   const dim3 grid(pl.tiles, p.kv_heads, p.splits);
@@ -941,9 +952,9 @@ cudaError_t launch_form(const WinAttnParams &p, int f32, const WinAttnPlan &pl, 
     if (pl.rows == 1) return launch_smem<win_attn_f32_rows<DP, 1, PAGED, VEC>>(grid, 0, stream, p);
     if (pl.rows == 2) return launch_smem<win_attn_f32_rows<DP, 2, PAGED, VEC>>(grid, 0, stream, p);
     if (pl.rows == 4) return launch_smem<win_attn_f32_rows<DP, 4, PAGED, VEC>>(grid, 0, stream, p);
-    if (pl.rows == 16) return launch_smem<win_attn_tf32<DP, 1, PAGED, VEC>>(grid, F32Smem<DP>::kBytes, stream, p);
-    if (pl.rows == 32) return launch_smem<win_attn_tf32<DP, 2, PAGED, VEC>>(grid, F32Smem<DP>::kBytes, stream, p);
-    return launch_smem<win_attn_tf32<DP, 4, PAGED, VEC>>(grid, F32Smem<DP>::kBytes, stream, p);
+    if (pl.rows == 16) return launch_tf32<DP, 1, PAGED, VEC>(grid, stream, p);
+    if (pl.rows == 32) return launch_tf32<DP, 2, PAGED, VEC>(grid, stream, p);
+    return launch_tf32<DP, 4, PAGED, VEC>(grid, stream, p);
   }
   if (pl.rows == 16) return launch_smem<win_attn_mma<DP, 1, kDeep, PAGED, VEC>>(grid, MmaSmem<DP, 16, kDeep>::kBytes, stream, p);
   if (pl.rows == 32) return launch_smem<win_attn_mma<DP, 2, kDeep, PAGED, VEC>>(grid, MmaSmem<DP, 32, kDeep>::kBytes, stream, p);
@@ -977,6 +988,12 @@ WinAttnPlan win_attn_plan(int sm_count, int f32, bool tensor, bool uniform, int 
     pl.rows = pl.pair * static_cast<int>(one);
   } else if (f32) {
     pl.rows = mean <= 1 ? 1 : mean <= 2 ? 2 : mean <= 4 ? 4 : mean <= 16 ? 16 : mean <= 32 ? 32 : 64;
+    // Where 64-row tiles leave SMs idle, 32-row ones end sooner (501 tokens, 10
+    // heads of 64, window 16 + 4: 12.3 -> 9.4 us; 8 x 100 tokens, 8 heads of 64:
+    // 14.8 -> 12.1); with more of them the keys' splitting twice costs more (4000
+    // tokens, 4 heads of 128, window 500, 252 tiles: 119 us, 32-row tiles 164).
+    const int64_t each = (rows + 63) / 64;
+    if (pl.rows == 64 && (each > seqs ? each : seqs) * kv_heads <= sm_count) pl.rows = 32;
   } else {
     pl.rows = mean <= 16 ? 16 : mean <= 32 ? 32 : 64;
   }
@@ -1007,7 +1024,7 @@ WinAttnPlan win_attn_plan(int sm_count, int f32, bool tensor, bool uniform, int 
   // 2048 to 8192 tokens, 32/8 heads of 128: 258 us, pieces of 512 keys 281; f32,
   // 32 sequences of up to 4000 tokens, 8 heads of 128: 131 us, of 1024 160).
   const int64_t piece = f32 ? 384 : 1024;
-  if (!tensor && pl.rows <= 32 && keys >= 2 * piece && z < (keys + piece - 1) / piece) {
+  if (!tensor && mean <= 32 && keys >= 2 * piece && z < (keys + piece - 1) / piece) {
     z = (keys + piece - 1) / piece;
     pl.split_keys = static_cast<int>(piece);
   }
