@@ -82,7 +82,8 @@ __device__ __forceinline__ bool find_tile(const WinAttnParams &p, int tile, int 
 // The keys of a row tile: the sinks [0, s_end) and the window [lo, hi].
 struct Keys {
   int lo, hi, s_end;  // s_end = 0 where the window's tiles hold the sinks too
-  int sink_tiles, tiles;
+  int gap_lo, gap_hi; // then [lo, hi] begins at 0, and no row sees its keys [gap_lo, gap_hi)
+  int sink_tiles;
 };
 template <int KT>
 __device__ __forceinline__ Keys keys_of(const WinAttnParams &p, const Seq &s, int i_first, int i_last) {
@@ -92,12 +93,16 @@ __device__ __forceinline__ Keys keys_of(const WinAttnParams &p, const Seq &s, in
   k.lo = p.left >= kWinUnlimited ? 0 : max(0, p_lo - p.left);
   k.s_end = max(0, min(min(p.sinks, k.lo), k.hi + 1));
   k.sink_tiles = (k.s_end + KT - 1) / KT;
+  k.gap_lo = k.gap_hi = 0;
   if (k.lo <= k.sink_tiles * KT) {  // the two parts touch: one run of tiles
-    if (k.s_end > 0) k.lo = 0;
+    if (k.s_end > 0) {
+      k.gap_lo = k.s_end;
+      k.gap_hi = k.lo;
+      k.lo = 0;
+    }
     k.s_end = 0;
     k.sink_tiles = 0;
   }
-  k.tiles = k.sink_tiles + (k.hi >= k.lo ? (k.hi - k.lo + KT) / KT : 0);
   return k;
 }
 }  // namespace win

@@ -229,11 +229,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     tl.n = static_cast<int>(static_cast<int64_t>(all) * (blockIdx.z + 1) / p.splits) - tl.off;
   }
   const int nt = tl.n;
-  // Rows of tile t that some query of the item may see: the others hold anything.
-  auto seen_rows = [&](int t, int &v0, int &v1) {
+  // Rows of tile t that some query of the item may see, [v0, v1) without [g0, g1)
+  // (between the sinks and the window): the others hold anything.
+  auto seen_rows = [&](int t, int &v0, int &v1, int &g0, int &g1) {
     const int base = tl.base(t);
     v0 = tl.in_sinks(t) ? 0 : max(0, ks.lo - base);
     v1 = min(kKT, (tl.in_sinks(t) ? ks.s_end : ks.hi + 1) - base);
+    g0 = max(0, ks.gap_lo - base);
+    g1 = min(kKT, ks.gap_hi - base);
   };
 
   // Registers: 384 threads launch with 168 each; 256 x 208 + 128 x 80 is less.
@@ -375,13 +378,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (!v_ready) {
               if (!(ok = wait(L::kVFull + v_slot, v_phase))) break;
               v_ready = true;
-              int v0, v1;
-              seen_rows(t - 1, v0, v1);
-              if (v0 > 0 || v1 < kKT) {
+              int v0, v1, g0, g1;
+              seen_rows(t - 1, v0, v1, g0, g1);
+              if (v0 > 0 || v1 < kKT || g0 < g1) {
                 k0 = uniform(v0 / 16);
                 k1 = uniform((v1 + 15) / 16);
                 for (int r = 16 * k0 + lane / 8; r < 16 * k1; r += 4)
-                  if (r < v0 || r >= v1)
+                  if (r < v0 || r >= v1 || (r >= g0 && r < g1))
                     for (int c = 0; c < DP / 64; ++c)
                       asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(va + c * L::kBox + r * 128 + (lane & 7) * 16), "r"(0) : "memory");
                 fence_proxy_async_smem();

@@ -1,0 +1,50 @@
+"""Edges of the decoding operators' contracts: what unseen rows, masked queries, full-size pools and directly following
+launches do, against plain implementations in 64 bits (tolerances as in test_decode_ops_gpu.py)."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from test_decode_ops_gpu import DT, attention64, check_rows, make_cache, nq, offsets  # noqa: E402, F401
+
+
+def unseen_keys(n_q, n_k, left, sinks):
+    """[a, b): the keys after the sinks that lie before the first query's window."""
+    return min(sinks, n_k), max(0, n_k - n_q - left)
+
+
+GAPS = [(200, 300, 50, 4), (300, 400, 20, 70), (150, 390, 5, 130), (400, 460, 59, 0), (129, 257, 0, 1), (150, 600, 100, 4), (40, 160, 9, 30)]
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("hq,hk,d", [(2, 2, 64), (6, 2, 128), (2, 1, 40)])
+@pytest.mark.parametrize("n_q,n_k,left,sinks", GAPS)
+def test_keys_between_the_sinks_and_the_window_may_hold_anything(dt, hq, hk, d, n_q, n_k, left, sinks):
+    """Of a sequence with more keys than queries, the keys that no query sees: their values change nothing."""
+    from nspeech_b200.attention import window_attention
+    a, b = unseen_keys(n_q, n_k, left, sinks)
+    assert b == 0 or a < b
+    g = torch.Generator().manual_seed(n_q + d)
+    q, k, v = (torch.randn((n, h, d), generator=g).to(DT[dt]) for n, h in ((n_q, hq), (n_k, hk), (n_k, hk)))
+    want = attention64(q, k, v, left, 0, sinks)
+    for bad in (float("nan"), float("inf")):
+        k[a:b], v[a:b] = bad, bad
+        check_rows(window_attention(q.cuda(), k.cuda(), v.cuda(), left, 0, sinks), *want)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("page", [8, 64, 256])
+@pytest.mark.parametrize("left,sinks", [(50, 4), (20, 70), (5, 130)])
+def test_cached_tokens_between_the_sinks_and_the_window_may_hold_anything(dt, page, left, sinks):
+    lens, news = [300, 390, 700], [200, 150, 180]
+    cache, rows = make_cache(dt, lens, page, 2, 64, seed=page)
+    for i, (m, n) in enumerate(zip(lens, news)):
+        for j in range(*unseen_keys(n, m, left, sinks)):
+            at = int(cache.table[i, j // page]), slice(None), j % page
+            cache.k[1][at], cache.v[1][at] = float("nan"), float("nan")
+    q = torch.randn((sum(news), 4, 64), generator=torch.Generator().manual_seed(left)).to(DT[dt])
+    got = cache.attention(q.cuda(), 1, offsets(news), left=left, sinks=sinks)
+    at = np.concatenate([[0], np.cumsum(news)])
+    for i, (a, b) in enumerate(zip(at, at[1:])):
+        check_rows(got[a:b], *attention64(q[a:b], rows[i][0][1], rows[i][1][1], left, 0, sinks))
