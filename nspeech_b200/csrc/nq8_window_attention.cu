@@ -136,18 +136,19 @@ __global__ void __launch_bounds__(kThreads) win_attn_join(const __grid_constant_
     for (int z = 0; z < p.splits; ++z) m = fmaxf(m, p.part_ml[z * all + row].x);
     float l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (m > -INFINITY) {
-      for (int z = 0; z < p.splits; ++z) {
-        const float2 ml = p.part_ml[z * all + row];
-        if (ml.x == -INFINITY) continue;
-        const float f = ex2(ml.x - m);
-        const float4 x = *reinterpret_cast<const float4 *>(p.part_o + (z * all + row) * DP + c);
-        l += ml.y * f;
-        o.x += x.x * f;
-        o.y += x.y * f;
-        o.z += x.z * f;
-        o.w += x.w * f;
+    for (int z = 0; z < p.splits; ++z) {
+      const float2 ml = p.part_ml[z * all + row];
+      if (ml.x == -INFINITY) {
+        l += ml.y;  // 0, or NaN where the scores are
+        continue;
       }
+      const float f = ex2(ml.x - m);
+      const float4 x = *reinterpret_cast<const float4 *>(p.part_o + (z * all + row) * DP + c);
+      l += ml.y * f;
+      o.x += x.x * f;
+      o.y += x.y * f;
+      o.z += x.z * f;
+      o.w += x.w * f;
     }
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
     T *out = static_cast<T *>(p.out) + (s.q0 + static_cast<int64_t>(i)) * p.o_ts + hq * p.o_hs;
@@ -900,7 +901,10 @@ __global__ void __launch_bounds__(kThreads) win_attn_f32_rows(const __grid_const
 #pragma unroll
     for (int w = 0; w < 4 * KPL; ++w) {
       const float2 ml = jml[w / KPL][r][w % KPL];
-      if (ml.x == -INFINITY) continue;
+      if (ml.x == -INFINITY) {
+        ll += ml.y;  // 0, or NaN where the scores are
+        continue;
+      }
       const float f = exp2f(ml.x - mm);
       const float4 z = jo[w / KPL][r][(w % KPL) * LPK + cc];
       ll += ml.y * f;

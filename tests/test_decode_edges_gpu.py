@@ -48,3 +48,35 @@ def test_cached_tokens_between_the_sinks_and_the_window_may_hold_anything(dt, pa
     at = np.concatenate([[0], np.cumsum(news)])
     for i, (a, b) in enumerate(zip(at, at[1:])):
         check_rows(got[a:b], *attention64(q[a:b], rows[i][0][1], rows[i][1][1], left, 0, sinks))
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("n_q,n_k,hq,hk,d", [(1, 5, 2, 2, 64), (1, 3000, 2, 2, 64), (1, 3000, 4, 1, 128), (4, 900, 2, 2, 64), (9, 3000, 2, 1, 64),
+                                             (40, 3000, 2, 2, 128), (300, 300, 4, 2, 64), (140, 5000, 2, 2, 64)])
+def test_a_query_that_is_not_a_number_gives_none(dt, n_q, n_k, hq, hk, d):
+    """Its softmax has no value, whatever form runs and however the keys are split; other rows are as they would be."""
+    from nspeech_b200.attention import window_attention
+    g = torch.Generator().manual_seed(n_q + n_k)
+    q, k, v = (torch.randn((n, h, d), generator=g).to(DT[dt]) for n, h in ((n_q, hq), (n_k, hk), (n_k, hk)))
+    want, tol = attention64(q, k, v, -1, 0, 0)
+    row = n_q // 2
+    q[row, 1, 3] = float("nan")
+    got = window_attention(q.cuda(), k.cuda(), v.cuda(), -1, 0).cpu()
+    assert bool(torch.isnan(got[row, 1]).all())
+    got[row, 1], want[row, 1] = 0, 0
+    check_rows(got, want, tol)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("lens", [[6, 40, 9], [3000, 5, 700]])
+def test_a_cached_token_s_query_that_is_not_a_number_gives_none(dt, lens):
+    cache, rows = make_cache(dt, lens, 16, 2, 64)
+    q = torch.randn((3, 4, 64), generator=torch.Generator().manual_seed(2)).to(DT[dt])
+    q[0, 2, 5] = float("nan")
+    got = cache.attention(q.cuda(), 0).cpu()
+    assert bool(torch.isnan(got[0, 2]).all())
+    for i in range(3):
+        want, tol = attention64(q[i:i + 1].nan_to_num(0.0), rows[i][0][0], rows[i][1][0], -1, 0, 0)
+        keep = torch.ones((1, 4), dtype=torch.bool)
+        keep[0, 2] = i > 0
+        check_rows(got[i:i + 1][keep], want[keep], tol[keep])
