@@ -472,13 +472,21 @@ __global__ void __launch_bounds__(256) cache_move_kernel(const CacheView c) {
   }
 }
 
-template <auto KERN>
+// The largest dynamic shared memory of each: with the kernels' static part it
+// stays below the 227 KB of a block.
+constexpr int kReserveSmem = kCacheMaxPages / 8 + kCacheMaxCall * 8;
+constexpr int kPlanSmem = kCacheMaxPages / 8;
+constexpr int fork_cols(int n) { return n <= 16 ? 32 : n <= 32 ? 16 : 8; }
+constexpr int kForkSmem = kCacheMaxCall * (fork_cols(kCacheMaxCall) + 1) * 4;
+static_assert(kReserveSmem <= 226 * 1024 && kForkSmem <= 226 * 1024, "1 KB for static shared memory");
+
+template <auto KERN, int MOST>
 cudaError_t set_smem(size_t bytes) {
   static bool done[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
-  if (bytes <= 48 * 1024 || (dev < 64 && done[dev])) return cudaSuccess;
-  const cudaError_t e = cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+  if (bytes <= 48 * 1024 - 1024 || (dev < 64 && done[dev])) return cudaSuccess;  // 1 KB: the static part
+  const cudaError_t e = cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST);
   if (e == cudaSuccess && dev < 64) done[dev] = true;
   return e;
 }
@@ -487,7 +495,7 @@ cudaError_t set_smem(size_t bytes) {
 
 cudaError_t launch_cache_reserve(const CacheView &c, const int *offsets, int uniform, int first, int n, cudaStream_t s) {
   const size_t smem = (static_cast<size_t>(c.pages) + 31) / 32 * 4 + static_cast<size_t>(n) * 8;
-  cudaError_t e = set_smem<cache_reserve_kernel>(smem);
+  cudaError_t e = set_smem<cache_reserve_kernel, kReserveSmem>(smem);
   if (e != cudaSuccess) return e;
   e = launch_pdl(cache_reserve_kernel, dim3(1), dim3(kBlock), smem, s, 1, c, offsets, uniform, first, n);
   if (e != cudaSuccess) return e;
@@ -517,9 +525,9 @@ cudaError_t launch_cache_write(const CacheView &c, const void *k, const void *v,
 
 cudaError_t launch_cache_fork(const CacheView &c, const int *src, int first, int n, cudaStream_t s) {
   // Few columns a CTA: two entries a thread, and whole 32-byte sectors; at most 144 KB of shared memory.
-  const int cols = n <= 16 ? 32 : n <= 32 ? 16 : 8;
+  const int cols = fork_cols(n);
   const size_t smem = static_cast<size_t>(n) * (cols + 1) * 4;
-  const cudaError_t e = set_smem<cache_fork_kernel>(smem);
+  const cudaError_t e = set_smem<cache_fork_kernel, kForkSmem>(smem);
   if (e != cudaSuccess) return e;
   return launch_pdl(cache_fork_kernel, dim3((c.max_pages + cols - 1) / cols + 1), dim3(256), smem, s, 1, c, src, first, n, cols);
 }
@@ -530,7 +538,7 @@ cudaError_t launch_cache_trim(const CacheView &c, int first, int n, int sinks, i
 
 cudaError_t launch_cache_compact(const CacheView &c, int sm_count, cudaStream_t s) {
   const size_t smem = (static_cast<size_t>(c.pages) + 31) / 32 * 4;
-  cudaError_t e = set_smem<cache_plan_kernel>(smem);
+  cudaError_t e = set_smem<cache_plan_kernel, kPlanSmem>(smem);
   if (e != cudaSuccess) return e;
   e = launch_pdl(cache_plan_kernel, dim3(1), dim3(kBlock), smem, s, 1, c);
   if (e != cudaSuccess) return e;

@@ -80,3 +80,40 @@ def test_a_cached_token_s_query_that_is_not_a_number_gives_none(dt, lens):
         keep = torch.ones((1, 4), dtype=torch.bool)
         keep[0, 2] = i > 0
         check_rows(got[i:i + 1][keep], want[keep], tol[keep])
+
+
+@pytest.mark.parametrize("pages,slots,longest", [(1 << 20, 4096, 2048), (400001, 37, 2048), (140003, 4096, 100)])
+def test_the_largest_pools_and_calls(pages, slots, longest):
+    """Pools and calls at the sizes that the header allows: room, forks and a compaction against numpy."""
+    from nspeech_b200.cache import PagedCache
+    cols = longest // 8 + 2
+    cache = PagedCache.create(1, pages, 8, 1, 8, slots, cols)
+    rng = np.random.default_rng(pages)
+    counts = rng.integers(0, longest, slots)
+    counts[0] = longest
+    cache.reserve(offsets(counts))
+    cache.check()
+    need = -(-counts // 8)
+    want = np.full((slots, cols), -1)
+    want[np.arange(cols) < need[:, None]] = np.arange(need.sum())
+    assert np.array_equal(cache.table.cpu().numpy(), want) and np.array_equal(cache.lens.cpu().numpy(), counts)
+    cache.k[0, :, 0, 0, 0] = (torch.arange(pages, device="cuda") % 251).bfloat16()  # marks that move with their pages
+    src = rng.integers(-1, slots, slots).astype(np.int32)
+    src[: slots // 2] = -1
+    cache.fork(torch.from_numpy(src).cuda())
+    cache.check()
+    want = np.where(src[:, None] >= 0, want[src], -1)
+    refs = np.bincount(want[want >= 0], minlength=pages)
+    assert np.array_equal(cache.table.cpu().numpy(), want) and np.array_equal(cache.refs.cpu().numpy(), refs)
+    marks = np.where(want >= 0, want % 251, 0)
+    cache.compact()
+    cache.check()
+    live = int((refs > 0).sum())
+    assert int(cache.live) == live
+    to = np.arange(pages)
+    to[live + np.flatnonzero(refs[live:])] = np.flatnonzero(refs[:live] == 0)
+    want = np.where(want >= 0, to[want], -1)
+    assert np.array_equal(cache.table.cpu().numpy(), want)
+    pos = torch.from_numpy(np.where(want >= 0, want, 0)).cuda().long()
+    got = cache.k[0, :, 0, 0, 0][pos].float().cpu().numpy()
+    assert np.array_equal(np.where(want >= 0, got, 0), marks)
