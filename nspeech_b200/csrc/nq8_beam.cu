@@ -133,8 +133,9 @@ __global__ void __launch_bounds__(kPartThreads, 4) beam_part_kernel(const __grid
   const char *src = static_cast<const char *>(p.logits) + row * p.ld * (BF16 ? 2 : 4);
   constexpr int kVec = VEC ? BF16 ? 8 : 4 : 1;  // logits of a load
   auto index = [&](int base, int e) { return base + (e / kVec * kPartThreads + tid) * kVec + e % kVec; };
-  // The thread's logits of a round lie in shared memory (its own place: no
-  // synchronisation), those of the next round are on their way in registers.
+  // The thread's logits of a round lie in shared memory, in a place of its own that
+  // its warp's lanes read when they list candidates; those of the next round are on
+  // their way in registers.
   constexpr int kRaw = VEC ? kPerThread / kVec * 4 : kPerThread;
   uint32_t raw[kRaw];
   auto fetch = [&](int c) {  // -inf past the end
@@ -386,7 +387,9 @@ __global__ void __launch_bounds__(kPartThreads, 4) beam_part_kernel(const __grid
     // Values below this round's bound are out, and those not above the floor:
     // W earlier ones go before them.
     // The threads that hold one, one after the other: a lane for each of the
-    // thread's elements.
+    // thread's elements, which the thread itself may have put in place after the
+    // round's synchronisation.
+    __syncwarp();
     const float *xf = reinterpret_cast<const float *>(xs);
     for (unsigned who = __ballot_sync(0xffffffffu, mine >= bound && (!floored || mine > floor) && index(base, 0) < p.vocab); who; who &= who - 1) {
       const int t = (tid & ~31) + __ffs(who) - 1;

@@ -6,7 +6,7 @@ import pytest
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_decode_ops_gpu import DT, attention64, check_rows, make_cache, nq, offsets  # noqa: E402, F401
+from test_decode_ops_gpu import DT, attention64, beam64, check_rows, make_cache, nq, offsets  # noqa: E402, F401
 
 
 def unseen_keys(n_q, n_k, left, sinks):
@@ -117,3 +117,28 @@ def test_the_largest_pools_and_calls(pages, slots, longest):
     pos = torch.from_numpy(np.where(want >= 0, want, 0)).cuda().long()
     got = cache.k[0, :, 0, 0, 0][pos].float().cpu().numpy()
     assert np.array_equal(np.where(want >= 0, got, 0), marks)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("beams", [1, 8, 32])
+@pytest.mark.parametrize("last", [5, 40, 700])
+def test_beam_select_after_rounds_of_equal_values(dt, beams, last):
+    """Rounds with more equal best values than are listed, each followed by one with a few better values at places of
+    other lanes: what a round lists is that round's logits."""
+    from nspeech_b200.beam import beam_select
+    rng, rounds = np.random.default_rng(last), 9
+    items = max(40, 320 // beams)  # several rounds a CTA
+    x = np.zeros((items, beams, rounds * 8192 + last), np.float32)
+    for r in range(rounds):
+        x[:, :, r * 8192:] = r / 2  # all of a round equal, above the one before
+        at = r * 8192 + rng.integers(0, 8192, 11)
+        if r % 2:
+            x[:, :, at] = r / 2 + 0.25 + np.arange(11) / 64
+    x += rng.integers(0, 2, (items, 1, 1))
+    lt = torch.from_numpy(x).to(DT[dt])
+    scores = np.arange(items * beams, dtype=np.float32).reshape(items, beams) * -0.0101  # no ties across beams: 0.6464 k is 0.01 off any integer
+    got = [t.cpu() for t in beam_select(lt.cuda(), torch.from_numpy(scores).cuda())]
+    for i in range(0, items, 13):
+        want = beam64(lt[i].float().numpy(), scores[i], np.zeros(beams, bool), -1)
+        assert got[1][i].tolist() == [i * beams + b for _, b, _ in want]
+        assert got[2][i].tolist() == [t for _, _, t in want]
