@@ -19,6 +19,9 @@
 // holds lie above it (many equal values), the same is done with keys (value
 // and inverted index, all different) and a second bound from the thread maxima
 // leaves W threads' values at most.
+//
+// The kernels start before the one ahead of them has ended, so the logits and
+// parents that it may write are read by plain loads, not by the read-only path.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <math.h>
@@ -145,7 +148,7 @@ __global__ void __launch_bounds__(kPartThreads, 4) beam_part_kernel(const __grid
         const int i = index(c * kPartElems, u * kVec);
         constexpr uint32_t none = BF16 ? 0xff80ff80u : 0xff800000u;
         uint4 v = make_uint4(none, none, none, none);
-        if (i < p.vocab) v = __ldg(reinterpret_cast<const uint4 *>(src + static_cast<int64_t>(i) * (BF16 ? 2 : 4)));
+        if (i < p.vocab) v = *reinterpret_cast<const uint4 *>(src + static_cast<int64_t>(i) * (BF16 ? 2 : 4));
         raw[4 * u] = v.x, raw[4 * u + 1] = v.y, raw[4 * u + 2] = v.z, raw[4 * u + 3] = v.w;
       }
     } else {
@@ -155,9 +158,9 @@ __global__ void __launch_bounds__(kPartThreads, 4) beam_part_kernel(const __grid
         raw[e] = BF16 ? 0xff80u : 0xff800000u;
         if (i < p.vocab) {
           if constexpr (BF16)
-            raw[e] = __ldg(reinterpret_cast<const uint16_t *>(src) + i);
+            raw[e] = reinterpret_cast<const uint16_t *>(src)[i];
           else
-            raw[e] = __ldg(reinterpret_cast<const uint32_t *>(src) + i);
+            raw[e] = reinterpret_cast<const uint32_t *>(src)[i];
         }
       }
     }
@@ -523,7 +526,7 @@ __global__ void __launch_bounds__(256) beam_gather_kernel(const __grid_constant_
   const int64_t lo = static_cast<int64_t>(strip - p.strip0[i]) * kCopyBytes;
   const int64_t left = p.row_bytes[i] - lo;
   const int n = static_cast<int>((left < kCopyBytes ? left : kCopyBytes) / static_cast<int>(sizeof(T)));
-  int from = __ldg(p.parents + r);
+  int from = p.parents[r];
   if (from < 0 || from >= p.rows) from = r;  // out of range: the row's own
   const T *src = reinterpret_cast<const T *>(static_cast<const char *>(p.src[i]) + from * p.src_ld[i] + lo);
   T *dst = reinterpret_cast<T *>(static_cast<char *>(p.dst[i]) + r * p.dst_ld[i] + lo);
@@ -557,7 +560,7 @@ __global__ void __launch_bounds__(256) beam_reorder_kernel(const __grid_constant
   char *dst = static_cast<char *>(p.dst[i]) + lo;
   for (int x = threadIdx.x; x < n * p.rows; x += blockDim.x) {
     const int r = x / n, c = x - r * n;
-    int from = __ldg(p.parents + r);
+    int from = p.parents[r];
     if (from < 0 || from >= p.rows) from = r;  // out of range: the row stays
     strip[x] = reinterpret_cast<const T *>(src + from * p.src_ld[i])[c];
   }

@@ -8,6 +8,10 @@
 // lowest number first, and counts are integers, so atomics' order is not seen.
 // A call that cannot be done changes nothing and sets a status bit; later
 // calls then do nothing until the host has read the status.
+// Kernels start before the one ahead of them has ended and wait for it, so
+// what that one may write (keys and values, offsets, sources) is read by plain
+// loads: the read-only path holds for data that stays as it is for a kernel's
+// whole life.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -48,7 +52,7 @@ __device__ __forceinline__ int block_scan(int x, int *warp_sums, int &all) {
 
 // Tokens that slot i of a call gets: offsets[i + 1] - offsets[i], or `uniform`.
 __device__ __forceinline__ int count_of(const int *offsets, int uniform, int i) {
-  return offsets ? max(0, __ldg(offsets + i + 1) - __ldg(offsets + i)) : uniform;
+  return offsets ? max(0, offsets[i + 1] - offsets[i]) : uniform;
 }
 
 // One bit per page, set where refs > 0, by whole warps.
@@ -77,8 +81,7 @@ __device__ __forceinline__ void held_bits(const CacheView &c, uint32_t *bits) {
 // "lowest free page first, in slot order" is one scan over all of them; bound by
 // latency (counts, lengths and tables, three scans, the rows' new entries): 64
 // slots 8.6 us by itself, of which its neighbours in the stream cover some.
-__global__ void __launch_bounds__(kBlock) cache_reserve_kernel(const CacheView c, const int *__restrict__ offsets, int uniform,
-                                                               int first, int n) {
+__global__ void __launch_bounds__(kBlock) cache_reserve_kernel(const CacheView c, const int *offsets, int uniform, int first, int n) {
   extern __shared__ uint32_t sh[];
   __shared__ int sums[32];
   __shared__ int bad, copies;
@@ -218,7 +221,7 @@ __device__ __forceinline__ int slot_of(const int *offsets, int n, int r) {
   while (len > 1) {
     const int step = (len + 31) / 32;
     const int i = lane * step;
-    const unsigned m = __ballot_sync(0xffffffffu, i < len && __ldg(offsets + lo + i) <= r);
+    const unsigned m = __ballot_sync(0xffffffffu, i < len && offsets[lo + i] <= r);
     const int at = max(__popc(m) - 1, 0) * step;  // the probes that hold come first
     lo += at;
     len = min(step, len - at);
@@ -232,10 +235,9 @@ __device__ __forceinline__ int slot_of(const int *offsets, int n, int r) {
 // 32 prompts of up to 1001 tokens, 14 layers, 10 heads of 64: 231 us, 0.99 of
 // the measured rate; a step's single tokens of 64 slots 5.4 us, by latency.
 template <typename T, int ROWS>
-__global__ void __launch_bounds__(256) cache_write_kernel(const CacheView c, const char *__restrict__ k, const char *__restrict__ v,
-                                                          int64_t k_ts, int64_t k_hs, int64_t k_ls, int64_t v_ts, int64_t v_hs,
-                                                          int64_t v_ls, int layer0, int rows, const int *__restrict__ offsets,
-                                                          int uniform, int first, int n) {
+__global__ void __launch_bounds__(256) cache_write_kernel(const CacheView c, const char *k, const char *v, int64_t k_ts,
+                                                          int64_t k_hs, int64_t k_ls, int64_t v_ts, int64_t v_hs, int64_t v_ls,
+                                                          int layer0, int rows, const int *offsets, int uniform, int first, int n) {
   __shared__ int64_t place[ROWS];  // page row of head 0 (in rows of `dim`), -1: none
   pdl_wait();
   pdl_trigger();
@@ -266,8 +268,8 @@ __global__ void __launch_bounds__(256) cache_write_kernel(const CacheView c, con
       int i, begin, end;
       if (offsets) {
         i = slot_of(offsets, n, r);
-        begin = __ldg(offsets + i);
-        end = __ldg(offsets + i + 1);
+        begin = offsets[i];
+        end = offsets[i + 1];
       } else {
         i = uniform > 0 ? r / uniform : n;
         begin = i * uniform;
@@ -303,19 +305,28 @@ __global__ void __launch_bounds__(256) cache_write_kernel(const CacheView c, con
     const int x = threadIdx.x + 256 * i;
     if (x < all && place[x / units % ROWS] >= 0) put(x, kk[i], vv[i]);
   }
-#pragma unroll 2
-  for (int x = threadIdx.x + 256 * U; x < all; x += 256)
-    if (place[x / units % ROWS] >= 0) {
-      const T a = *source(k, k_ts, k_hs, k_ls, x), b = *source(v, v_ts, v_hs, v_ls, x);
-      put(x, a, b);
+  for (int x0 = threadIdx.x + 256 * U; x0 < all; x0 += 256 * U) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int x = x0 + 256 * i;
+      if (x < all && place[x / units % ROWS] >= 0) {
+        kk[i] = *source(k, k_ts, k_hs, k_ls, x);
+        vv[i] = *source(v, v_ts, v_hs, v_ls, x);
+      }
     }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int x = x0 + 256 * i;
+      if (x < all && place[x / units % ROWS] >= 0) put(x, kk[i], vv[i]);
+    }
+  }
 }
 
 // Slots [first, first + n) become what the slots src[i] were.  A CTA owns a
 // few columns of the table for all n rows and reads them before it writes
 // any, so sources may be among the rows written and repeat.  Bound by latency
 // (status, source, entry, count): 64 slots of up to 16 pages 5.4 us.
-__global__ void __launch_bounds__(256) cache_fork_kernel(const CacheView c, const int *__restrict__ src, int first, int n, int cols) {
+__global__ void __launch_bounds__(256) cache_fork_kernel(const CacheView c, const int *src, int first, int n, int cols) {
   extern __shared__ int fork_sh[];  // sources [n], new entries [n][cols]
   int *from = fork_sh, *entry = fork_sh + n;
   pdl_wait();
@@ -327,7 +338,7 @@ __global__ void __launch_bounds__(256) cache_fork_kernel(const CacheView c, cons
   // Every CTA looks at all sources, so that a bad one leaves all columns alone.
   int wrong = status;
   for (int i = threadIdx.x; i < n; i += blockDim.x) {
-    const int f = src ? __ldg(src + i) : -1;
+    const int f = src ? src[i] : -1;
     from[i] = f;
     wrong |= f < -1 || f >= c.slots;
   }

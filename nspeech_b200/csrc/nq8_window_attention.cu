@@ -108,7 +108,7 @@ __device__ __forceinline__ int64_t key_row(const WinAttnParams &p, const KeyList
   if (u >= k.n) return -1;
   const int j = k.key(u);
   if constexpr (PAGED) {
-    const int pg = __ldg(table + (j >> p.page_shift));
+    const int pg = table[j >> p.page_shift];
     if (pg < 0 || pg >= p.pages) return -1;
     const int r = j & ((1 << p.page_shift) - 1);
     return (((static_cast<int64_t>(pg) * p.kv_heads + h) << p.page_shift) + r) * p.dim;
@@ -810,7 +810,7 @@ __global__ void __launch_bounds__(kThreads) win_attn_f32_rows(const __grid_const
   auto fetch = [&](const float *src, bool there) {
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
     if constexpr (VEC) {
-      if (there && c < p.dim) x = __ldg(reinterpret_cast<const float4 *>(src + c));
+      if (there && c < p.dim) x = *reinterpret_cast<const float4 *>(src + c);
     } else if (there) {
       if (c < p.dim) x.x = src[c];
       if (c + 1 < p.dim) x.y = src[c + 1];

@@ -1,5 +1,8 @@
 // nq8_window_attention.cuh -- what the window attention kernels share: a
 // sequence's rows, the row tile of a CTA, and the keys that a tile sees.
+// The kernels start before the one ahead of them has ended, so what it may
+// write (rows, lengths, offsets, page tables) is read by plain loads, not by
+// the read-only path.
 #pragma once
 
 #include "nq8_window_attention.h"
@@ -20,22 +23,22 @@ struct Seq {
 __device__ __forceinline__ void span(const int *off, const int *len, int rows, int seqs, int b, int &begin, int &n) {
   int e;
   if (off) {
-    begin = min(max(__ldg(off + b), 0), rows);
-    e = min(max(__ldg(off + b + 1), begin), rows);
+    begin = min(max(off[b], 0), rows);
+    e = min(max(off[b + 1], begin), rows);
   } else {
     const int each = rows / seqs;
     begin = b * each;
     e = begin + each;
   }
   n = e - begin;
-  if (len) n = min(n, max(__ldg(len + b), 0));
+  if (len) n = min(n, max(len[b], 0));
 }
 __device__ __forceinline__ Seq seq_of(const WinAttnParams &p, int b) {
   Seq s;
   span(p.q_off, p.q_len, p.q_rows, p.seqs, b, s.q0, s.nq);
   if (p.table) {
     s.k0 = 0;
-    s.nk = static_cast<int>(min(static_cast<long long>(max(__ldg(p.k_len + b), 0)),
+    s.nk = static_cast<int>(min(static_cast<long long>(max(p.k_len[b], 0)),
                                 static_cast<long long>(p.max_pages) << p.page_shift));
   } else {
     span(p.k_off, p.k_len, p.k_rows, p.seqs, b, s.k0, s.nk);

@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         auto page_of = [&](int t) {  // of this lane's box; -1: none, or no key of the list
           const int key = t < nt ? tl.base(t) + lane * box : 0;
           if (t >= nt || lane * box >= kKT || key > ks.hi || (tl.in_sinks(t) && key >= ks.s_end)) return -1;
-          const int pg = __ldg(table + (key >> p.page_shift));
+          const int pg = table[key >> p.page_shift];
           return pg < p.pages ? pg : -1;
         };
         int pg = PAGED ? page_of(0) : 0;

@@ -142,3 +142,71 @@ def test_beam_select_after_rounds_of_equal_values(dt, beams, last):
         want = beam64(lt[i].float().numpy(), scores[i], np.zeros(beams, bool), -1)
         assert got[1][i].tolist() == [i * beams + b for _, b, _ in want]
         assert got[2][i].tolist() == [t for _, _, t in want]
+
+
+class Layers:
+    """Layers of attention between Q8_0-path projections (weights kept at bf16 precision, f32 activations)."""
+
+    def __init__(self, layers=3, heads=2, kv=1, dim=64, width=128):
+        from nspeech_b200.fast_matmul import QWeight
+        g = torch.Generator().manual_seed(23)
+        self.heads, self.kv, self.dim, self.width, self.layers = heads, kv, dim, width, layers
+        sizes = {"qkv": ((heads + 2 * kv) * dim, width), "o": (width, heads * dim)}
+        self.w = [{n: (torch.randn(s, generator=g) * s[1] ** -0.5).bfloat16().float() for n, s in sizes.items()} for _ in range(layers)]
+        self.q = [{n: QWeight.from_f32(t.numpy()) for n, t in w.items()} for w in self.w]
+
+    def step(self, cache, x):
+        """One token a slot: a projection's keys and values go straight into the cache, a layer after the other."""
+        n = x.shape[0]
+        cache.reserve(1, 0, n)
+        for i, q in enumerate(self.q):
+            qkv = q["qkv"].linear(x).view(n, -1, self.dim)
+            q1, k, v = qkv.split([self.heads, self.kv, self.kv], 1)
+            cache.write(k, v, 1, 0, n, layer=i)
+            a = cache.attention(q1, i, n=n)
+            x = q["o"].linear(a.reshape(n, -1)) + x
+        return x
+
+    def run64(self, xs):
+        """The last token's output after the tokens xs [t, width] of one sequence."""
+        x = xs.double()
+        for w in self.w:
+            q, k, v = (x @ w["qkv"].double().T).view(len(x), -1, self.dim).split([self.heads, self.kv, self.kv], 1)
+            a = attention64(q, k, v, -1, 0, 0)[0]
+            x = a.reshape(len(x), -1) @ w["o"].double().T + x
+        return x[-1]
+
+
+@pytest.mark.parametrize("slots", [1, 6])
+def test_layers_write_what_the_projection_before_has_just_made(slots):
+    """Projection, write and attention follow one another directly in every layer, eagerly and in a replayed graph, over
+    buffers that hold the step before's values."""
+    from nspeech_b200.cache import PagedCache
+    net, steps = Layers(), 12
+    xs = torch.randn((slots, steps, net.width), generator=torch.Generator().manual_seed(slots))
+    want = torch.stack([torch.stack([net.run64(xs[i, :t + 1]) for t in range(steps)]) for i in range(slots)])
+    # six projections of f32 activations as bf16 hi + lo planes, each 2^-16 of a sum of absolute terms below 8; gains below 2
+    def close(y, t):
+        assert bool(((y.double().cpu() - want[:, t]).abs() < 2e-3).all()), t
+
+    def begin():
+        return PagedCache.create(net.layers, 4 * slots, 8, net.kv, net.dim, slots, 4, torch.float32)
+
+    cache = begin()
+    for t in range(steps):
+        close(net.step(cache, xs[:, t].contiguous().cuda()), t)
+    cache.check()
+    cache, x = begin(), torch.zeros((slots, net.width), device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        net.step(begin(), x)  # this stream's workspaces
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        y = net.step(cache, x)
+    for t in range(steps):
+        x.copy_(xs[:, t])
+        graph.replay()
+        close(y, t)
+    cache.check()
