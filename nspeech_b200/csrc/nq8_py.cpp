@@ -299,7 +299,7 @@ PyObject *beam_select(PyObject *const *a) {
   const at::Tensor &x = tensor(a[0], "logits"), &s = tensor(a[1], "scores");
   if (x.dim() != 3) misfit("logits must be [items, beams, vocab]");
   const int64_t items = x.size(0), beams = x.size(1), vocab = x.size(2);
-  if ((vocab > 1 && x.stride(2) != 1) || (items > 1 && x.stride(0) != beams * x.stride(1)))
+  if ((vocab > 1 && x.stride(2) != 1) || (items > 1 && beams > 1 && x.stride(0) != beams * x.stride(1)))
     misfit("logits must have unit stride along the vocabulary and evenly spaced rows");
   const int code = code_of(x, "logits");
   const Device dev(x, "logits");

@@ -17,3 +17,15 @@ def test_decoding_kernels_read_by_plain_loads(name):
     with open(os.path.join(CSRC, name)) as f:
         code = re.sub(r"//[^\n]*", "", f.read())
     assert not re.findall(r"__ldg|__ldcs|ld\.global\.nc|__restrict__", code)
+
+
+def test_one_beam_s_rows_may_lie_any_distance_apart():
+    """Greedy decoding over a padded lm_head: with one beam its own stride means nothing.  The refusal left is the host tensor's."""
+    from nspeech_b200.beam import beam_select
+    from nspeech_b200.fast_matmul import MatMulError
+    padded, scores = torch.zeros((4, 100)), torch.zeros((4, 1))
+    for logits in (padded[:, :90].unsqueeze(1), torch.zeros((4, 3, 90))[:, -1:], torch.zeros((4, 1, 90))):
+        with pytest.raises(MatMulError, match="CUDA"):
+            beam_select(logits, scores)
+    with pytest.raises(MatMulError, match="evenly spaced"):
+        beam_select(torch.zeros((4, 3, 90))[:, :2], torch.zeros((4, 2)))

@@ -210,3 +210,16 @@ def test_layers_write_what_the_projection_before_has_just_made(slots):
         graph.replay()
         close(y, t)
     cache.check()
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_greedy_decoding_over_padded_rows(dt):
+    from nspeech_b200.beam import beam_select
+    g = torch.Generator().manual_seed(12)
+    padded = torch.randn((5, 1032), generator=g).to(DT[dt]).cuda()
+    last = torch.randn((5, 3, 1001), generator=g).to(DT[dt]).cuda()
+    scores = -torch.rand((5, 1), generator=g).cuda()
+    for logits in (padded[:, :1000].unsqueeze(1), last[:, -1:]):
+        want = beam_select(logits.contiguous(), scores)
+        assert all(torch.equal(a, b) for a, b in zip(beam_select(logits, scores), want))
+        assert torch.equal(want[2][:, 0].long(), logits[:, 0].float().argmax(1))
