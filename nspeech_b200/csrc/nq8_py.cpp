@@ -10,6 +10,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -47,6 +48,11 @@ void check(int64_t rc) {
   throw Failed();
 }
 
+struct Ref {  // owned reference
+  PyObject *p;
+  ~Ref() { Py_XDECREF(p); }
+};
+
 std::string text(at::IntArrayRef s) {
   std::string r = "(";
   for (size_t i = 0; i < s.size(); ++i) r += (i ? ", " : "") + std::to_string(s[i]);
@@ -54,9 +60,18 @@ std::string text(at::IntArrayRef s) {
 }
 std::string where(int dev) { return "cuda:" + std::to_string(dev); }
 
+// A tensor whose memory is what it stands for; the operators have no gradients.
 const at::Tensor &tensor(PyObject *o, const char *name) {
   if (!THPVariable_Check(o)) misfit(std::string(name) + " must be a tensor");
-  return THPVariable_Unpack(o);
+  const at::Tensor &t = THPVariable_Unpack(o);
+  if (t.is_neg() || t.is_conj()) misfit(std::string(name) + " is a negated or conjugated view (resolve_neg, resolve_conj)");
+  if (t.requires_grad() && c10::GradMode::is_enabled())
+    misfit(std::string(name) + " requires a gradient, which this operator does not have (torch.no_grad, detach)");
+  return t;
+}
+// A given output is written: autograd's saved uses of it are out of date.
+void written(const at::Tensor &t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 int64_t integer(PyObject *o) {
   const long long v = PyLong_AsLongLong(o);
@@ -147,6 +162,7 @@ PyObject *window_attention(PyObject *const *a) {
   if (v.sizes() != k.sizes() || k.size(2) != q.size(2) || k.size(1) == 0 || q.size(1) % k.size(1))
     misfit("q " + text(q.sizes()) + ", k " + text(k.sizes()) + " and v " + text(v.sizes()) + " do not fit together");
   const int code = code_of(q, "q");
+  if (a[12] != Py_None) tensor(a[12], "out");
   const Device dev(q, "q");
   int64_t seqs = 1;
   if (a[11] != Py_None)
@@ -172,7 +188,9 @@ PyObject *window_attention(PyObject *const *a) {
   if (need) ws = empty({need}, at::kByte, dev);
   check(nq_window_attention(r, r + 1, r + 2, r + 3, code, n, q.size(0), k.size(0), qo, ko, ql, kl, hq, hk, d, left, right, sinks,
                             scale_of(a[6], d), need ? ws.data_ptr() : nullptr, need, dev.stream()));
-  return a[12] == Py_None ? THPVariable_Wrap(out) : (Py_INCREF(a[12]), a[12]);
+  if (a[12] == Py_None) return THPVariable_Wrap(out);
+  written(out);
+  return Py_INCREF(a[12]), a[12];
 }
 
 const nq_cache *cache_of(PyObject *o) { return reinterpret_cast<const nq_cache *>(integer(o)); }
@@ -198,7 +216,9 @@ PyObject *cache_attention(PyObject *const *a) {
   if (need) ws = empty({need}, at::kByte, dev);
   check(nq_cache_attention(c, small(a[3], "layer"), &rq, &ro, first, n, q.size(0), off, hq, left, right, sinks,
                            scale_of(a[10], q.size(2)), need ? ws.data_ptr() : nullptr, need, dev.stream()));
-  return a[11] == Py_None ? THPVariable_Wrap(out) : (Py_INCREF(a[11]), a[11]);
+  if (a[11] == Py_None) return THPVariable_Wrap(out);
+  written(out);
+  return Py_INCREF(a[11]), a[11];
 }
 
 // New tokens of a range of slots: offsets, or the same number each.
@@ -317,15 +337,9 @@ PyObject *beam_select(PyObject *const *a) {
   } else {
     PyObject *seq = PySequence_Fast(a[4], "out must be (scores, parents, tokens, finished)");
     if (!seq) throw Failed();
-    const bool four = PySequence_Fast_GET_SIZE(seq) == 4;
-    bool all = four;
-    for (int i = 0; i < 4 && all; ++i) {
-      PyObject *e = PySequence_Fast_GET_ITEM(seq, i);
-      all = THPVariable_Check(e);
-      if (all) o[i] = THPVariable_Unpack(e);
-    }
-    Py_DECREF(seq);
-    if (!all) misfit("out must be (scores, parents, tokens, finished)");
+    const Ref hold{seq};
+    if (PySequence_Fast_GET_SIZE(seq) != 4) misfit("out must be (scores, parents, tokens, finished)");
+    for (int i = 0; i < 4; ++i) o[i] = tensor(PySequence_Fast_GET_ITEM(seq, i), "each of out");
   }
   const at::ScalarType types[4] = {at::kFloat, at::kInt, at::kInt, at::kBool};
   void *po[4];
@@ -336,7 +350,10 @@ PyObject *beam_select(PyObject *const *a) {
                        static_cast<const uint8_t *>(finished), small(a[3], "eos"), static_cast<float *>(po[0]),
                        static_cast<int32_t *>(po[1]), static_cast<int32_t *>(po[2]), static_cast<uint8_t *>(po[3]), ws.data_ptr(), need,
                        dev.stream()));
-  if (a[4] != Py_None) return Py_INCREF(a[4]), a[4];
+  if (a[4] != Py_None) {
+    for (const at::Tensor &t : o) written(t);
+    return Py_INCREF(a[4]), a[4];
+  }
   PyObject *r = PyTuple_New(4);
   if (!r) throw Failed();
   for (int i = 0; i < 4; ++i) PyTuple_SET_ITEM(r, i, THPVariable_Wrap(o[i]));
@@ -361,10 +378,6 @@ PyObject *beam_reorder(PyObject *const *a) {
   if (parents.scalar_type() != at::kInt || !parents.is_contiguous()) misfit("parents must be contiguous int32 on " + where(dev.index));
   const int64_t rows = parents.numel();
   if (rows > INT32_MAX) misfit("too many rows");
-  struct Ref {  // owned reference
-    PyObject *p;
-    ~Ref() { Py_XDECREF(p); }
-  };
   const Ref in{PySequence_Fast(a[0], "states must be a sequence of tensors")};
   if (!in.p) throw Failed();
   const Py_ssize_t n = PySequence_Fast_GET_SIZE(in.p);
@@ -377,6 +390,7 @@ PyObject *beam_reorder(PyObject *const *a) {
   std::vector<const void *> src;
   std::vector<void *> dst;
   std::vector<int64_t> bytes, src_by, dst_by;
+  std::vector<at::Tensor> outs;  // given ones
   for (Py_ssize_t i = 0; i < n; ++i) {
     const at::Tensor &t = tensor(PySequence_Fast_GET_ITEM(in.p, i), "a state");
     const std::string want = "a state must be [" + std::to_string(rows) + ", ...] on " + where(dev.index) + ", like its output";
@@ -388,6 +402,7 @@ PyObject *beam_reorder(PyObject *const *a) {
       if (o.sizes() != t.sizes() || o.scalar_type() != t.scalar_type() || !o.is_cuda() || o.get_device() != dev.index) misfit(want);
       Py_INCREF(e);
       PyList_SET_ITEM(result.p, i, e);
+      outs.push_back(o);
     } else {
       o = empty(t.sizes(), t.scalar_type(), dev);
       PyList_SET_ITEM(result.p, i, THPVariable_Wrap(o));
@@ -407,6 +422,7 @@ PyObject *beam_reorder(PyObject *const *a) {
   for (size_t i = 0; i < src.size(); i += kMost)
     check(nq_beam_reorder(&src[i], &dst[i], &bytes[i], &src_by[i], &dst_by[i], static_cast<int>(std::min(kMost, src.size() - i)),
                           static_cast<int>(rows), static_cast<const int32_t *>(parents.data_ptr()), dev.stream()));
+  for (const at::Tensor &t : outs) written(t);
   PyObject *r = result.p;
   result.p = nullptr;
   return r;

@@ -29,3 +29,23 @@ def test_one_beam_s_rows_may_lie_any_distance_apart():
             beam_select(logits, scores)
     with pytest.raises(MatMulError, match="evenly spaced"):
         beam_select(torch.zeros((4, 3, 90))[:, :2], torch.zeros((4, 2)))
+
+
+def test_python_refuses_what_wants_a_gradient_or_stands_for_other_values():
+    from nspeech_b200.attention import window_attention
+    from nspeech_b200.beam import beam_reorder, beam_select
+    from nspeech_b200.fast_matmul import MatMulError
+    q, x, s, parents = torch.zeros((4, 2, 64)), torch.zeros((1, 2, 9)), torch.zeros((1, 2)), torch.zeros(4, dtype=torch.int32)
+    calls = [lambda t: window_attention(t(q), q, q), lambda t: window_attention(q, t(q), q), lambda t: window_attention(q, q, t(q)),
+             lambda t: window_attention(q, q, q, out=t(q)), lambda t: beam_select(t(x), s), lambda t: beam_select(x, t(s))]
+    learns = [lambda t: t.clone().requires_grad_(), lambda t: t.clone().requires_grad_() * 1]
+    for call in calls:
+        for how in learns:
+            with pytest.raises(MatMulError, match="gradient"):
+                call(how)
+            with torch.no_grad(), pytest.raises(MatMulError, match="CUDA"):  # as far as any host tensor comes
+                call(how)
+        with pytest.raises(MatMulError, match="negated"):
+            call(torch._neg_view)
+    with pytest.raises(MatMulError, match="negated"):
+        beam_reorder([q], torch._neg_view(parents))

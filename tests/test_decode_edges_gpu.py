@@ -223,3 +223,28 @@ def test_greedy_decoding_over_padded_rows(dt):
         want = beam_select(logits.contiguous(), scores)
         assert all(torch.equal(a, b) for a, b in zip(beam_select(logits, scores), want))
         assert torch.equal(want[2][:, 0].long(), logits[:, 0].float().argmax(1))
+
+
+def test_states_that_stand_for_other_values_and_outputs_that_autograd_has_saved():
+    from nspeech_b200.attention import window_attention
+    from nspeech_b200.beam import beam_reorder, beam_select
+    from nspeech_b200.fast_matmul import MatMulError
+    parents = torch.tensor([1, 0], dtype=torch.int32, device="cuda")
+    state = torch.randn((2, 3), device="cuda")
+    for bad, word in ((torch._neg_view(state), "negated"), (torch.randn((2, 3), dtype=torch.cfloat, device="cuda").conj(), "conjugated"),
+                      (state.clone().requires_grad_(), "gradient")):
+        with pytest.raises(MatMulError, match=word):
+            beam_reorder([bad], parents)
+    q, w = torch.randn((8, 2, 64), device="cuda"), torch.ones((), device="cuda", requires_grad=True)
+    kept = torch.randn((2, 3), device="cuda")
+    scores, logits = torch.zeros((1, 2), device="cuda"), torch.randn((1, 2, 9), device="cuda")
+    rest = [t.clone() for t in beam_select(logits, scores)[1:]]
+    for out, write in ((torch.empty_like(q), lambda t: window_attention(q, q, q, out=t)), (kept, lambda t: beam_reorder([state], parents, out=[t])),
+                       (scores, lambda t: beam_select(logits, scores.clone(), out=(t, *rest)))):
+        loss = (out * w).sum()  # saves out
+        write(out)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    with torch.inference_mode():  # nothing is tracked there
+        out = torch.empty_like(q)
+        assert torch.equal(window_attention(q, q, q, out=out), window_attention(q, q, q))
