@@ -9,6 +9,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
@@ -148,9 +149,24 @@ float scale_of(PyObject *o, int64_t dim) {
   if (v == -1.0 && PyErr_Occurred()) throw Failed();
   return static_cast<float>(v);
 }
+// An output that shares memory with itself or with `other` (which it may be,
+// where `same`) as far as torch can say.
+void apart(const at::Tensor &out, const at::Tensor &other, bool same, const std::string &what) {
+  if (at::has_internal_overlap(out) == at::MemOverlap::Yes) misfit("an output overlaps itself");
+  const auto how = at::get_overlap_status(out, other);
+  if (how == at::MemOverlapStatus::Partial || (how == at::MemOverlapStatus::Full && !same)) misfit("an output overlaps " + what);
+}
+// out, if given.
+void check_output(PyObject *o, const at::Tensor &q, const at::Tensor *k, const at::Tensor *v) {
+  if (o == Py_None) return;
+  const at::Tensor &out = tensor(o, "out");
+  apart(out, q, true, "q");
+  if (k) apart(out, *k, false, "k");
+  if (v) apart(out, *v, false, "v");
+}
 at::Tensor output(PyObject *o, const at::Tensor &q, const Device &dev) {
   if (o == Py_None) return empty(q.sizes(), q.scalar_type(), dev);
-  const at::Tensor &out = tensor(o, "out");
+  const at::Tensor &out = THPVariable_Unpack(o);
   if (out.sizes() != q.sizes()) misfit("out has shape " + text(out.sizes()) + ", q " + text(q.sizes()));
   return out;
 }
@@ -162,7 +178,7 @@ PyObject *window_attention(PyObject *const *a) {
   if (v.sizes() != k.sizes() || k.size(2) != q.size(2) || k.size(1) == 0 || q.size(1) % k.size(1))
     misfit("q " + text(q.sizes()) + ", k " + text(k.sizes()) + " and v " + text(v.sizes()) + " do not fit together");
   const int code = code_of(q, "q");
-  if (a[12] != Py_None) tensor(a[12], "out");
+  check_output(a[12], q, &k, &v);
   const Device dev(q, "q");
   int64_t seqs = 1;
   if (a[11] != Py_None)
@@ -203,6 +219,7 @@ PyObject *cache_attention(PyObject *const *a) {
   const at::Tensor &q = tensor(a[2], "q");
   if (q.dim() != 3 || q.size(2) != c->head_dim || q.size(1) % c->kv_heads)
     misfit("q must be [rows, a multiple of " + std::to_string(c->kv_heads) + " heads, " + std::to_string(c->head_dim) + "]");
+  check_output(a[11], q, nullptr, nullptr);
   const int first = small(a[5], "first");
   const int n = a[6] != Py_None ? small(a[6], "n") : a[4] != Py_None ? static_cast<int>(tensor(a[4], "offsets").numel()) - 1 : c->slots - first;
   const nq_rows rq = rows_of(q, "q", type_of(c), dev.index);
@@ -322,24 +339,30 @@ PyObject *beam_select(PyObject *const *a) {
   if ((vocab > 1 && x.stride(2) != 1) || (items > 1 && beams > 1 && x.stride(0) != beams * x.stride(1)))
     misfit("logits must have unit stride along the vocabulary and evenly spaced rows");
   const int code = code_of(x, "logits");
+  at::Tensor o[4];
+  if (a[4] != Py_None) {
+    const Ref seq{PySequence_Fast(a[4], "out must be (scores, parents, tokens, finished)")};
+    if (!seq.p) throw Failed();
+    if (PySequence_Fast_GET_SIZE(seq.p) != 4) misfit("out must be (scores, parents, tokens, finished)");
+    for (int i = 0; i < 4; ++i) {
+      o[i] = tensor(PySequence_Fast_GET_ITEM(seq.p, i), "each of out");
+      apart(o[i], x, false, "the logits");
+      apart(o[i], s, i == 0, "the scores");
+      if (a[2] != Py_None) apart(o[i], tensor(a[2], "finished"), i == 3, "finished");
+      for (int j = 0; j < i; ++j) apart(o[i], o[j], false, "another output");
+    }
+  }
   const Device dev(x, "logits");
   if (items > 65535 || beams > 65535) misfit("too many items or beams");
   const int64_t need = nq_beam_workspace(static_cast<int>(items), static_cast<int>(beams), vocab);
   check(need);
   const void *scores = pair(s, "scores", items, beams, false, at::kFloat, dev.index);
   const void *finished = a[2] == Py_None ? nullptr : pair(tensor(a[2], "finished"), "finished", items, beams, true, at::kBool, dev.index);
-  at::Tensor o[4];
   if (a[4] == Py_None) {
     o[0] = empty({items, beams}, at::kFloat, dev);
     o[1] = empty({items, beams}, at::kInt, dev);
     o[2] = empty({items, beams}, at::kInt, dev);
     o[3] = empty({items, beams}, at::kBool, dev);
-  } else {
-    PyObject *seq = PySequence_Fast(a[4], "out must be (scores, parents, tokens, finished)");
-    if (!seq) throw Failed();
-    const Ref hold{seq};
-    if (PySequence_Fast_GET_SIZE(seq) != 4) misfit("out must be (scores, parents, tokens, finished)");
-    for (int i = 0; i < 4; ++i) o[i] = tensor(PySequence_Fast_GET_ITEM(seq, i), "each of out");
   }
   const at::ScalarType types[4] = {at::kFloat, at::kInt, at::kInt, at::kBool};
   void *po[4];

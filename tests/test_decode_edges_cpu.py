@@ -49,3 +49,24 @@ def test_python_refuses_what_wants_a_gradient_or_stands_for_other_values():
             call(torch._neg_view)
     with pytest.raises(MatMulError, match="negated"):
         beam_reorder([q], torch._neg_view(parents))
+
+
+def test_python_refuses_outputs_that_overlap():
+    from nspeech_b200.attention import window_attention
+    from nspeech_b200.beam import beam_select
+    from nspeech_b200.fast_matmul import MatMulError
+    whole = torch.zeros((12, 2, 64))
+    q, k, v, out = whole[:4], whole[4:8], whole[8:], torch.zeros((4, 2, 64))
+    for bad in (k, v, whole[2:6], whole[1:5], torch.zeros((4, 1, 64)).expand(4, 2, 64), torch.zeros((1, 2, 64)).expand(4, 2, 64)):
+        with pytest.raises(MatMulError, match="overlaps"):
+            window_attention(q, k, v, out=bad)
+    for good in (out, q):  # rows are read before their places are written
+        with pytest.raises(MatMulError, match="CUDA"):
+            window_attention(q, k, v, out=good)
+    x, s, fin = torch.zeros((1, 2, 9)), torch.zeros((1, 2)), torch.zeros((1, 2), dtype=torch.bool)
+    a, b = torch.zeros((1, 2), dtype=torch.int32), torch.zeros((1, 2), dtype=torch.int32)
+    for bad in ((s, a, a, fin), (x[0, :1, :2], a, b, fin), (s, s.view(torch.int32), b, fin)):
+        with pytest.raises(MatMulError, match="overlaps"):
+            beam_select(x, s, fin, 1, out=bad)
+    with pytest.raises(MatMulError, match="CUDA"):
+        beam_select(x, s, fin, 1, out=(s, a, b, fin))

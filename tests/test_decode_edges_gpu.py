@@ -248,3 +248,13 @@ def test_states_that_stand_for_other_values_and_outputs_that_autograd_has_saved(
     with torch.inference_mode():  # nothing is tracked there
         out = torch.empty_like(q)
         assert torch.equal(window_attention(q, q, q, out=out), window_attention(q, q, q))
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("n,m,hq,hk,d", [(1, 3000, 4, 2, 64), (5, 90, 2, 2, 64), (300, 300, 8, 2, 64), (1000, 1000, 3, 3, 128), (130, 4000, 2, 1, 40)])
+def test_attention_in_place_of_its_queries(dt, n, m, hq, hk, d):
+    from nspeech_b200.attention import window_attention
+    g = torch.Generator().manual_seed(n + d)
+    q, k, v = (torch.randn((r, h, d), generator=g).to(DT[dt]).cuda() for r, h in ((n, hq), (m, hk), (m, hk)))
+    want = window_attention(q, k, v, 200, 0, 3)
+    assert torch.equal(window_attention(q, k, v, 200, 0, 3, out=q), want)
