@@ -207,7 +207,7 @@ def native():
         load()
         path = os.path.join(_HERE, "_lib", "nq8_py.so")
         if not os.path.exists(path):
-            raise ImportError(f"{path} is missing: build it with `make -C nspeech_b200/csrc` (there is no CPU fallback)")
+            raise ImportError(f"{path} is missing: build it with `make -C nspeech_b200/csrc python` (there is no CPU fallback)")
         import importlib.machinery
         import importlib.util
 

@@ -1,6 +1,7 @@
 """Edges of the decoding operators' contracts that need no GPU."""
 import os
 import re
+import subprocess
 
 import pytest
 
@@ -70,3 +71,13 @@ def test_python_refuses_outputs_that_overlap():
             beam_select(x, s, fin, 1, out=bad)
     with pytest.raises(MatMulError, match="CUDA"):
         beam_select(x, s, fin, 1, out=(s, a, b, fin))
+
+
+def test_the_library_builds_without_python():
+    """The C ABI's users have nvcc and g++: by itself `make` asks for nothing of Python or torch."""
+    def commands(*targets):
+        r = subprocess.run(["make", "-n", "-B", "-C", CSRC, *targets], capture_output=True, text=True, timeout=60)
+        assert r.returncode == 0, r.stderr
+        return r.stdout
+    assert "libnq8.so" in commands() and not re.search("torch|nq8_py|python", commands())
+    assert "nq8_py.so" in commands("python") and "libnq8.so" in commands("python")
