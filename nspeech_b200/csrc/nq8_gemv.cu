@@ -73,7 +73,9 @@ GemvPlan gemv_plan(int sm_count, int total_tiles, int kc, int m) {
 
 // Activation fragments of one 64-wide chunk for this lane (g, c): for each
 // k quarter q the four bf16 at k = 16q + 4c .. +3 of its row (the k order of
-// the weight words ldsm_x4 hands the lane), zero for rows beyond M.
+// the weight words ldsm_x4 hands the lane), zero for rows beyond M.  Plain
+// loads: the launch before, which may still run when this kernel starts,
+// writes them, and the read-only path is not for such data.
 template <int MT>
 __device__ __forceinline__ void load_x_chunk(uint2 (&v)[MT][4], const __nv_bfloat16 *const (&xr)[MT],
                                              const bool (&live)[MT], int ch) {
@@ -81,7 +83,7 @@ __device__ __forceinline__ void load_x_chunk(uint2 (&v)[MT][4], const __nv_bfloa
   for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
     for (int q = 0; q < 4; ++q)
-      v[mt][q] = live[mt] ? __ldg(reinterpret_cast<const uint2 *>(xr[mt] + static_cast<size_t>(ch) * kPackK + 16 * q))
+      v[mt][q] = live[mt] ? *reinterpret_cast<const uint2 *>(xr[mt] + static_cast<size_t>(ch) * kPackK + 16 * q)
                           : make_uint2(0u, 0u);
   }
 }

@@ -12,7 +12,7 @@ CSRC = os.path.join(ROOT, "nspeech_b200", "csrc")
 
 
 @pytest.mark.parametrize("name", ["nq8_beam.cu", "nq8_cache.cu", "nq8_window_attention.cu", "nq8_window_attention.cuh",
-                                  "nq8_window_attention_tc.cu"])
+                                  "nq8_window_attention_tc.cu", "nq8_gemv.cu"])
 def test_decoding_kernels_read_by_plain_loads(name):
     """These kernels start before their predecessor has ended: what it writes must not go through the read-only path."""
     with open(os.path.join(CSRC, name)) as f:
