@@ -152,7 +152,7 @@ __device__ __forceinline__ Item item_of(const AttnTcParams &p, int it) {
   r.h = bh % heads;
   r.b = bh / heads;
   r.i0 = qt * kBQ;
-  r.L = max(0, min(__ldg(p.len + r.b), p.Tp));
+  r.L = max(0, min(p.len[r.b], p.Tp));
   r.nt = r.i0 < r.L ? (r.L + kBK - 1) / kBK : 0;
   return r;
 }
@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float *vrel = p.vrel + static_cast<int64_t>(w.h) * nrel;
       for (int x = threadIdx.x; x < W; x += kSoftThreads) {
         const int pr = P0 + x;
-        vr_s[x] = (pr >= 0 && pr < nrel) ? __ldg(vrel + pr) : 0.f;
+        vr_s[x] = (pr >= 0 && pr < nrel) ? vrel[pr] : 0.f;
       }
       named_bar_sync(5, kSoftThreads);
       float m_use = -INFINITY, l_part = 0.f;
@@ -571,7 +571,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // vrel[li][h][p] = (v - u)[li][h] . krel[p][li D + h hd : + hd], f32.
 // One warp per (li, h) and relative row p; lanes read 4 consecutive bf16.
-__global__ void __launch_bounds__(256) relpos_bias_kernel(const __nv_bfloat16 *__restrict__ krel,
+__global__ void __launch_bounds__(256) relpos_bias_kernel(const __nv_bfloat16 *krel,
                                                           const float *__restrict__ vmu, int nrel, int pairs, int D,
                                                           int64_t ldr, float *__restrict__ vrel) {
   pdl_wait();

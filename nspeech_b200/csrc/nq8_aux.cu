@@ -6,7 +6,7 @@ namespace nq {
 
 // hi[m, k] = bf16(x), lo[m, k] = bf16(x - hi); rows of k_pad, zero for k >= K.
 // Four consecutive k per thread (8-byte stores).
-__global__ void split_x_kernel(const void *__restrict__ x, int x_dtype, int64_t ldx, int64_t M, int64_t K,
+__global__ void split_x_kernel(const void *x, int x_dtype, int64_t ldx, int64_t M, int64_t K,
                                int64_t k_pad, __nv_bfloat16 *__restrict__ hi, __nv_bfloat16 *__restrict__ lo) {
   pdl_wait();  // predecessor kernel complete, its writes visible
   pdl_trigger();

@@ -26,7 +26,9 @@ inline cudaError_t launched() {
 // a launch then overlaps its launch latency and prologue with the tail of
 // the previous kernel on the stream, and waits for that kernel's completion
 // (and memory) before touching data.  A predecessor that never triggers
-// completes first, as without the attribute.
+// completes first, as without the attribute.  What a predecessor may write is
+// read by plain loads: __ldg and const __restrict__ pointers (the read-only
+// path) are for data that no kernel changes while this one lives, such as weights.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -40,7 +40,7 @@ __device__ __forceinline__ float leaky(float v, float slope) { return v >= 0.f ?
 // The block of the last chunk also zero-fills [c_in K, ld).  ld % 8 == 0 and
 // cb K % 8 == 0 unless cb == c_in keep every 8-element group aligned.
 constexpr int kIcTTMax = 32;
-__global__ void __launch_bounds__(256) im2col_kernel(const void *__restrict__ x, int x_dtype, int64_t ldx, int c_in,
+__global__ void __launch_bounds__(256) im2col_kernel(const void *x, int x_dtype, int64_t ldx, int c_in,
                                                      int t_in, int K, int stride, int pad, int dil, float slope,
                                                      int t_out, int64_t ld, int a_dtype, void *__restrict__ rows, int cb,
                                                      int tt, int W, int pitch) {
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(256) im2col_kernel(const void *__restrict__ x,
 // 16 bytes per thread where the vector lies inside the row (issued before
 // their use).  Stores write whole 128-byte channel runs per frame.
 constexpr int kTokT = 32;
-__global__ void __launch_bounds__(256) conv_tokens_kernel(const void *__restrict__ x, int x_dtype, int64_t ldx, int c_in,
+__global__ void __launch_bounds__(256) conv_tokens_kernel(const void *x, int x_dtype, int64_t ldx, int c_in,
                                                           int t_in, float slope, __nv_bfloat16 *__restrict__ hi,
                                                           __nv_bfloat16 *__restrict__ lo, int vec) {
   pdl_wait();
@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(256) conv_tokens_kernel(const void *__restrict
     const __nv_bfloat16 *src = xb + static_cast<int64_t>(c0 + c) * ldx + t;
     uint4 v;
     if (vec && t + 8 <= t_in) {
-      v = __ldg(reinterpret_cast<const uint4 *>(src));
+      v = *reinterpret_cast<const uint4 *>(src);
     } else {
       uint16_t e[8];
 #pragma unroll
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(256) conv_tokens_kernel(const void *__restrict
       const int q = threadIdx.x + i * 256, c = q >> 3, t = t0 + (q & 7) * 4;
       const float *src = xf + static_cast<int64_t>(c0 + c) * ldx + t;
       if (vec && t + 4 <= t_in) {
-        v[i] = __ldg(reinterpret_cast<const float4 *>(src));
+        v[i] = *reinterpret_cast<const float4 *>(src);
       } else {
         v[i] = make_float4(t < t_in ? src[0] : 0.f, t + 1 < t_in ? src[1] : 0.f, t + 2 < t_in ? src[2] : 0.f,
                            t + 3 < t_in ? src[3] : 0.f);
@@ -218,7 +218,7 @@ __global__ void conv_poly_weight_kernel(const __nv_bfloat16 *__restrict__ src, i
 }
 
 // y[c][t] (ldy) = src[t][c] (lds): 32 x 32 tiles through shared memory.
-__global__ void transpose_out_kernel(const void *__restrict__ src, int src_dtype, int64_t lds, int rows_t, int cols_c,
+__global__ void transpose_out_kernel(const void *src, int src_dtype, int64_t lds, int rows_t, int cols_c,
                                      void *__restrict__ y, int y_dtype, int64_t ldy) {
   pdl_wait();
   pdl_trigger();
@@ -242,7 +242,7 @@ __global__ void transpose_out_kernel(const void *__restrict__ src, int src_dtype
 
 // y[co][t] = act(bias[co] + sum over taps j ascending with (t + pad - j) % stride
 // == 0 and ti = (t + pad - j) / stride in [0, t_in) of cols[ti][co * K + j]).
-__global__ void col2im_kernel(const float *__restrict__ cols, int64_t ldc, int t_in, int c_out, int K, int stride,
+__global__ void col2im_kernel(const float *cols, int64_t ldc, int t_in, int c_out, int K, int stride,
                               int pad, int t_out, const float *__restrict__ bias, int epi, void *__restrict__ y,
                               int y_dtype, int64_t ldy) {
   pdl_wait();

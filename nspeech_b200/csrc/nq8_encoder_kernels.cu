@@ -23,7 +23,7 @@ __device__ __forceinline__ float bf(const __nv_bfloat16 v) { return __bfloat162f
 // thread c computes channel c for every output frequency; each output row
 // position is one contiguous C-wide store across the block.
 constexpr int kMaxFeat = 512;
-__global__ void conv0_relu_kernel(const float *__restrict__ mel, const int *__restrict__ len0, int T, int F,
+__global__ void conv0_relu_kernel(const float *mel, const int *len0, int T, int F,
                                   int T1, int F1, int C, const float *__restrict__ w, const float *__restrict__ bias,
                                   __nv_bfloat16 *__restrict__ out) {
   pdl_wait();  // predecessor kernel complete, its writes visible
@@ -126,7 +126,7 @@ __device__ __forceinline__ uint64_t f32x2_of_bf16x2(uint32_t v) {
 }
 
 __global__ void __launch_bounds__(256) conv0_dw_s2_kernel(
-    const float *__restrict__ mel, const int *__restrict__ len0, const int *__restrict__ len1, int T, int F, int T1,
+    const float *mel, const int *len0, const int *len1, int T, int F, int T1,
     int F1, int T2, int F2, int C, const float *__restrict__ w0, const float *__restrict__ b0,
     const float *__restrict__ w2, const float *__restrict__ b2, __nv_bfloat16 *__restrict__ out) {
   extern __shared__ __align__(16) unsigned char cd_smem[];
@@ -171,8 +171,9 @@ __global__ void __launch_bounds__(256) conv0_dw_s2_kernel(
       const bool live = t >= 0 && t < T && t < L0;
       const float *src = mel + (static_cast<int64_t>(b) * T + (live ? t : 0)) * F;
       if (live && vec) {
+#pragma unroll 1  // once or twice; unrolled, the kernel takes 150 registers and one block an SM
         for (int f = 4 * lane; f < F; f += 128) {
-          const float4 v = __ldg(reinterpret_cast<const float4 *>(src + f));
+          const float4 v = *reinterpret_cast<const float4 *>(src + f);
           dst[f + 1] = v.x;
           dst[f + 2] = v.y;
           dst[f + 3] = v.z;
@@ -295,9 +296,8 @@ __global__ void __launch_bounds__(256) conv0_dw_s2_kernel(
 // the same tap order (dt, then df) as a per-output loop.
 constexpr int kDwRows = 2, kDwCols = 4;
 
-__global__ void __launch_bounds__(256) dwconv2d_s2_kernel(const __nv_bfloat16 *__restrict__ in,
-                                                          const int *__restrict__ len_in, int Tin, int Fin, int Tout,
-                                                          int Fout, int C, const float *__restrict__ w,
+__global__ void __launch_bounds__(256) dwconv2d_s2_kernel(const __nv_bfloat16 *in, const int *len_in, int Tin,
+                                                          int Fin, int Tout, int Fout, int C, const float *__restrict__ w,
                                                           const float *__restrict__ bias,
                                                           __nv_bfloat16 *__restrict__ out) {
   const int lane = threadIdx.x & 31;
@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(256) dwconv2d_s2_kernel(const __nv_bfloat16 *_
 #pragma unroll
     for (int cc = 0; cc < 2 * kDwCols + 1; ++cc) {
       const int f = 2 * fo0 - 1 + cc;
-      const uint32_t p = f >= 0 && f < Fin ? __ldg(reinterpret_cast<const unsigned int *>(row + static_cast<int64_t>(f) * C)) : 0u;
+      const uint32_t p = f >= 0 && f < Fin ? *reinterpret_cast<const unsigned int *>(row + static_cast<int64_t>(f) * C) : 0u;
       v[cc] = f2(__uint_as_float(p << 16), __uint_as_float(p & 0xffff0000u));
     }
 #pragma unroll
@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(256) dwconv2d_s2_kernel(const __nv_bfloat16 *_
 }
 
 // Any C: one output per thread (the general fallback of the kernel above).
-__global__ void dwconv2d_s2_any_kernel(const __nv_bfloat16 *__restrict__ in, const int *__restrict__ len_in, int Tin,
+__global__ void dwconv2d_s2_any_kernel(const __nv_bfloat16 *in, const int *len_in, int Tin,
                                    int Fin, int Tout, int Fout, int C, const float *__restrict__ w,
                                    const float *__restrict__ bias, __nv_bfloat16 *__restrict__ out) {
   pdl_wait();  // predecessor kernel complete, its writes visible
@@ -392,7 +392,7 @@ __global__ void dwconv2d_s2_any_kernel(const __nv_bfloat16 *__restrict__ in, con
 
 // NHWC [B*T, F, C] -> [B*T, C*F] (the reference flattens transpose(1,2) of
 // NCHW, feature index c*F + f; fast_conformer.rs:184-186).
-__global__ void flatten_cf_kernel(const __nv_bfloat16 *__restrict__ in, int rows, int F, int C,
+__global__ void flatten_cf_kernel(const __nv_bfloat16 *in, int rows, int F, int C,
                                   __nv_bfloat16 *__restrict__ out) {
   pdl_wait();  // predecessor kernel complete, its writes visible
   pdl_trigger();
@@ -423,7 +423,7 @@ constexpr int kLnThreads = 256;
 __host__ __device__ constexpr int ln_min_blocks(int kVec) { return kVec >= 8 ? 2 : 3; }
 template <int kVec>
 __global__ void __launch_bounds__(kLnThreads, ln_min_blocks(kVec))
-    ln_row_kernel(int mode, float *__restrict__ x, const void *__restrict__ u, float alpha, int rows,
+    ln_row_kernel(int mode, float *__restrict__ x, const void *u, float alpha, int rows,
                   const float *__restrict__ g1, const float *__restrict__ b1, const float *__restrict__ g2,
                   const float *__restrict__ b2, __nv_bfloat16 *__restrict__ h, float eps) {
   constexpr int D = 32 * 4 * kVec;
@@ -546,7 +546,7 @@ __global__ void __launch_bounds__(kLnThreads, ln_min_blocks(kVec))
 // registers, so every input element is read once per chunk.
 template <int K>
 __global__ void __launch_bounds__(128) dwconv1d_bn_silu_kernel(
-    const __nv_bfloat16 *__restrict__ in, const int *__restrict__ len, int Tp, int D, int t_chunk,
+    const __nv_bfloat16 *in, const int *len, int Tp, int D, int t_chunk,
     const float *__restrict__ w, const float *__restrict__ bias, const float *__restrict__ bn_scale,
     const float *__restrict__ bn_shift, __nv_bfloat16 *__restrict__ out) {
   pdl_wait();  // predecessor kernel complete, its writes visible
@@ -675,9 +675,9 @@ __device__ __forceinline__ void load_rows_async(__nv_bfloat16 *dst, const __nv_b
 }
 
 __global__ void __launch_bounds__(32 * kAWarps, 1)
-    relpos_attention_kernel(const __nv_bfloat16 *__restrict__ qkv, const __nv_bfloat16 *__restrict__ krel, int64_t ldr,
+    relpos_attention_kernel(const __nv_bfloat16 *qkv, const __nv_bfloat16 *krel, int64_t ldr,
                             const float *__restrict__ bias_u, const float *__restrict__ bias_v,
-                            const int *__restrict__ len, int Tp, int D, float scale, __nv_bfloat16 *__restrict__ out) {
+                            const int *len, int Tp, int D, float scale, __nv_bfloat16 *__restrict__ out) {
   pdl_wait();  // predecessor kernel complete, its writes visible
   pdl_trigger();
   extern __shared__ __align__(16) uint8_t sm[];
@@ -902,7 +902,7 @@ __global__ void __launch_bounds__(32 * kAWarps, 1)
   }
 }
 
-__global__ void copy_masked_kernel(const float *__restrict__ x, const int *__restrict__ len, int Tp, int D,
+__global__ void copy_masked_kernel(const float *x, const int *len, int Tp, int D,
                                    float *__restrict__ out) {
   pdl_wait();  // predecessor kernel complete, its writes visible
   pdl_trigger();

@@ -116,11 +116,11 @@ __global__ void __launch_bounds__(32 * kQtWarps) qtiled_kernel(const QtiledParam
 #pragma unroll
       for (int t = 0; t < TN; ++t) {
         const int8_t *xr = xb[t] + kb * 32 + tig * 4;
-        const uint32_t b0 = __ldg(reinterpret_cast<const unsigned int *>(xr));
-        const uint32_t b1 = __ldg(reinterpret_cast<const unsigned int *>(xr + 16));
+        const uint32_t b0 = *reinterpret_cast<const unsigned int *>(xr);
+        const uint32_t b1 = *reinterpret_cast<const unsigned int *>(xr + 16);
         int d[4];
         mma_s8(d, a, b0, b1);
-        const float x0 = __ldg(sx0[t] + kb), x1 = __ldg(sx1[t] + kb);
+        const float x0 = sx0[t][kb], x1 = sx1[t][kb];
         // (n = g, m = 2 tig), (g, 2 tig + 1), (g + 8, 2 tig), (g + 8, 2 tig + 1)
         acc[t][0] = __fadd_rn(acc[t][0], __fmul_rn(__fmul_rn(__int2float_rn(d[0]), dw0), x0));
         acc[t][1] = __fadd_rn(acc[t][1], __fmul_rn(__fmul_rn(__int2float_rn(d[1]), dw0), x1));

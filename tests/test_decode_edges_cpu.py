@@ -20,6 +20,16 @@ def test_decoding_kernels_read_by_plain_loads(name):
     assert not re.findall(r"__ldg|__ldcs|ld\.global\.nc|__restrict__", code)
 
 
+@pytest.mark.parametrize("name,data", [("nq8_aux.cu", "x"), ("nq8_conv.cu", "x|cols"), ("nq8_qtiled.cu", r"xr|sx\d"), ("nq8_attention.cu", r"krel|p\.len|vrel"),
+                                       ("nq8_encoder_kernels.cu", "mel|len0|len1|len|len_in|in|u|qkv|krel|x|src|row")])
+def test_activations_and_lengths_are_read_by_plain_loads(name, data):
+    """The same for the other kernels; weights, which no kernel changes, may take the read-only path."""
+    with open(os.path.join(CSRC, name)) as f:
+        code = re.sub(r"//[^\n]*", "", f.read())
+    assert not re.findall(rf"const \w+ \*__restrict__ (?:{data})\b", code)
+    assert not re.findall(rf"__ldg\((?:reinterpret_cast<[^>]*>\()?(?:{data})\b", code)
+
+
 def test_one_beam_s_rows_may_lie_any_distance_apart():
     """Greedy decoding over a padded lm_head: with one beam its own stride means nothing.  The refusal left is the host tensor's."""
     from nspeech_b200.beam import beam_select
