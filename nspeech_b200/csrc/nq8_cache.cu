@@ -305,21 +305,12 @@ __global__ void __launch_bounds__(256) cache_write_kernel(const CacheView c, con
     const int x = threadIdx.x + 256 * i;
     if (x < all && place[x / units % ROWS] >= 0) put(x, kk[i], vv[i]);
   }
-  for (int x0 = threadIdx.x + 256 * U; x0 < all; x0 += 256 * U) {
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int x = x0 + 256 * i;
-      if (x < all && place[x / units % ROWS] >= 0) {
-        kk[i] = *source(k, k_ts, k_hs, k_ls, x);
-        vv[i] = *source(v, v_ts, v_hs, v_ls, x);
-      }
+#pragma unroll 1  // the other warps hide the loads; two units at a time took 276 us for 260 (the prompts above, whole passes)
+  for (int x = threadIdx.x + 256 * U; x < all; x += 256)
+    if (place[x / units % ROWS] >= 0) {
+      const T a = *source(k, k_ts, k_hs, k_ls, x), b = *source(v, v_ts, v_hs, v_ls, x);
+      put(x, a, b);
     }
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int x = x0 + 256 * i;
-      if (x < all && place[x / units % ROWS] >= 0) put(x, kk[i], vv[i]);
-    }
-  }
 }
 
 // Slots [first, first + n) become what the slots src[i] were.  A CTA owns a
