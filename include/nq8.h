@@ -316,7 +316,7 @@ int nq_conv_transpose1d(const nq_weight *w, const void *x, int x_dtype, int64_t 
  * src/moonshine/gpu_decoder.rs:21-88, and by the encoder,
  * src/moonshine/encoder.rs:116-135), the cache it reads (kv_cache_append) and
  * the choice of the next tokens (argmax_logits, src/moonshine/
- * gpu_decoder_metal.rs:110-243; beam_decode, src/parakeet/transducer.rs:1116).
+ * gpu_decoder_metal.rs:110-243).
  * Common rules:
  *   - All arrays are the caller's device memory; nothing is allocated and
  *     nothing is kept between calls, so every call may be captured into a
@@ -330,8 +330,8 @@ int nq_conv_transpose1d(const nq_weight *w, const void *x, int x_dtype, int64_t 
  *     lose 2^-20 of it at most.
  *   - Sequences are ragged: `offsets` (device int32 [n + 1], ascending) gives
  *     the rows of each; NULL: the same number of rows each.  Rows that belong
- *     to no sequence are neither read nor written.  Offsets and lengths are
- *     clamped to the rows there are. */
+ *     to no sequence are not written, and what they hold changes nothing.
+ *     Offsets and lengths are clamped to the rows there are. */
 
 /* Rows [token][head][head_dim]; unit stride within a head, the others in
  * elements.  Rows on 16 bytes (address, strides, head_dim) load fastest. */
@@ -353,11 +353,11 @@ typedef struct nq_rows {
  * batches); k_offsets / q_offsets NULL: k_rows / seqs (q_rows / seqs) rows
  * each.  K and V rows that no query of the call sees may hold anything; those
  * that one sees should be finite (a weight of 0 times an infinity is NaN; f32
- * below 2^127 in magnitude).
- * out must not overlap the inputs.  workspace (16-byte aligned, at least
+ * below 2^127 in magnitude).  A query that is NaN gives NaN.
+ * out may be q itself; otherwise it overlaps no input.  workspace (16-byte aligned, at least
  * nq_window_attention_workspace bytes; NULL: none) lets few query rows over
- * many keys be split over more of the GPU; results then differ by f32
- * summation order.  Deterministic. */
+ * many keys be split over more of the GPU (up to 64 pieces); results then
+ * differ by f32 summation order.  Deterministic. */
 int64_t nq_window_attention_workspace(int dtype, int seqs, int64_t q_rows, int64_t k_rows, int q_heads, int kv_heads,
                                       int head_dim, int left, int right, int sinks);
 int nq_window_attention(const nq_rows *q, const nq_rows *k, const nq_rows *v, const nq_rows *out, int dtype, int seqs,
@@ -411,7 +411,9 @@ int nq_cache_write(const nq_cache *c, const nq_rows *k, const nq_rows *v, int64_
  * with all its tokens as keys and the rows of q between offsets[i] and
  * offsets[i + 1] as its last tokens' queries.  A key whose page is gone
  * (nq_cache_trim) is not seen.  Single tokens (offsets NULL, q_rows = n) and
- * whole chunks of a prompt alike. */
+ * whole chunks of a prompt alike.  How the keys are split follows from what a
+ * slot may hold, max_pages * page_tokens: room far above the lengths there are
+ * costs time and workspace (pieces without keys, and their join). */
 int64_t nq_cache_attention_workspace(const nq_cache *c, int seqs, int64_t q_rows, int q_heads, int left, int right, int sinks);
 int nq_cache_attention(const nq_cache *c, int layer, const nq_rows *q, const nq_rows *out, int first, int n, int64_t q_rows,
                        const int32_t *offsets, int q_heads, int left, int right, int sinks, float scale, void *workspace,
@@ -447,7 +449,8 @@ int nq_cache_status(const nq_cache *c, int *bits, void *stream);
  * take), tokens, and whether they are finished (out_finished, may be NULL).
  * NaN and +inf logits count as -inf, as does a NaN score; a candidate of score
  * -inf is taken only after all others.  finished may be NULL; beams up to 32.
- * Outputs may be the inputs of the same kind.  Two launches. */
+ * Outputs may be the inputs of the same kind; otherwise they overlap neither
+ * inputs nor one another.  Two launches. */
 int64_t nq_beam_workspace(int items, int beams, int64_t vocab);
 int nq_beam_select(const void *logits, int dtype, int64_t ld, int items, int beams, int64_t vocab, const float *scores,
                    const uint8_t *finished, int eos, float *out_scores, int32_t *out_parents, int32_t *out_tokens,

@@ -37,8 +37,9 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: in
     Ragged batches: sequence b has the rows between ``q_offsets[b]`` and ``q_offsets[b + 1]`` (CUDA int32 [seqs + 1]),
     keys by ``k_offsets`` alike.  Without offsets each of `seqs` sequences (1 unless given) has as many rows.
     ``q_lens`` / ``k_lens`` (int32 [seqs]): only so many of a span's rows count, the others are padding.  Rows of no
-    sequence are left as they are in `out`; a query that sees no key gives zeros.  With `stream` the call runs as under
-    ``torch.cuda.stream(stream)``."""
+    sequence are left as they are in `out`, which may be q itself and otherwise overlaps no input; a query that sees no key
+    gives zeros, one that is NaN gives NaN.  There is no gradient: inputs that want one are refused unless gradients are
+    off.  With `stream` the call runs as under ``torch.cuda.stream(stream)``."""
     if stream is not None:
         with _on(stream, q):
             return window_attention(q, k, v, left, right, sinks, scale, q_offsets, k_offsets, q_lens, k_lens, seqs, out)

@@ -2,8 +2,8 @@
 
 One step takes the lm_head's logits of all beams, picks the best continuations by log probability, and says for each
 which row it comes from, so that ``PagedCache.fork`` and ``beam_reorder`` bring the beams' pages and recurrent states
-along.  One beam is greedy decoding (the reference's ``argmax_logits``, src/moonshine/gpu_decoder_metal.rs:110-243;
-its beam search is ``beam_decode``, src/parakeet/transducer.rs:1116).
+along.  One beam is greedy decoding (the reference's ``argmax_logits``, src/moonshine/gpu_decoder_metal.rs:110-243).  A
+transducer's search over tokens, durations and blanks (``beam_decode``, src/parakeet/transducer.rs:1116) is another one.
 """
 from __future__ import annotations
 
@@ -25,7 +25,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: Optional[t
 
     logits [items, beams, vocab] (f32 or bf16), scores f32 [items, beams] (sums of log probabilities; -inf for beams that
     do not exist yet), finished bool [items, beams]: a finished beam goes on only as itself, with token `eos` and its
-    score unchanged.  parents are rows of all items' beams (item * beams + beam).  Up to 32 beams."""
+    score unchanged.  parents are rows of all items' beams (item * beams + beam).  Up to 32 beams.  Rows may lie any even
+    distance apart (a padded lm_head).  `out` may hold the inputs of the same kind; otherwise outputs overlap nothing."""
     if stream is not None:
         with _on(stream, logits):
             return beam_select(logits, scores, finished, eos, out)

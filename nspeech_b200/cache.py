@@ -9,6 +9,9 @@ of its decoder's contiguous caches (src/moonshine/gpu_decoder.rs:21-88) for batc
 A decoding step: ``reserve`` once, then per layer ``write`` and ``attention``.  A call that cannot be done (no free
 pages, a full slot, a bad index) changes nothing, and the calls that change the cache do nothing after it, until
 ``check`` has raised it; attention goes on over what is there.
+
+Attention splits its keys by what a slot may hold, ``max_pages * page_tokens``, so take `max_pages` for the longest
+sequence that there will be, not for more.
 """
 from __future__ import annotations
 
@@ -26,7 +29,8 @@ _n = _l.native()
 
 class PagedCache:
     """Pages k, v [layers, pages, kv_heads, page_tokens, head_dim] (f32 or bf16), table int32 [slots, max_pages] (-1: no
-    page), lens int32 [slots], refs int32 [pages]: the caller's contiguous CUDA tensors, read and updated in place."""
+    page), lens int32 [slots], refs int32 [pages]: the caller's contiguous CUDA tensors, read and updated in place (autograd
+    does not see it)."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor):
         if k.dim() != 5 or k.shape != v.shape or k.dtype != v.dtype:

@@ -544,7 +544,8 @@ __global__ void __launch_bounds__(256) beam_gather_kernel(const __grid_constant_
 }
 
 // The same in place (or between any two): a CTA holds one strip of every row of one
-// state, and reads all rows before it writes any.
+// state, and reads all rows before it writes any.  512 rows of four states of 640
+// f32: 4.8 us in a stream (into other memory 2.9).
 template <typename T>
 __global__ void __launch_bounds__(256) beam_reorder_kernel(const __grid_constant__ ReorderParams p) {
   extern __shared__ __align__(16) uint8_t strip_raw[];

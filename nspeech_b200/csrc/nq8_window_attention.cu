@@ -1023,6 +1023,10 @@ WinAttnPlan win_attn_plan(int sm_count, int f32, bool tensor, bool uniform, int 
   pl.split_keys = tensor ? 1024 : rows_form ? 64 : 256;
   const int64_t most = keys / pl.split_keys;
   z = z < most ? z : most;
+  // The keys are what a sequence may have, not what it has (that is on the device):
+  // over a cache, what a slot has room for.  One token over 201 cached ones, 10
+  // heads of 64: room for 240 tokens 5.1 us, 1024 7.3 (two launches), 8192 9.8,
+  // 65536 12.9; of 64 sequences 11.9, 11.8, 25.7, 141.
   // Few rows over long contexts: pieces of 1024 keys (f32: 384), so that
   // sequences of unlike lengths keep all SMs busy to the end (64 sequences of
   // 2048 to 8192 tokens, 32/8 heads of 128: 258 us, pieces of 512 keys 281; f32,

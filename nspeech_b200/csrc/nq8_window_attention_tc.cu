@@ -25,9 +25,11 @@
 // flops (2048 clocks at DP = 128), the exponentials 2 x 128 x 128 at 16 a clock
 // (2048 clocks), and shared memory moves about as long (operands of QK^T 1024,
 // of PV 512, TMA 512).  Such a step takes about 3300 clocks.  16384 tokens, 16
-// query heads over 4 kv heads of 128, window 4096 and 4 sinks: 429 us, 0.67 of
-// the time of its flops at the measured 1666 TFLOP/s; the warp-level form takes
-// 2460 us.  On the way: registers limited for all code by a setmaxnreg ahead of
+// query heads over 4 kv heads of 128, window 4096 and 4 sinks: 430 us in bursts
+// of 20 calls at 1965 MHz, 0.67 of the time of its flops at the measured burst
+// rate of 1666 TFLOP/s; call after call, where the power cap holds the clock at
+// 1710 MHz, 497 us (0.58); the warp-level form takes 2460 us.  On the way, in
+// bursts: registers limited for all code by a setmaxnreg ahead of
 // the branches 661 us, MMAs issued by one lane of a divergent warp 471 us, a
 // quarter to three quarters of the exponentials on the FMA pipe 501 to 514 us.
 //
