@@ -460,7 +460,7 @@ int nq_beam_select(const void *logits, int dtype, int64_t ld, int items, int bea
  * 12288): row_bytes[i] bytes, src_stride[i] and dst_stride[i] bytes apart.  A
  * parent out of range stands for the row itself.  dst[i] may be src[i] (with
  * the same stride); an output that otherwise overlaps a state or another
- * output is refused.  One launch. */
+ * output is refused.  No output overlaps the parents.  One launch. */
 int nq_beam_reorder(const void *const *src, void *const *dst, const int64_t *row_bytes, const int64_t *src_stride,
                     const int64_t *dst_stride, int count, int rows, const int32_t *parents, void *stream);
 

@@ -37,7 +37,7 @@ def beam_reorder(states: Sequence[torch.Tensor], parents: torch.Tensor, out: Opt
                  stream: Optional[torch.cuda.Stream] = None) -> List[torch.Tensor]:
     """out[i][r] = states[i][parents[r]] for every state (any dtype, [rows, ...] with contiguous rows), in one launch for
     up to 16 states.  parents: int32, `rows` of them in any shape (``beam_select``'s); one out of range stands for the row
-    itself.  out[i] may be states[i], but overlaps no other state or output."""
+    itself.  out[i] may be states[i], but overlaps no other state or output, nor parents."""
     if stream is not None:
         with _on(stream, parents):
             return beam_reorder(states, parents, out)

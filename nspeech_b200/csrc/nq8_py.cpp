@@ -442,6 +442,8 @@ PyObject *beam_reorder(PyObject *const *a) {
   if (src.size() > kMost &&
       nq::reorder_overlaps(src.data(), dst.data(), bytes.data(), src_by.data(), dst_by.data(), static_cast<int>(src.size()), rows))
     misfit("an output overlaps another state");
+  for (size_t i = 0; i < dst.size(); ++i)
+    if (nq::overlap({dst[i], bytes[i], dst_by[i]}, {parents.data_ptr(), 4, 4}, rows)) misfit("an output overlaps the parents");
   for (size_t i = 0; i < src.size(); i += kMost)
     check(nq_beam_reorder(&src[i], &dst[i], &bytes[i], &src_by[i], &dst_by[i], static_cast<int>(std::min(kMost, src.size() - i)),
                           static_cast<int>(rows), static_cast<const int32_t *>(parents.data_ptr()), dev.stream()));

@@ -258,3 +258,18 @@ def test_attention_in_place_of_its_queries(dt, n, m, hq, hk, d):
     q, k, v = (torch.randn((r, h, d), generator=g).to(DT[dt]).cuda() for r, h in ((n, hq), (m, hk), (m, hk)))
     want = window_attention(q, k, v, 200, 0, 3)
     assert torch.equal(window_attention(q, k, v, 200, 0, 3, out=q), want)
+
+
+def test_beam_reorder_leaves_its_parents_alone():
+    from nspeech_b200.beam import beam_reorder
+    from nspeech_b200.fast_matmul import MatMulError
+    parents = torch.tensor([2, 0, 0, 1], dtype=torch.int32, device="cuda")
+    state = torch.arange(8, device="cuda").view(4, 2)
+    with pytest.raises(MatMulError, match="parents"):
+        beam_reorder([state, parents], parents, out=[state, parents])
+    many = [state.clone() for _ in range(17)]
+    with pytest.raises(MatMulError, match="parents"):
+        beam_reorder(many + [parents], parents, out=many + [parents])
+    assert all(torch.equal(t, state) for t in many) and parents.tolist() == [2, 0, 0, 1]
+    got = beam_reorder([state, parents], parents)  # they may be read as a state
+    assert got[1].tolist() == [0, 2, 2, 0] and torch.equal(got[0], state[parents.long()])
